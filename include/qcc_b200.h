@@ -46,6 +46,8 @@ extern "C" {
 #define QCC_DTYPE_BF16 0
 #define QCC_DTYPE_F16 1
 #define QCC_DTYPE_F32 2
+/* Output type of the block norms only: int8 with one fp32 scale a row. */
+#define QCC_DTYPE_I8 3
 /* Index types. */
 #define QCC_INDEX_I32 0
 #define QCC_INDEX_I64 1
@@ -520,6 +522,83 @@ QCC_API int qcc_indexed_ffn_prefill(const void* x, int64_t ldx, int n_tokens, in
                                     int64_t n_records, int dtype, const int32_t* tile_blocks,
                                     const int32_t* tile_offsets, void* workspace, size_t workspace_bytes, void* y,
                                     int64_t ldy, int y_dtype, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Norms before and after an FFN block, and int8 rows.
+ *
+ * N is the identity (QCC_NORM_NONE), the RMS norm
+ *   v * rsqrt(mean(v^2) + eps) * (weight_offset + weight) + bias
+ * or the layer norm
+ *   (v - mean(v)) * rsqrt(var(v) + eps) * (weight_offset + weight) + bias
+ * over a row's hidden values; weight (NULL: the factor is 1) and bias (NULL:
+ * 0) are [hidden] in param_dtype.  Statistics, products and sums are fp32 and
+ * each output is rounded once.  The reference leaves its models' norms to the
+ * host framework (end_to_end/model_patcher.py:12-33 replaces only the MLPs).
+ *
+ * Outputs of type QCC_DTYPE_I8 are int8 rows with one scale each:
+ *   row_scale[t] = amax / 127,  q = round_half_even(v * (127 / amax)),
+ * amax the row's largest magnitude.  A row with amax < 2^-119 gets scale 0
+ * and zeros; a row that holds a NaN or an infinity gets scale NaN and zeros,
+ * so that every product with it is NaN.
+ * ------------------------------------------------------------------------- */
+#define QCC_NORM_NONE 0
+#define QCC_NORM_RMS 1
+#define QCC_NORM_LAYER 2
+#define QCC_GATE_NONE 0
+#define QCC_GATE_SIGMOID 1
+#define QCC_GATE_TANH 2
+
+/* out[t] = N(x[t]) for the rows of x [rows, hidden] (row stride ldx >= hidden,
+ * elements) in dtype; out in out_dtype (bf16, fp16, fp32, or QCC_DTYPE_I8 with
+ * row_scale [rows]).  QCC_NORM_NONE with QCC_DTYPE_I8 quantises rows as they
+ * are.  out may be x itself (same type and stride).  hidden <= 32768.  Rows
+ * whose addresses are all multiples of 16 bytes take wide loads. */
+QCC_API int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, int kind, const void* weight,
+                          const void* bias, int param_dtype, float weight_offset, float eps, void* out,
+                          int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);
+
+/* The end of one block and the start of the next, per row t:
+ *   r = residual_scale * residual[t] + branch_scale * act(gate_t) * N_post(branch[t])
+ *   residual_out[t] = r,   out[t] = N_next(r)   (out NULL: residual_out only)
+ * with N_next taken from r before its rounding to residual_out.  branch is in
+ * dtype, residual and residual_out in residual_dtype (dtype or fp32), out in
+ * out_dtype as for qcc_norm_rows.  gate (NULL: 1): row t uses gate row
+ * t / gate_rows_each, of gate_cols values (1, or hidden), rows ld_gate apart
+ * (0: one row for all); act is the identity, the sigmoid or tanh.
+ * residual_out may be residual itself, and out may be branch itself (same
+ * type and stride).  hidden <= 32768.  One launch. */
+QCC_API int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtype, const void* residual,
+                              int64_t ld_residual, int residual_dtype, int rows, int hidden, int post_kind,
+                              const void* post_weight, const void* post_bias, int post_dtype, float post_offset,
+                              float post_eps, const void* gate, int64_t ld_gate, int gate_rows_each, int gate_cols,
+                              int gate_dtype, int gate_act, float residual_scale, float branch_scale,
+                              void* residual_out, int64_t ld_residual_out, int next_kind, const void* next_weight,
+                              const void* next_bias, int next_dtype, float next_offset, float next_eps, void* out,
+                              int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit integer products (the dense form of the FFN's projections).
+ *
+ * x [tokens, cols] and w [rows, cols] int8 (row strides ldx, ldw bytes:
+ * multiples of 16, as the base addresses are; bytes of a row past cols are
+ * ignored), x_scale [tokens] and w_scale [rows] fp32.  Sums are int32 and
+ * exact (cols <= 131071); the scales, the bias and silu are fp32; y [tokens,
+ * channels] (row stride ldy, elements) is rounded once to y_dtype.  tokens <=
+ * 2^20, channels <= 2^19.  The reference's dense projections run in the model's
+ * float type (runtime/ffn.py:11-17).
+ * ------------------------------------------------------------------------- */
+
+/* y[t, n] = (sum_k x[t, k] w[n, k]) * (x_scale[t] * w_scale[n]) + bias[n];
+ * bias (NULL: none) is [channels] in bias_dtype; w has `channels` rows. */
+QCC_API int qcc_int8_linear(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+                            const float* w_scale, const void* bias, int bias_dtype, int tokens, int channels,
+                            int cols, void* y, int64_t ldy, int y_dtype, cudaStream_t stream);
+
+/* y[t, n] = silu(g) * u: g the product of row n of w, u that of row channels + n
+ * (w has 2 * channels rows: the gate projection's, then the up projection's). */
+QCC_API int qcc_int8_gated_linear(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
+                                  const float* w_scale, int tokens, int channels, int cols, void* y, int64_t ldy,
+                                  int y_dtype, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

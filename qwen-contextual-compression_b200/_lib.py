@@ -16,6 +16,9 @@ _PACKAGE_DIR = Path(__file__).resolve().parent
 _LIBRARY_PATH = _PACKAGE_DIR / "libqcc_b200.so"
 
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+DTYPE_I8 = 3  # output type of the block norms: int8 with one fp32 scale a row
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_NONE, GATE_SIGMOID, GATE_TANH = 0, 1, 2
 INDEX_I32, INDEX_I64 = 0, 1
 IDS_READY = 0x100  # OR-ed into the index type: the ids are not written by an earlier qcc launch on the stream
 
@@ -32,6 +35,7 @@ TORCH_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.floa
 INDEX_DTYPES = {torch.int32: INDEX_I32, torch.int64: INDEX_I64}
 
 _c_void_p, _c_int, _c_int64, _c_size_t = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_c_float = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/qcc_b200.h
 SIGNATURES = {
@@ -97,6 +101,17 @@ SIGNATURES = {
     "qcc_indexed_ffn_prefill": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_void_p, _c_int64, _c_int,
                                          _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_int64, _c_int,
                                          _c_void_p]),
+    "qcc_norm_rows": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int,
+                               _c_float, _c_float, _c_void_p, _c_int64, _c_int, _c_void_p, _c_void_p]),
+    "qcc_residual_norm": (_c_int, [_c_void_p, _c_int64, _c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int,
+                                   _c_void_p, _c_void_p, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
+                                   _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
+                                   _c_void_p, _c_void_p, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
+                                   _c_void_p, _c_void_p]),
+    "qcc_int8_linear": (_c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int,
+                                 _c_int, _c_int, _c_int, _c_void_p, _c_int64, _c_int, _c_void_p]),
+    "qcc_int8_gated_linear": (_c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_void_p, _c_int,
+                                       _c_int, _c_int, _c_void_p, _c_int64, _c_int, _c_void_p]),
 }
 
 _lock = threading.Lock()
@@ -157,6 +172,22 @@ def dtype_code(dtype: torch.dtype) -> int:
         return TORCH_DTYPES[dtype]
     except KeyError:
         raise TypeError(f"unsupported dtype {dtype}; expected bfloat16, float16 or float32") from None
+
+
+def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise where autograd would expect a gradient: these entry points have no backward."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or detach its inputs")
+
+
+def on_device(device: torch.device, fn, *args) -> int:
+    """fn(*args) with `device` as the current device (a launch needs its stream's device to be current)."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
