@@ -4,12 +4,15 @@
 //   y[t, n]   = fp32(acc) * (xs[t] * ws[n]) + bias[n]     rounded once
 // and, for the gated form (wq holds the gate rows 0..N-1, then the up rows),
 //   y[t, n]   = silu(g) * u  with g, u the two products of channel n.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "qcc_common.cuh"
 #include "qcc_host.h"
+#include "qcc_tc.cuh"
 
 namespace qcc {
 namespace {
@@ -30,6 +33,7 @@ struct Int8Args {
   void* y;
   int64_t ldy;
   int y_dtype;
+  bool y_vec4 = false;  // y's rows take stores of four values
 };
 
 __device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
@@ -41,48 +45,284 @@ __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) 
   return static_cast<const float*>(bias)[n];
 }
 
-// One output a thread, 16 x 16 outputs a CTA, 64 columns of both operands in
-// shared memory at a time.
-template <bool GATED>
-__global__ void __launch_bounds__(256) int8_linear_kernel(const Int8Args a) {
-  constexpr int kStep = 64, kRow = kStep / 4 + 1;
-  constexpr int kParts = GATED ? 2 : 1;
-  __shared__ int xt[16 * kRow], wt[kParts * 16 * kRow];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int t0 = blockIdx.x * 16, n0 = blockIdx.y * 16;
-  int acc[kParts] = {};
-  for (int k0 = 0; k0 < a.cols; k0 += kStep) {
-    for (int i = threadIdx.x; i < 16 * (kStep / 4) * (1 + kParts); i += 256) {
-      const int part = i / (16 * (kStep / 4)), r = i / (kStep / 4) % 16, c = i % (kStep / 4);
-      const int8_t* base = part == 0 ? a.x : a.w;
-      const int64_t row = part == 0 ? t0 + r : n0 + r;
-      const bool in = part == 0 ? row < a.tokens : row < a.channels;
-      const int64_t at = part == 0 ? row * a.ldx : (row + (part - 1) * static_cast<int64_t>(a.channels)) * a.ldw;
-      uint32_t word = 0;
-      for (int b = 0; b < 4; ++b) {
-        const int k = k0 + c * 4 + b;
-        if (in && k < a.cols) word |= static_cast<uint32_t>(static_cast<uint8_t>(base[at + k])) << (8 * b);
-      }
-      (part == 0 ? xt : wt + (part - 1) * 16 * kRow)[r * kRow + c] = static_cast<int>(word);
-    }
-    __syncthreads();
-    for (int c = 0; c < kStep / 4; ++c)
-#pragma unroll
-      for (int p = 0; p < kParts; ++p) acc[p] = __dp4a(xt[ty * kRow + c], wt[(p * 16 + tx) * kRow + c], acc[p]);
-    __syncthreads();
-  }
-  const int t = t0 + ty, n = n0 + tx;
-  if (t >= a.tokens || n >= a.channels) return;
-  const float xs = a.xs[t];
-  float v = static_cast<float>(acc[0]) * (xs * a.ws[n]);
-  if (GATED)
-    v = silu(v) * (static_cast<float>(acc[kParts - 1]) * (xs * a.ws[a.channels + n]));
-  else
-    v += bias_value(a.bias, a.bias_dtype, n);
-  store_as(a.y, t * a.ldy + n, a.y_dtype, v);
+// ---------------------------------------------------------------------------
+// Stream kernel: one CTA computes 128 weight rows x BN tokens of the product
+// over its share of the columns.  The weight rows are the M operand of
+// tcgen05.mma kind::i8 (TMEM lanes), the tokens its N operand (TMEM columns),
+// so one decoded token costs 16 columns of N, not 128 rows of M.  A cluster of
+// S CTAs splits the columns; every CTA leaves its int32 partial sums in its own
+// shared memory, and the cluster adds them over distributed shared memory --
+// integer sums, so the split changes no bit of the result, and no workspace.
+// Gated: the 128 rows are 64 gate rows and the 64 up rows of the same channels.
+//
+// Waits are bounded; a tile whose wait ran out is written as NaN.
+// ---------------------------------------------------------------------------
+
+constexpr int kTileRows = 128;   // TMEM lanes
+constexpr int kTileCols = 128;   // bytes of K per stage (one swizzled row)
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+template <int BN, int STAGES>
+struct StreamSmem {
+  static constexpr int kWBytes = kTileRows * kTileCols, kXBytes = BN * kTileCols;
+  static constexpr int kStage = kWBytes + kXBytes;
+  static constexpr int kPartial = BN * kTileRows * 4;
+  static constexpr int kRing = STAGES * kStage;
+  static constexpr int kBody = kRing > kPartial ? kRing : kPartial;
+  static constexpr int kBytes = 1024 + kBody;  // ring aligned to 1024
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-int run_int8_linear(const Int8Args& a, bool gated, cudaStream_t stream) {
+__device__ __forceinline__ int4 cluster_load4(uint32_t smem, uint32_t rank) {
+  uint32_t remote;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int cluster_load1(uint32_t smem, uint32_t rank) {
+  uint32_t remote;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store4(const Int8Args& a, int t, int n, const float (&v)[4]) {
+  const int64_t at = static_cast<int64_t>(t) * a.ldy + n;
+  if (a.y_vec4 && n + 4 <= a.channels) {
+    if (a.y_dtype == QCC_DTYPE_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (a.y_dtype == QCC_DTYPE_BF16) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.y) + at) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(static_cast<__half*>(a.y) + at) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n + j < a.channels) store_as(a.y, at + j, a.y_dtype, v[j]);
+}
+
+template <bool GATED, int BN, int STAGES>
+__global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, const __grid_constant__ CUtensorMap tm_x,
+                                                          const __grid_constant__ CUtensorMap tm_w) {
+  using S = StreamSmem<BN, STAGES>;
+  constexpr int kChannels = GATED ? kTileRows / 2 : kTileRows;
+  constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[STAGES], empty[STAGES], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  uint32_t rank, splits;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const int n0 = static_cast<int>(blockIdx.x / splits) * kChannels, t0 = static_cast<int>(blockIdx.y) * BN;
+  const int blocks = (a.cols + kTileCols - 1) / kTileCols;
+  const int first = static_cast<int>(static_cast<int64_t>(blocks) * rank / splits);
+  const int count = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / splits) - first;
+
+  if (warp == 0) {
+    if (threadIdx.x == 0) {
+      tma_prefetch_map(&tm_x);
+      tma_prefetch_map(&tm_w);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(&done, 1);
+      failed = 0;
+      fence_barrier_init();
+    }
+  }
+  // Tensor memory is taken only once the launches ahead have finished: a CTA
+  // of theirs that still waits for its own columns must not wait for ours.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  if (threadIdx.x == 0) {
+    const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
+    int issued = 0;
+    for (; issued < count; ++issued) {
+      const int s = issued % STAGES;
+      if (issued >= STAGES && !mbar_wait_bounded(&empty[s], (issued / STAGES - 1) & 1, kWaitNs)) {
+        failed = 1;
+        break;
+      }
+      uint8_t* w = ring + s * S::kStage;
+      mbar_arrive_expect_tx(&full[s], S::kStage);
+      const int k = (first + issued) * kTileCols;
+      if (GATED) {
+        tma_load_2d_hint(w, &tm_w, k, n0, &full[s], stream);
+        tma_load_2d_hint(w + S::kWBytes / 2, &tm_w, k, a.channels + n0, &full[s], stream);
+      } else {
+        tma_load_2d_hint(w, &tm_w, k, n0, &full[s], stream);
+      }
+      tma_load_2d_hint(w + S::kWBytes, &tm_x, k, t0, &full[s], keep);
+    }
+    // A copy must not land after this CTA has gone: after a wait that ran out, see the issued ones in.
+    if (issued < count)
+      for (int i = issued - STAGES < 0 ? 0 : issued - STAGES; i < issued; ++i)
+        mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1, kWaitNs);
+  } else if (threadIdx.x == 32) {
+    constexpr uint32_t idesc = idesc_s8(kTileRows, BN);
+    for (int i = 0; i < count; ++i) {
+      const int s = i % STAGES;
+      if (!mbar_wait_bounded(&full[s], (i / STAGES) & 1, kWaitNs)) {
+        failed = 1;
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t w = smem_addr(ring + s * S::kStage);
+      const uint64_t wd = smem_desc_sw128(w, 16, 1024), xd = smem_desc_sw128(w + S::kWBytes, 16, 1024);
+#pragma unroll
+      for (int k = 0; k < kTileCols / 32; ++k)
+        tc_mma_i8(tmem, wd + k * 2, xd + k * 2, idesc, (i | k) != 0 ? 1u : 0u);
+      tc_commit(&empty[s]);
+    }
+    tc_commit(&done);
+  }
+  __syncwarp();
+  if (!mbar_wait_bounded(&done, 0, 4 * kWaitNs)) failed = 1;
+  tc_fence_after_sync();
+
+  // TMEM -> this CTA's shared memory as [token][row] int32 (the ring is free: every MMA has completed).
+  int* partial = reinterpret_cast<int*>(ring);
+  const int tokens = min(BN, a.tokens - t0);
+#pragma unroll 1
+  for (int c = 0; c < tokens; c += 16) {
+    float v[16];
+    tmem_load16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) partial[(c + j) * kTileRows + threadIdx.x] = count > 0 ? __float_as_int(v[j]) : 0;
+  }
+  tc_fence_before_sync();
+  cluster_sync();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+
+  // Sum over the cluster, scale and store: 4 channels of one token a thread at a time.
+  constexpr int kVecs = kChannels / 4;
+  const uint32_t base = smem_addr(partial);
+  int broken = 0;
+  for (uint32_t r = 0; r < splits; ++r) broken |= cluster_load1(smem_addr(&failed), r);
+  for (int i = static_cast<int>(rank) * 128 + static_cast<int>(threadIdx.x); i < tokens * kVecs;
+       i += 128 * static_cast<int>(splits)) {
+    const int t = i / kVecs, c = i % kVecs * 4;
+    int g[4] = {}, u[4] = {};
+    for (uint32_t r = 0; r < splits; ++r) {
+      const int4 p = cluster_load4(base + (t * kTileRows + c) * 4, r);
+      g[0] += p.x, g[1] += p.y, g[2] += p.z, g[3] += p.w;
+      if (GATED) {
+        const int4 q = cluster_load4(base + (t * kTileRows + kChannels + c) * 4, r);
+        u[0] += q.x, u[1] += q.y, u[2] += q.z, u[3] += q.w;
+      }
+    }
+    const float xs = a.xs[t0 + t];
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = min(n0 + c + j, a.channels - 1);
+      v[j] = static_cast<float>(g[j]) * (xs * a.ws[n]);
+      if (GATED)
+        v[j] = silu(v[j]) * (static_cast<float>(u[j]) * (xs * a.ws[a.channels + n]));
+      else
+        v[j] += bias_value(a.bias, a.bias_dtype, n);
+      if (broken) v[j] = NAN;
+    }
+    store4(a, t0 + t, n0 + c, v);
+  }
+  cluster_sync();  // the other CTAs have read this one's sums
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    cudaGetLastError();
+    return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+  }();
+  return fn;
+}
+
+// int8 rows [rows, cols], ld bytes apart, read in boxes of box_rows x 128 bytes (zeros outside).
+bool make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  auto fn = encode_tiled();
+  if (fn == nullptr) return false;
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld)};
+  const uint32_t box[2] = {kTileCols, static_cast<uint32_t>(box_rows)}, elem[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool GATED, int BN, int STAGES>
+int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
+  using S = StreamSmem<BN, STAGES>;
+  auto* kernel = int8_stream_kernel<GATED, BN, STAGES>;
+  CUtensorMap tm_x, tm_w;
+  const int64_t rows = GATED ? 2ll * a.channels : a.channels;
+  if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, BN) ||
+      !make_map(&tm_w, a.w, rows, a.cols, a.ldw, GATED ? kTileRows / 2 : kTileRows))
+    return QCC_ERR_UNSUPPORTED;
+  if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
+  const int channels = GATED ? kTileRows / 2 : kTileRows;
+  const int tiles = (a.channels + channels - 1) / channels, token_tiles = (a.tokens + BN - 1) / BN;
+  const int slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kBytes + 2048));
+  const int blocks = (a.cols + kTileCols - 1) / kTileCols;
+  const int split = std::max(1, std::min({8, blocks, static_cast<int>(slots / (static_cast<int64_t>(tiles) * token_tiles))}));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * split, token_tiles);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a, tm_x, tm_w)) ? QCC_OK : QCC_ERR_CUDA;
+}
+
+template <bool GATED>
+int launch(const Int8Args& a, int device, cudaStream_t stream) {
+  if (a.tokens <= 16) return launch_stream<GATED, 16, 4>(a, device, stream);
+  if (a.tokens <= 32) return launch_stream<GATED, 32, 4>(a, device, stream);
+  if (a.tokens <= 64) return launch_stream<GATED, 64, 4>(a, device, stream);
+  if (a.tokens <= 128) return launch_stream<GATED, 128, 3>(a, device, stream);
+  return launch_stream<GATED, 256, 4>(a, device, stream);
+}
+
+int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
   if (!valid_dtype(a.y_dtype) || (a.bias != nullptr && !valid_dtype(a.bias_dtype))) return QCC_ERR_DTYPE;
   if (a.tokens < 0 || a.channels < 1 || a.cols < 1 || a.ldx < a.cols || a.ldw < a.cols || a.ldy < a.channels)
     return QCC_ERR_SHAPE;
@@ -91,13 +331,11 @@ int run_int8_linear(const Int8Args& a, bool gated, cudaStream_t stream) {
   if (a.x == nullptr || a.xs == nullptr || a.w == nullptr || a.ws == nullptr || a.y == nullptr)
     return QCC_ERR_INVALID_ARGUMENT;
   if (!aligned16(a.x) || !aligned16(a.w) || a.ldx % 16 != 0 || a.ldw % 16 != 0) return QCC_ERR_ALIGNMENT;
-  const dim3 grid((a.tokens + 15) / 16, (a.channels + 15) / 16);
+  int device = 0;
+  if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
+  a.y_vec4 = reinterpret_cast<uintptr_t>(a.y) % (4 * dtype_bytes(a.y_dtype)) == 0 && a.ldy % 4 == 0;
   clear_stale_error();
-  if (gated)
-    int8_linear_kernel<true><<<grid, 256, 0, stream>>>(a);
-  else
-    int8_linear_kernel<false><<<grid, 256, 0, stream>>>(a);
-  return launch_ok() ? QCC_OK : QCC_ERR_CUDA;
+  return gated ? launch<true>(a, device, stream) : launch<false>(a, device, stream);
 }
 
 }  // namespace

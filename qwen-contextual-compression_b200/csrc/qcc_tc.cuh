@@ -1,7 +1,7 @@
 // Tensor-core (tcgen05 / TMEM) and tiled-TMA helpers for sm_100a kernels.
 //
 // Conventions used by the kernels of this library:
-// * operands are bf16 / fp16 (kind::f16) or fp32 (kind::tf32), staged in
+// * operands are bf16 / fp16 (kind::f16), fp32 (kind::tf32) or int8 (kind::i8), staged in
 //   shared memory by tiled TMA loads with the 128-byte swizzle: a box row is
 //   128 bytes (64 16-bit or 32 fp32 elements) and rows come in 1024-byte
 //   groups of eight; every operand tile starts on a 1024-byte boundary;
@@ -118,6 +118,18 @@ __device__ __forceinline__ void tc_mma_tf32(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
+// The same with kind::i8: A and B hold 8-bit integers, D 32-bit integers
+// (K = 32 per instruction, 32 bytes of a row as for kind::f16).
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // 32 consecutive fp32 columns of this thread's TMEM lane (32x32b shape: warp
 // w reads lanes 32*(w%4) .. +31).  The wait is inside the same statement, so
 // the registers are valid when it returns.
@@ -210,6 +222,14 @@ __host__ __device__ constexpr uint32_t idesc_f32acc(int m, int n, int fmt, bool 
   return (1u << 4) |                                                          // D format: f32
          (static_cast<uint32_t>(fmt) << 7) | (static_cast<uint32_t>(fmt) << 10) |  // A, B format
          ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor of tcgen05.mma kind::i8, signed A and B (both
+// K-major), 32-bit integer accumulation without saturation.
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
+  return (2u << 4) |               // D format: s32
+         (1u << 7) | (1u << 10) |  // A, B format: s8
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
