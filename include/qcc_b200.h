@@ -548,33 +548,51 @@ QCC_API int qcc_indexed_ffn_prefill(const void* x, int64_t ldx, int n_tokens, in
 #define QCC_GATE_SIGMOID 1
 #define QCC_GATE_TANH 2
 
+/* One norm: its parameters (device pointers) and constants. */
+typedef struct qcc_norm_params {
+  const void* weight; /* [hidden] in dtype, or NULL: the factor is 1 */
+  const void* bias;   /* [hidden] in dtype, or NULL: 0 */
+  int dtype;
+  int kind;
+  float weight_offset;
+  float eps;
+} qcc_norm_params;
+
+/* A gate: row t of the branch uses row t / rows_each of values, whose rows of
+ * cols values (1, or hidden) are ld elements apart (0: one row for all); act
+ * is applied to each value (the identity, the sigmoid or tanh). */
+typedef struct qcc_gate_params {
+  const void* values;
+  int64_t ld;
+  int rows_each;
+  int cols;
+  int dtype;
+  int act;
+} qcc_gate_params;
+
 /* out[t] = N(x[t]) for the rows of x [rows, hidden] (row stride ldx >= hidden,
  * elements) in dtype; out in out_dtype (bf16, fp16, fp32, or QCC_DTYPE_I8 with
- * row_scale [rows]).  QCC_NORM_NONE with QCC_DTYPE_I8 quantises rows as they
- * are.  out may be x itself (same type and stride).  hidden <= 32768.  Rows
- * whose addresses are all multiples of 16 bytes take wide loads. */
-QCC_API int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, int kind, const void* weight,
-                          const void* bias, int param_dtype, float weight_offset, float eps, void* out,
-                          int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);
+ * row_scale [rows]).  norm (host memory) NULL is the identity: with
+ * QCC_DTYPE_I8 it quantises rows as they are.  out may be x itself (same type
+ * and stride).  hidden <= 32768.  Rows whose addresses are all multiples of 16
+ * bytes take wide loads. */
+QCC_API int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, const qcc_norm_params* norm,
+                          void* out, int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);
 
 /* The end of one block and the start of the next, per row t:
  *   r = residual_scale * residual[t] + branch_scale * act(gate_t) * N_post(branch[t])
  *   residual_out[t] = r,   out[t] = N_next(r)   (out NULL: residual_out only)
  * with N_next taken from r before its rounding to residual_out.  branch is in
  * dtype, residual and residual_out in residual_dtype (dtype or fp32), out in
- * out_dtype as for qcc_norm_rows.  gate (NULL: 1): row t uses gate row
- * t / gate_rows_each, of gate_cols values (1, or hidden), rows ld_gate apart
- * (0: one row for all); act is the identity, the sigmoid or tanh.
- * residual_out may be residual itself, and out may be branch itself (same
- * type and stride).  hidden <= 32768.  One launch. */
+ * out_dtype as for qcc_norm_rows.  post, next and gate are in host memory; NULL
+ * is the identity.  residual_out may be residual itself, and out may be branch
+ * itself (same type and stride).  hidden <= 32768.  One launch. */
 QCC_API int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtype, const void* residual,
-                              int64_t ld_residual, int residual_dtype, int rows, int hidden, int post_kind,
-                              const void* post_weight, const void* post_bias, int post_dtype, float post_offset,
-                              float post_eps, const void* gate, int64_t ld_gate, int gate_rows_each, int gate_cols,
-                              int gate_dtype, int gate_act, float residual_scale, float branch_scale,
-                              void* residual_out, int64_t ld_residual_out, int next_kind, const void* next_weight,
-                              const void* next_bias, int next_dtype, float next_offset, float next_eps, void* out,
-                              int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);
+                              int64_t ld_residual, int residual_dtype, int rows, int hidden,
+                              const qcc_norm_params* post, const qcc_gate_params* gate, float residual_scale,
+                              float branch_scale, void* residual_out, int64_t ld_residual_out,
+                              const qcc_norm_params* next, void* out, int64_t ld_out, int out_dtype,
+                              float* row_scale, cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------
  * 8-bit integer products (the dense form of the FFN's projections).

@@ -37,6 +37,20 @@ INDEX_DTYPES = {torch.int32: INDEX_I32, torch.int64: INDEX_I64}
 _c_void_p, _c_int, _c_int64, _c_size_t = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 _c_float = ctypes.c_float
 
+
+
+class NormParams(ctypes.Structure):
+    """qcc_norm_params."""
+    _fields_ = [("weight", _c_void_p), ("bias", _c_void_p), ("dtype", _c_int), ("kind", _c_int),
+                ("weight_offset", _c_float), ("eps", _c_float)]
+
+
+class GateParams(ctypes.Structure):
+    """qcc_gate_params."""
+    _fields_ = [("values", _c_void_p), ("ld", _c_int64), ("rows_each", _c_int), ("cols", _c_int), ("dtype", _c_int),
+                ("act", _c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/qcc_b200.h
 SIGNATURES = {
     "qcc_version": (_c_int, []),
@@ -101,13 +115,11 @@ SIGNATURES = {
     "qcc_indexed_ffn_prefill": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_void_p, _c_int64, _c_int,
                                          _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_int64, _c_int,
                                          _c_void_p]),
-    "qcc_norm_rows": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int,
-                               _c_float, _c_float, _c_void_p, _c_int64, _c_int, _c_void_p, _c_void_p]),
-    "qcc_residual_norm": (_c_int, [_c_void_p, _c_int64, _c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int,
-                                   _c_void_p, _c_void_p, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
-                                   _c_int, _c_int, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
-                                   _c_void_p, _c_void_p, _c_int, _c_float, _c_float, _c_void_p, _c_int64, _c_int,
-                                   _c_void_p, _c_void_p]),
+    "qcc_norm_rows": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int64, _c_int,
+                               _c_void_p, _c_void_p]),
+    "qcc_residual_norm": (_c_int, [_c_void_p, _c_int64, _c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_void_p,
+                                   _c_void_p, _c_float, _c_float, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64,
+                                   _c_int, _c_void_p, _c_void_p]),
     "qcc_int8_linear": (_c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int,
                                  _c_int, _c_int, _c_int, _c_void_p, _c_int64, _c_int, _c_void_p]),
     "qcc_int8_gated_linear": (_c_int, [_c_void_p, _c_int64, _c_void_p, _c_void_p, _c_int64, _c_void_p, _c_int,
@@ -176,18 +188,26 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
     """Raise where autograd would expect a gradient: these entry points have no backward."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or detach its inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or detach its inputs")
 
 
-def on_device(device: torch.device, fn, *args) -> int:
-    """fn(*args) with `device` as the current device (a launch needs its stream's device to be current)."""
-    if torch.cuda.current_device() == device.index:
-        return fn(*args)
-    with torch.cuda.device(device):
-        return fn(*args)
+def launch(device_index: int, fn, *args) -> int:
+    """fn(*args, current stream of the device), with the device current (a launch needs its stream's device)."""
+    if _get_device() == device_index:
+        return fn(*args, _raw_stream(device_index))
+    with torch.cuda.device(device_index):
+        return fn(*args, _raw_stream(device_index))
+
+
+try:  # the raw queries avoid building a torch.cuda.Stream and the lazy-initialisation check per call
+    _raw_stream, _get_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+except AttributeError:  # pragma: no cover  (a torch build without CUDA)
+    def _raw_stream(device_index: int) -> int:
+        return torch.cuda.current_stream(device_index).cuda_stream
+
+    _get_device = torch.cuda.current_device
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

@@ -32,15 +32,6 @@ constexpr int kMaxHidden = kMaxThreads * kMaxVecs * 8;    // 32768
 // (and 127 / amax) would leave the normal fp32 range.
 constexpr float kSmallestAmax = 1.504632769052528e-36f;   // 2^-119
 
-struct NormArgs {
-  const void* weight;
-  const void* bias;
-  int dtype;
-  int kind;
-  float offset;
-  float eps;
-};
-
 struct BlockNormArgs {
   const void* y;
   int64_t ldy;
@@ -48,10 +39,8 @@ struct BlockNormArgs {
   int64_t ld_res;
   int rows, hidden;
   float residual_scale, branch_scale;
-  NormArgs post, next;
-  const void* gate;
-  int64_t ld_gate;
-  int gate_div, gate_cols, gate_dtype, gate_act;
+  qcc_norm_params post, next;
+  qcc_gate_params gate;  // values NULL: none
   void* res_out;
   int64_t ld_res_out;
   void* out;  // NULL: residual_out only
@@ -192,7 +181,7 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch) {
 
 // v <- N(v) over the row's `n` values (entries past the row are 0 on entry and on exit).
 template <int VPT, bool VEC>
-__device__ __forceinline__ void normalise(float (&v)[VPT][8], const NormArgs& a, int n, float* scratch) {
+__device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_params& a, int n, float* scratch) {
   if (a.kind == QCC_NORM_NONE) return;
   float mean = 0.f;
   if (a.kind == QCC_NORM_LAYER) {
@@ -220,7 +209,7 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const NormArgs& a,
     if (a.weight != nullptr) {
       load_any8<VEC>(a.weight, a.dtype, i, n, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * (a.offset + w[j]);
+      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * (a.weight_offset + w[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
@@ -250,15 +239,15 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const BlockNorm
   for (int i = 0; i < VPT; ++i) load_row8<T, VEC>(static_cast<const T*>(a.y) + t * a.ldy, i, n, v[i]);
   if (a.res != nullptr) {
     normalise<VPT, VEC>(v, a.post, n, scratch);
-    if (a.gate != nullptr) {
-      const size_t gs = a.gate_dtype == QCC_DTYPE_F32 ? 4 : 2;
-      const char* row = static_cast<const char*>(a.gate) + (t / a.gate_div) * a.ld_gate * gs;
-      if (a.gate_cols == 1) {
-        const float g = a.gate_dtype == QCC_DTYPE_BF16
+    if (a.gate.values != nullptr) {
+      const size_t gs = a.gate.dtype == QCC_DTYPE_F32 ? 4 : 2;
+      const char* row = static_cast<const char*>(a.gate.values) + (t / a.gate.rows_each) * a.gate.ld * gs;
+      if (a.gate.cols == 1) {
+        const float g = a.gate.dtype == QCC_DTYPE_BF16
                             ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(row))
-                        : a.gate_dtype == QCC_DTYPE_F16 ? __half2float(*reinterpret_cast<const __half*>(row))
+                        : a.gate.dtype == QCC_DTYPE_F16 ? __half2float(*reinterpret_cast<const __half*>(row))
                                                         : *reinterpret_cast<const float*>(row);
-        const float s = gate_value(g, a.gate_act);
+        const float s = gate_value(g, a.gate.act);
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
@@ -267,9 +256,9 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const BlockNorm
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           float g[8];
-          load_any8<VEC>(row, a.gate_dtype, i, n, g);
+          load_any8<VEC>(row, a.gate.dtype, i, n, g);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= gate_value(g[j], a.gate_act);
+          for (int j = 0; j < 8; ++j) v[i][j] *= gate_value(g[j], a.gate.act);
         }
       }
     }
@@ -320,7 +309,7 @@ bool row_vectors(const void* p, int64_t ld, int dtype_size) {
 
 int size_of(int dtype) { return dtype == QCC_DTYPE_I8 ? 1 : dtype_bytes(dtype); }
 
-bool norm_vectors(const NormArgs& a) { return row_vectors(a.weight, 0, 1) && row_vectors(a.bias, 0, 1); }
+bool norm_vectors(const qcc_norm_params& a) { return row_vectors(a.weight, 0, 1) && row_vectors(a.bias, 0, 1); }
 
 template <typename T, typename R>
 bool launch_block_norm(const BlockNormArgs& a, bool vec, cudaStream_t stream) {
@@ -342,17 +331,18 @@ bool launch_block_norm(const BlockNormArgs& a, bool vec, cudaStream_t stream) {
   return launch_ok();
 }
 
-bool valid_norm(int kind, const void* weight, const void* bias, int dtype) {
-  if (kind != QCC_NORM_NONE && kind != QCC_NORM_RMS && kind != QCC_NORM_LAYER) return false;
-  if (kind == QCC_NORM_NONE) return weight == nullptr && bias == nullptr;
-  return (weight == nullptr && bias == nullptr) || valid_dtype(dtype);
+bool valid_norm(const qcc_norm_params* p) {
+  if (p == nullptr) return true;
+  if (p->kind == QCC_NORM_NONE) return p->weight == nullptr && p->bias == nullptr;
+  return (p->kind == QCC_NORM_RMS || p->kind == QCC_NORM_LAYER) &&
+         ((p->weight == nullptr && p->bias == nullptr) || valid_dtype(p->dtype));
 }
 
 int run_block_norm(const BlockNormArgs& a, int dtype, int res_dtype, cudaStream_t stream) {
   const int es = dtype_bytes(dtype), rs = dtype_bytes(res_dtype);
   const bool vec = row_vectors(a.y, a.ldy, es) && row_vectors(a.res, a.ld_res, rs) &&
                    row_vectors(a.res_out, a.ld_res_out, rs) && norm_vectors(a.post) && norm_vectors(a.next) &&
-                   (a.gate_cols == 1 || row_vectors(a.gate, a.ld_gate, dtype_bytes(a.gate_dtype))) &&
+                   (a.gate.cols == 1 || row_vectors(a.gate.values, a.gate.ld, dtype_bytes(a.gate.dtype))) &&
                    row_vectors(a.out, a.ld_out, size_of(a.out_dtype));
   bool ok;
   if (dtype == QCC_DTYPE_BF16)
@@ -369,11 +359,10 @@ int run_block_norm(const BlockNormArgs& a, int dtype, int res_dtype, cudaStream_
 }  // namespace
 }  // namespace qcc
 
-extern "C" int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, int kind, const void* weight,
-                             const void* bias, int param_dtype, float weight_offset, float eps, void* out,
-                             int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream) {
+extern "C" int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, const qcc_norm_params* norm,
+                             void* out, int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream) {
   if (!qcc::valid_dtype(dtype) || !(qcc::valid_dtype(out_dtype) || out_dtype == QCC_DTYPE_I8)) return QCC_ERR_DTYPE;
-  if (!qcc::valid_norm(kind, weight, bias, param_dtype)) return QCC_ERR_INVALID_ARGUMENT;
+  if (!qcc::valid_norm(norm)) return QCC_ERR_INVALID_ARGUMENT;
   if (rows < 0 || hidden < 1 || ldx < hidden || ld_out < hidden) return QCC_ERR_SHAPE;
   if (hidden > qcc::kMaxHidden) return QCC_ERR_UNSUPPORTED;
   if (rows == 0) return QCC_OK;
@@ -384,9 +373,7 @@ extern "C" int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, in
   a.ldy = ldx;
   a.rows = rows;
   a.hidden = hidden;
-  a.next = {weight, bias, param_dtype, kind, weight_offset, eps};
-  a.gate_cols = 1;
-  a.gate_div = 1;
+  if (norm != nullptr) a.next = *norm;
   a.out = out;
   a.ld_out = ld_out;
   a.out_dtype = out_dtype;
@@ -395,24 +382,20 @@ extern "C" int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, in
 }
 
 extern "C" int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtype, const void* residual,
-                                 int64_t ld_residual, int residual_dtype, int rows, int hidden, int post_kind,
-                                 const void* post_weight, const void* post_bias, int post_dtype, float post_offset,
-                                 float post_eps, const void* gate, int64_t ld_gate, int gate_rows_each, int gate_cols,
-                                 int gate_dtype, int gate_act, float residual_scale, float branch_scale,
-                                 void* residual_out, int64_t ld_residual_out, int next_kind, const void* next_weight,
-                                 const void* next_bias, int next_dtype, float next_offset, float next_eps, void* out,
-                                 int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream) {
+                                 int64_t ld_residual, int residual_dtype, int rows, int hidden,
+                                 const qcc_norm_params* post, const qcc_gate_params* gate, float residual_scale,
+                                 float branch_scale, void* residual_out, int64_t ld_residual_out,
+                                 const qcc_norm_params* next, void* out, int64_t ld_out, int out_dtype,
+                                 float* row_scale, cudaStream_t stream) {
   if (!qcc::valid_dtype(dtype) || !(residual_dtype == dtype || residual_dtype == QCC_DTYPE_F32)) return QCC_ERR_DTYPE;
-  if (!qcc::valid_norm(post_kind, post_weight, post_bias, post_dtype) ||
-      !qcc::valid_norm(next_kind, next_weight, next_bias, next_dtype))
-    return QCC_ERR_INVALID_ARGUMENT;
+  if (!qcc::valid_norm(post) || !qcc::valid_norm(next)) return QCC_ERR_INVALID_ARGUMENT;
   if (rows < 0 || hidden < 1 || ld_branch < hidden || ld_residual < hidden || ld_residual_out < hidden)
     return QCC_ERR_SHAPE;
   if (gate != nullptr) {
-    if (!qcc::valid_dtype(gate_dtype)) return QCC_ERR_DTYPE;
-    if (gate_act != QCC_GATE_NONE && gate_act != QCC_GATE_SIGMOID && gate_act != QCC_GATE_TANH)
+    if (!qcc::valid_dtype(gate->dtype)) return QCC_ERR_DTYPE;
+    if (gate->act != QCC_GATE_NONE && gate->act != QCC_GATE_SIGMOID && gate->act != QCC_GATE_TANH)
       return QCC_ERR_INVALID_ARGUMENT;
-    if (gate_rows_each < 1 || (gate_cols != 1 && gate_cols != hidden) || ld_gate < 0) return QCC_ERR_SHAPE;
+    if (gate->rows_each < 1 || (gate->cols != 1 && gate->cols != hidden) || gate->ld < 0) return QCC_ERR_SHAPE;
   }
   if (out != nullptr) {
     if (!(qcc::valid_dtype(out_dtype) || out_dtype == QCC_DTYPE_I8)) return QCC_ERR_DTYPE;
@@ -421,7 +404,9 @@ extern "C" int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtyp
   }
   if (hidden > qcc::kMaxHidden) return QCC_ERR_UNSUPPORTED;
   if (rows == 0) return QCC_OK;
-  if (branch == nullptr || residual == nullptr || residual_out == nullptr) return QCC_ERR_INVALID_ARGUMENT;
+  if (branch == nullptr || residual == nullptr || residual_out == nullptr ||
+      (gate != nullptr && gate->values == nullptr))
+    return QCC_ERR_INVALID_ARGUMENT;
   qcc::BlockNormArgs a = {};
   a.y = branch;
   a.ldy = ld_branch;
@@ -431,14 +416,9 @@ extern "C" int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtyp
   a.hidden = hidden;
   a.residual_scale = residual_scale;
   a.branch_scale = branch_scale;
-  a.post = {post_weight, post_bias, post_dtype, post_kind, post_offset, post_eps};
-  a.next = {next_weight, next_bias, next_dtype, next_kind, next_offset, next_eps};
-  a.gate = gate;
-  a.ld_gate = ld_gate;
-  a.gate_div = gate == nullptr ? 1 : gate_rows_each;
-  a.gate_cols = gate == nullptr ? 1 : gate_cols;
-  a.gate_dtype = gate == nullptr ? QCC_DTYPE_F32 : gate_dtype;
-  a.gate_act = gate_act;
+  if (post != nullptr) a.post = *post;
+  if (next != nullptr) a.next = *next;
+  if (gate != nullptr) a.gate = *gate;
   a.res_out = residual_out;
   a.ld_res_out = ld_residual_out;
   a.out = out;

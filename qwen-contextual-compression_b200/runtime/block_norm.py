@@ -14,6 +14,8 @@ All arithmetic is fp32, each output is rounded once.  Forward only.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -23,44 +25,45 @@ GATES = {None: _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_T
 MAX_HIDDEN = 32768
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x [..., hidden] as rows [T, hidden], contiguous along hidden."""
+def _check_hidden(x: torch.Tensor, what: str) -> None:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} must be [..., hidden] with hidden >= 1, got {tuple(x.shape)}")
     if x.shape[-1] > MAX_HIDDEN:
         raise ValueError(f"{what} has {x.shape[-1]} values a row: at most {MAX_HIDDEN}")
+
+
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x [..., hidden] as rows [T, hidden] contiguous along hidden, and their stride."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 and x.shape[1] != 1 or x.stride(0) < x.shape[1]:
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
         x = x.contiguous()
-    return x
+    return x, x.stride(0)
 
 
-def _row_stride(x: torch.Tensor) -> int:
-    """The row stride the C entry points take (a single row's own stride says nothing)."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
-
-
-def _out_rows(out: torch.Tensor | None, shape: torch.Size, rows: int, dtype: torch.dtype, device: torch.device,
-              what: str) -> tuple[torch.Tensor, torch.Tensor]:
-    """(the tensor to return, its rows [T, hidden])."""
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-        return out, out.view(rows, shape[-1])
-    if out.shape != shape or out.dtype != dtype or out.device != device:
-        raise ValueError(f"{what} must be {tuple(shape)} in {dtype} on {device}")
+def _out_rows(out: torch.Tensor, shape: torch.Size, rows: int, dtype: torch.dtype, index: int, what: str) -> int:
+    """Checks a caller's output tensor; returns the stride of its rows."""
+    if out.shape != shape or out.dtype != dtype or out.get_device() != index:
+        raise ValueError(f"{what} must be {tuple(shape)} in {dtype} on the inputs' device")
+    hidden = shape[-1]
+    if out.is_contiguous():
+        return hidden
     try:
-        view = out.view(rows, shape[-1])
+        view = out.view(rows, hidden)
     except RuntimeError:
         view = None
-    if view is None or (view.stride(1) != 1 and shape[-1] != 1) or (rows > 1 and view.stride(0) < shape[-1]):
+    if view is None or (view.stride(1) != 1 and hidden != 1) or (rows > 1 and view.stride(0) < hidden):
         raise ValueError(f"{what} must be row-contiguous with rows one stride apart")
-    return out, view
+    return max(view.stride(0), hidden)
 
 
 def int8_rows(rows: int, cols: int, device: torch.device) -> torch.Tensor:
-    """Uninitialised int8 [rows, cols] whose rows start 16 bytes apart or a multiple of it."""
-    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :cols]
+    """Uninitialised int8 [rows, cols] whose rows start on multiples of 16 bytes."""
+    pad = -cols % 16
+    q = torch.empty((rows, cols + pad), dtype=torch.int8, device=device)
+    return q[:, :cols] if pad else q
 
 
 class BlockNorm:
@@ -73,8 +76,7 @@ class BlockNorm:
     for models that store the weight's difference from one.
     """
 
-    __slots__ = ("weight", "bias", "kind", "eps", "weight_offset", "hidden", "_kind", "_code", "_weight_ptr",
-                 "_bias_ptr", "device")
+    __slots__ = ("weight", "bias", "hidden", "_index", "_params", "_ref", "_pointers")
 
     def __init__(self, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, kind: str = "rms",
                  eps: float = 1e-6, weight_offset: float = 0.0):
@@ -84,63 +86,94 @@ class BlockNorm:
             raise ValueError("eps must be finite and not negative")
         if weight is None and weight_offset != 0.0:
             raise ValueError("weight_offset needs a weight")
-        params = [p for p in (weight, bias) if p is not None]
-        self.hidden, self.device, self._code = None, None, _lib.DTYPE_F32
-        if params:
-            self.device = _lib.require_cuda(*params)
-            if any(p.dim() != 1 or not p.is_contiguous() or p.shape != params[0].shape for p in params):
+        self.hidden, self._index, code = None, None, _lib.DTYPE_F32
+        for p in (weight, bias):
+            if p is None:
+                continue
+            if p.get_device() < 0:
+                _lib.require_cuda(p)
+            if p.dim() != 1 or not p.is_contiguous() or self.hidden not in (None, p.shape[0]):
                 raise ValueError("weight and bias must be contiguous one-dimensional tensors of one length")
-            if any(p.dtype != params[0].dtype for p in params):
+            self.hidden, self._index, code = p.shape[0], p.get_device(), _lib.dtype_code(p.dtype)
+        if weight is not None and bias is not None:
+            if weight.dtype != bias.dtype:
                 raise TypeError("weight and bias must share a dtype")
-            self._code = _lib.dtype_code(params[0].dtype)
-            self.hidden = params[0].shape[0]
-        self.weight, self.bias, self.kind, self.eps = weight, bias, kind, float(eps)
-        self.weight_offset = float(weight_offset)
-        self._kind = KINDS[kind]
+            _lib.require_cuda(weight, bias)
+        self.weight, self.bias = weight, bias
+        self._pointers = (_lib.ptr(weight), _lib.ptr(bias))
+        self._params = _lib.NormParams(*self._pointers, code, KINDS[kind], weight_offset, eps)
+        self._ref = ctypes.byref(self._params)
 
-    def args(self, x: torch.Tensor) -> tuple:
-        """The norm's C arguments for rows x, after its checks against them."""
+    @property
+    def kind(self) -> str:
+        return next(name for name, code in KINDS.items() if code == self._params.kind)
+
+    @property
+    def eps(self) -> float:
+        return self._params.eps
+
+    @property
+    def weight_offset(self) -> float:
+        return self._params.weight_offset
+
+    def _for(self, hidden: int, index: int):
+        """The norm as a C argument for rows of `hidden` values on a device, after its checks against them."""
         if self.hidden is not None:
-            if self.hidden != x.shape[-1]:
-                raise ValueError(f"the norm has {self.hidden} weights, its input {x.shape[-1]} values a row")
-            if self.device != x.device:
+            if self.hidden != hidden:
+                raise ValueError(f"the norm has {self.hidden} weights, its input {hidden} values a row")
+            if self._index != index:
                 raise RuntimeError("all tensors must share a device")
-        _lib.refuse_grad("BlockNorm", self.weight, self.bias)
-        return (self._kind, _lib.ptr(self.weight), _lib.ptr(self.bias), self._code, self.weight_offset, self.eps)
+            _lib.refuse_grad("BlockNorm", self.weight, self.bias)
+            pointers = (_lib.ptr(self.weight), _lib.ptr(self.bias))
+            if pointers != self._pointers:  # the parameters' storage was replaced
+                self._pointers = pointers
+                self._params.weight, self._params.bias = pointers
+        return self._ref
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
                  quantize: bool = False):
         """The normed rows of x [..., hidden]: a tensor like x (in out_dtype when given), or with
         ``quantize=True`` a pair (int8 [T, hidden] with rows padded to 16 bytes, fp32 scales [T]).
         ``out`` may be x itself."""
-        args = self.args(x)
-        return _run_norm(x, args, out, out_dtype, quantize)
+        return _run_norm(x, self, out, out_dtype, quantize)
 
 
-_NO_NORM = (_lib.NORM_NONE, None, None, _lib.DTYPE_F32, 0.0, 0.0)
-
-
-def _run_norm(x, args, out, out_dtype, quantize):
-    device = _lib.require_cuda(x)
+def _run_norm(x, norm, out, out_dtype, quantize):
+    index = x.get_device()
+    if index < 0:
+        _lib.require_cuda(x)
+    shape = x.shape
+    hidden = shape[-1] if shape else 0
+    if not 0 < hidden <= MAX_HIDDEN:
+        _check_hidden(x, "x")
     code = _lib.dtype_code(x.dtype)
-    _lib.refuse_grad("BlockNorm", x)
-    rows = _rows(x, "x")
-    t, hidden = rows.shape
-    scale = None
+    if x.requires_grad:
+        _lib.refuse_grad("BlockNorm", x)
+    norm_ref = None if norm is None else norm._for(hidden, index)
+    rows, ld = _rows(x)
+    t = x.numel() // hidden
+    scale, ld_out = None, hidden
     if quantize:
         if out is not None or out_dtype is not None:
             raise ValueError("quantize=True returns its own int8 rows: out and out_dtype do not apply")
-        out = out_rows = int8_rows(t, hidden, device)
-        scale = torch.empty(t, dtype=torch.float32, device=device)
+        out = int8_rows(t, hidden, x.device)
+        ld_out += -hidden % 16
+        scale = torch.empty(t, dtype=torch.float32, device=x.device)
         out_code = _lib.DTYPE_I8
+    elif out is None:
+        if out_dtype is None or out_dtype == x.dtype:
+            out_code = code
+            out = torch.empty_like(rows) if rows is x else x.new_empty(shape)
+        else:
+            out_code = _lib.dtype_code(out_dtype)
+            out = torch.empty(shape, dtype=out_dtype, device=x.device)
     else:
-        dtype = out_dtype or (x.dtype if out is None else out.dtype)
-        out_code = _lib.dtype_code(dtype)
-        out, out_rows = _out_rows(out, x.shape, t, dtype, device, "out")
+        out_dtype = out_dtype or out.dtype
+        out_code = _lib.dtype_code(out_dtype)
+        ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
     lib = _lib.library()
-    status = _lib.on_device(device, lib.qcc_norm_rows, rows.data_ptr(), _row_stride(rows), code, t, hidden, *args,
-                            out_rows.data_ptr(), _row_stride(out_rows), out_code, _lib.ptr(scale),
-                            _lib.stream_handle(device))
+    status = _lib.launch(index, lib.qcc_norm_rows, rows.data_ptr(), ld, code, t, hidden, norm_ref, out.data_ptr(),
+                         ld_out, out_code, None if scale is None else scale.data_ptr())
     if status:
         _lib.check(status, "qcc_norm_rows")
     return (out, scale) if quantize else out
@@ -154,33 +187,31 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     gets scale NaN and zeros, so every product with it is NaN.  The int8 rows
     are padded to a multiple of 16 bytes, as ``runtime.int8_dense`` wants them.
     """
-    return _run_norm(x, _NO_NORM, None, None, True)
+    return _run_norm(x, None, None, None, True)
 
 
-def _gate_args(gate: torch.Tensor | None, activation: str | None, shape: torch.Size) -> tuple:
-    """(gate kept alive, C arguments): the gate as rows of 1 or hidden values, each used by consecutive rows of x."""
-    if activation not in GATES:
-        raise ValueError(f"gate_activation must be one of {tuple(GATES)}")
-    if gate is None:
-        return None, (None, 0, 1, 1, _lib.DTYPE_F32, _lib.GATE_NONE)
+def _gate_params(gate: torch.Tensor, activation: str | None, shape: torch.Size):
+    """(gate rows, kept alive for the call; the gate as a C argument): rows of 1 or hidden values, each used by
+    consecutive rows of the branch."""
     code = _lib.dtype_code(gate.dtype)
     cols = gate.shape[-1] if gate.dim() else 1
-    lead = list(gate.shape[:-1])
-    x_lead = list(shape[:-1])
-    if cols not in (1, shape[-1]) or len(lead) > len(x_lead):
+    if cols != 1 and cols != shape[-1] or gate.dim() > len(shape):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
-    # Rows shared by the trailing leading axes (per sequence, or one row for all), full before them.
-    lead = [1] * (len(x_lead) - len(lead)) + lead
     each = 1
-    while lead and (lead[-1] == 1):
-        lead.pop()
-        each *= x_lead[len(lead)]
-    if lead != x_lead[:len(lead)]:
-        raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)} along its last axes")
-    rows = gate.reshape(-1, cols)
-    if rows.stride(1) != 1 or rows.stride(0) < cols:
+    if gate.shape[:-1] != shape[:-1]:
+        # Rows shared by the trailing leading axes (per sequence, or one row for all), full before them.
+        lead, x_lead = list(gate.shape[:-1]), list(shape[:-1])
+        lead = [1] * (len(x_lead) - len(lead)) + lead
+        while lead and lead[-1] == 1:
+            lead.pop()
+            each *= x_lead[len(lead)]
+        if lead != x_lead[:len(lead)]:
+            raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)} along its last axes")
+    rows = gate if gate.dim() == 2 else gate.reshape(-1, cols)
+    if rows.stride(1) != 1 and cols != 1:
         rows = rows.contiguous()
-    return rows, (rows.data_ptr(), rows.stride(0), max(each, 1), cols, code, GATES[activation])
+    return rows, ctypes.byref(_lib.GateParams(rows.data_ptr(), rows.stride(0), max(each, 1), cols, code,
+                                              GATES[activation]))
 
 
 def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNorm | None = None,
@@ -201,41 +232,58 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
     ``quantize=True``.  ``residual_out`` may be residual (in place) and ``out``
     branch; other overlaps of inputs and outputs are not supported.
     """
-    device = _lib.require_cuda(branch, residual, gate)
-    if residual.shape != branch.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} must have branch's shape {tuple(branch.shape)}")
-    code = _lib.dtype_code(branch.dtype)
-    if residual.dtype != branch.dtype and residual.dtype != torch.float32:
+    index = branch.get_device()
+    if index < 0 or residual.get_device() != index or (gate is not None and gate.get_device() != index):
+        _lib.require_cuda(branch, residual, gate)
+    shape = branch.shape
+    if residual.shape != shape:
+        raise ValueError(f"residual {tuple(residual.shape)} must have branch's shape {tuple(shape)}")
+    hidden = shape[-1] if shape else 0
+    if not 0 < hidden <= MAX_HIDDEN:
+        _check_hidden(branch, "branch")
+    code, res_code = _lib.dtype_code(branch.dtype), _lib.dtype_code(residual.dtype)
+    if res_code != code and res_code != _lib.DTYPE_F32:
         raise TypeError("residual must be in branch's dtype or float32")
-    _lib.refuse_grad("residual_norm", branch, residual, gate)
+    if gate_activation not in GATES:
+        raise ValueError(f"gate_activation must be one of {tuple(GATES)}")
     if next_norm is None and (quantize or out is not None or out_dtype is not None):
         raise ValueError("quantize, out and out_dtype need a next_norm")
-    shape = branch.shape
-    post_args = _NO_NORM if post is None else post.args(branch)
-    next_args = _NO_NORM if next_norm is None else next_norm.args(branch)
-    gate_rows, gate_args = _gate_args(gate, gate_activation, shape)
-    rows, res_rows = _rows(branch, "branch"), _rows(residual, "residual")
-    t, hidden = rows.shape
-    residual_out, res_out_rows = _out_rows(residual_out, shape, t, residual.dtype, device, "residual_out")
-    scale, out_ptr, ld_out, out_code = None, None, hidden, code
+    _lib.refuse_grad("residual_norm", branch, residual, gate)
+    post_ref = None if post is None else post._for(hidden, index)
+    next_ref = None if next_norm is None else next_norm._for(hidden, index)
+    gate_rows, gate_ref = (None, None) if gate is None else _gate_params(gate, gate_activation, shape)
+    rows, ld = _rows(branch)
+    res_rows, ld_res = _rows(residual)
+    t = branch.numel() // hidden
+    if residual_out is None:
+        residual_out = torch.empty_like(residual) if res_rows is residual else residual.new_empty(shape)
+        ld_res_out = hidden
+    else:
+        ld_res_out = _out_rows(residual_out, shape, t, residual.dtype, index, "residual_out")
+    scale_ptr, out_ptr, ld_out, out_code = None, None, hidden, code
     if next_norm is not None:
         if quantize:
             if out is not None or out_dtype is not None:
                 raise ValueError("quantize=True returns its own int8 rows: out and out_dtype do not apply")
-            out = out_rows = int8_rows(t, hidden, device)
-            scale = torch.empty(t, dtype=torch.float32, device=device)
-            out_code = _lib.DTYPE_I8
+            out = int8_rows(t, hidden, branch.device)
+            ld_out += -hidden % 16
+            scale = torch.empty(t, dtype=torch.float32, device=branch.device)
+            scale_ptr, out_code = scale.data_ptr(), _lib.DTYPE_I8
+        elif out is None:
+            if out_dtype is None or out_dtype == branch.dtype:
+                out = torch.empty_like(rows) if rows is branch else branch.new_empty(shape)
+            else:
+                out_code = _lib.dtype_code(out_dtype)
+                out = torch.empty(shape, dtype=out_dtype, device=branch.device)
         else:
-            dtype = out_dtype or (branch.dtype if out is None else out.dtype)
-            out_code = _lib.dtype_code(dtype)
-            out, out_rows = _out_rows(out, shape, t, dtype, device, "out")
-        out_ptr, ld_out = out_rows.data_ptr(), _row_stride(out_rows)
+            out_dtype = out_dtype or out.dtype
+            out_code = _lib.dtype_code(out_dtype)
+            ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
+        out_ptr = out.data_ptr()
     lib = _lib.library()
-    status = _lib.on_device(device, lib.qcc_residual_norm, rows.data_ptr(), _row_stride(rows), code,
-                            res_rows.data_ptr(), _row_stride(res_rows), _lib.dtype_code(residual.dtype), t, hidden,
-                            *post_args, *gate_args, float(residual_scale), float(branch_scale),
-                            res_out_rows.data_ptr(), _row_stride(res_out_rows), *next_args, out_ptr, ld_out, out_code,
-                            _lib.ptr(scale), _lib.stream_handle(device))
+    status = _lib.launch(index, lib.qcc_residual_norm, rows.data_ptr(), ld, code, res_rows.data_ptr(), ld_res,
+                         res_code, t, hidden, post_ref, gate_ref, residual_scale, branch_scale,
+                         residual_out.data_ptr(), ld_res_out, next_ref, out_ptr, ld_out, out_code, scale_ptr)
     if status:
         _lib.check(status, "qcc_residual_norm")
     if next_norm is None:

@@ -30,53 +30,62 @@ MAX_CHANNELS = 1 << 19
 
 def _int8_operand(q: torch.Tensor, scale: torch.Tensor, what: str) -> int:
     """Checks an int8 matrix with its row scales; returns the row stride."""
-    if q.dim() != 2 or q.dtype != torch.int8 or (q.stride(1) != 1 and q.shape[1] != 1):
-        raise ValueError(f"{what} must be a row-contiguous int8 matrix")
-    if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != q.shape[0] or not scale.is_contiguous():
+    if q.dim() != 2 or q.dtype != torch.int8:
+        raise ValueError(f"{what} must be an int8 matrix")
+    (rows, cols), (ld, step) = q.shape, q.stride()
+    if step != 1 and cols != 1:
+        raise ValueError(f"{what} must be contiguous along its columns")
+    if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != rows or not scale.is_contiguous():
         raise ValueError(f"the scales of {what} must be a contiguous float32 tensor with one value per row")
-    ld = q.stride(0) if q.shape[0] > 1 else (q.shape[1] + 15) // 16 * 16
-    if ld % 16 != 0 or q.data_ptr() % 16 != 0 or ld < q.shape[1]:
+    if rows <= 1:
+        ld = cols + -cols % 16
+    if ld % 16 or q.data_ptr() % 16 or ld < cols:
         raise ValueError(f"the rows of {what} must start on multiples of 16 bytes (quantize_rows stores them so)")
     return ld
 
 
 def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
     ldx, ldw = _int8_operand(xq, x_scale, "x"), _int8_operand(wq, w_scale, "w")
-    device = _lib.require_cuda(xq, x_scale, wq, w_scale, bias, out)
+    index = xq.get_device()
+    if (index < 0 or x_scale.get_device() != index or wq.get_device() != index or w_scale.get_device() != index
+            or (bias is not None and bias.get_device() != index) or (out is not None and out.get_device() != index)):
+        _lib.require_cuda(xq, x_scale, wq, w_scale, bias, out)
     tokens, cols = xq.shape
-    channels = wq.shape[0] // 2 if gated else wq.shape[0]
-    if wq.shape[1] != cols:
-        raise ValueError(f"x has {cols} columns, w {wq.shape[1]}")
-    if gated and wq.shape[0] % 2:
+    rows, w_cols = wq.shape
+    if w_cols != cols:
+        raise ValueError(f"x has {cols} columns, w {w_cols}")
+    if gated and rows % 2:
         raise ValueError("a gated weight has as many up rows as gate rows")
+    channels = rows // 2 if gated else rows
     if channels < 1 or cols < 1:
         raise ValueError("w must have rows and columns")
     if cols > MAX_COLS or tokens > MAX_TOKENS or channels > MAX_CHANNELS:
         raise ValueError(f"at most {MAX_TOKENS} tokens, {MAX_CHANNELS} channels and {MAX_COLS} columns")
     _lib.refuse_grad("the int8 product", x_scale, w_scale, bias)
-    out_dtype = out_dtype or (torch.bfloat16 if out is None else out.dtype)
-    y_code = _lib.dtype_code(out_dtype)
     if out is None:
-        out = torch.empty((tokens, channels), dtype=out_dtype, device=device)
-    elif (out.shape != (tokens, channels) or out.dtype != out_dtype or (out.stride(1) != 1 and channels != 1)
-          or (tokens > 1 and out.stride(0) < channels)):
-        raise ValueError("out must be a row-contiguous [tokens, channels] tensor of out_dtype")
-    ldy = out.stride(0) if tokens > 1 else max(out.stride(0), channels)
-    lib = _lib.library()
-    stream = _lib.stream_handle(device)
-    if gated:
-        status = _lib.on_device(device, lib.qcc_int8_gated_linear, xq.data_ptr(), ldx, x_scale.data_ptr(),
-                                wq.data_ptr(), ldw, w_scale.data_ptr(), tokens, channels, cols, out.data_ptr(), ldy,
-                                y_code, stream)
+        out_dtype = out_dtype or torch.bfloat16
+        y_code = _lib.dtype_code(out_dtype)
+        out = torch.empty((tokens, channels), dtype=out_dtype, device=xq.device)
+        ldy = channels
     else:
-        bias_code = _lib.DTYPE_F32
+        y_code = _lib.dtype_code(out.dtype)
+        if (out.shape != (tokens, channels) or (out_dtype or out.dtype) != out.dtype
+                or (out.stride(1) != 1 and channels != 1) or (tokens > 1 and out.stride(0) < channels)):
+            raise ValueError("out must be a row-contiguous [tokens, channels] tensor of out_dtype")
+        ldy = max(out.stride(0), channels)
+    lib = _lib.library()
+    if gated:
+        status = _lib.launch(index, lib.qcc_int8_gated_linear, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(),
+                             ldw, w_scale.data_ptr(), tokens, channels, cols, out.data_ptr(), ldy, y_code)
+    else:
+        bias_ptr, bias_code = None, _lib.DTYPE_F32
         if bias is not None:
-            if bias.shape != (channels,) or not bias.is_contiguous():
+            if bias.dim() != 1 or bias.shape[0] != channels or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous tensor with one value per channel")
-            bias_code = _lib.dtype_code(bias.dtype)
-        status = _lib.on_device(device, lib.qcc_int8_linear, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(),
-                                ldw, w_scale.data_ptr(), _lib.ptr(bias), bias_code, tokens, channels, cols,
-                                out.data_ptr(), ldy, y_code, stream)
+            bias_ptr, bias_code = bias.data_ptr(), _lib.dtype_code(bias.dtype)
+        status = _lib.launch(index, lib.qcc_int8_linear, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw,
+                             w_scale.data_ptr(), bias_ptr, bias_code, tokens, channels, cols, out.data_ptr(), ldy,
+                             y_code)
     if status:
         _lib.check(status, "qcc_int8_gated_linear" if gated else "qcc_int8_linear")
     return out

@@ -15,9 +15,13 @@ P = ctypes.c_void_p(64)
 BF16, F32, I8 = _lib.DTYPE_BF16, _lib.DTYPE_F32, _lib.DTYPE_I8
 
 
+def params(kind=_lib.NORM_RMS, weight=64, bias=None, dtype=BF16):
+    return ctypes.byref(_lib.NormParams(weight, bias, dtype, kind, 0.0, 1e-6))
+
+
 def norm_args(**changed):
-    a = dict(x=P, ldx=64, dtype=BF16, rows=2, hidden=64, kind=_lib.NORM_RMS, weight=P, bias=None, param=BF16,
-             offset=0.0, eps=1e-6, out=P, ld_out=64, out_dtype=BF16, scale=None, stream=None)
+    a = dict(x=P, ldx=64, dtype=BF16, rows=2, hidden=64, norm=params(), out=P, ld_out=64, out_dtype=BF16, scale=None,
+             stream=None)
     assert set(changed) <= set(a)
     a.update(changed)
     return list(a.values())
@@ -25,22 +29,24 @@ def norm_args(**changed):
 
 @pytest.mark.parametrize("changed,status", [
     (dict(dtype=7), _lib.ERR_DTYPE), (dict(dtype=I8), _lib.ERR_DTYPE), (dict(out_dtype=9), _lib.ERR_DTYPE),
-    (dict(kind=5), _lib.ERR_INVALID_ARGUMENT), (dict(param=8), _lib.ERR_INVALID_ARGUMENT),
-    (dict(kind=_lib.NORM_NONE), _lib.ERR_INVALID_ARGUMENT), (dict(rows=-1), _lib.ERR_SHAPE),
+    (dict(norm=params(kind=5)), _lib.ERR_INVALID_ARGUMENT), (dict(norm=params(dtype=8)), _lib.ERR_INVALID_ARGUMENT),
+    (dict(norm=params(kind=_lib.NORM_NONE)), _lib.ERR_INVALID_ARGUMENT), (dict(rows=-1), _lib.ERR_SHAPE),
     (dict(hidden=0), _lib.ERR_SHAPE), (dict(ldx=63), _lib.ERR_SHAPE), (dict(ld_out=63), _lib.ERR_SHAPE),
     (dict(hidden=32769, ldx=32769, ld_out=32769), _lib.ERR_UNSUPPORTED), (dict(x=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(out=None), _lib.ERR_INVALID_ARGUMENT), (dict(out_dtype=I8), _lib.ERR_INVALID_ARGUMENT),
-    (dict(rows=0, x=None, out=None), _lib.OK)])
+    (dict(rows=0, x=None, out=None, norm=None), _lib.OK)])
 def test_norm_rows_status(changed, status):
     assert _lib.library().qcc_norm_rows(*norm_args(**changed)) == status
 
 
+def gate(values=64, ld=1, each=1, cols=1, dtype=BF16, act=0):
+    return ctypes.byref(_lib.GateParams(values, ld, each, cols, dtype, act))
+
+
 def join_args(**changed):
     a = dict(branch=P, ld_branch=64, dtype=BF16, residual=P, ld_residual=64, residual_dtype=BF16, rows=2, hidden=64,
-             post_kind=0, post_weight=None, post_bias=None, post_dtype=BF16, post_offset=0.0, post_eps=0.0, gate=None,
-             ld_gate=0, each=1, cols=1, gate_dtype=BF16, gate_act=0, rscale=1.0, bscale=1.0, residual_out=P,
-             ld_residual_out=64, next_kind=0, next_weight=None, next_bias=None, next_dtype=BF16, next_offset=0.0,
-             next_eps=0.0, out=None, ld_out=0, out_dtype=BF16, scale=None, stream=None)
+             post=None, gate=None, rscale=1.0, bscale=1.0, residual_out=P, ld_residual_out=64, next=None, out=None,
+             ld_out=0, out_dtype=BF16, scale=None, stream=None)
     assert set(changed) <= set(a)
     a.update(changed)
     return list(a.values())
@@ -48,11 +54,12 @@ def join_args(**changed):
 
 @pytest.mark.parametrize("changed,status", [
     (dict(residual_dtype=_lib.DTYPE_F16), _lib.ERR_DTYPE), (dict(dtype=F32), _lib.ERR_DTYPE),
-    (dict(post_kind=4), _lib.ERR_INVALID_ARGUMENT), (dict(next_kind=-1), _lib.ERR_INVALID_ARGUMENT),
+    (dict(post=params(kind=4)), _lib.ERR_INVALID_ARGUMENT), (dict(next=params(kind=-1)), _lib.ERR_INVALID_ARGUMENT),
     (dict(ld_residual=60), _lib.ERR_SHAPE), (dict(ld_residual_out=60), _lib.ERR_SHAPE),
-    (dict(gate=P, gate_dtype=I8), _lib.ERR_DTYPE), (dict(gate=P, gate_act=3), _lib.ERR_INVALID_ARGUMENT),
-    (dict(gate=P, each=0), _lib.ERR_SHAPE), (dict(gate=P, cols=32), _lib.ERR_SHAPE),
-    (dict(gate=P, ld_gate=-1), _lib.ERR_SHAPE), (dict(out=P, ld_out=60), _lib.ERR_SHAPE),
+    (dict(gate=gate(dtype=I8)), _lib.ERR_DTYPE), (dict(gate=gate(act=3)), _lib.ERR_INVALID_ARGUMENT),
+    (dict(gate=gate(each=0)), _lib.ERR_SHAPE), (dict(gate=gate(cols=32)), _lib.ERR_SHAPE),
+    (dict(gate=gate(ld=-1)), _lib.ERR_SHAPE), (dict(gate=gate(values=None)), _lib.ERR_INVALID_ARGUMENT),
+    (dict(out=P, ld_out=60), _lib.ERR_SHAPE),
     (dict(out=P, ld_out=64, out_dtype=I8), _lib.ERR_INVALID_ARGUMENT), (dict(residual=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(residual_out=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(hidden=40000, ld_branch=40000, ld_residual=40000, ld_residual_out=40000), _lib.ERR_UNSUPPORTED),
