@@ -72,10 +72,6 @@ struct StreamSmem {
   static constexpr int kBytes = 1024 + kBody;  // ring aligned to 1024
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 __device__ __forceinline__ int4 cluster_load4(uint32_t smem, uint32_t rank) {
   uint32_t remote;
   int4 v;
@@ -256,6 +252,206 @@ __global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, cons
   cluster_sync();  // the other CTAs have read this one's sums
 }
 
+// ---------------------------------------------------------------------------
+// Pair kernel: persistent CTA pairs (cta_group::2), tiles of 256 weight rows x
+// up to 256 tokens over all columns, for token counts that make the product
+// compute bound.  Warp 0 loads, warp 1 of the even CTA issues the MMAs, warps
+// 2-5 drain the accumulators; two accumulators (2 x 256 of the 512 TMEM
+// columns) let a tile's epilogue run beside the next tile's MMAs.  A pair reads
+// each operand byte of its tile once (128 rows of each per CTA), half of what
+// two single CTAs would.
+// Gated: the rows of a tile alternate 16 gate and 16 up rows, so that lane l
+// of a warp holds the gate and lane l + 16 the up product of one channel and
+// one shuffle brings two tokens' pairs together.
+// ---------------------------------------------------------------------------
+
+constexpr int kPairStages = 6;
+constexpr int kPairTokens = 256;                       // most tokens of a tile
+constexpr int kPairStage = 2 * 128 * kTileCols;        // bytes a CTA loads per stage, at most
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage;
+constexpr int kPairThreads = 192;
+
+struct PairPlan {
+  int row_tiles, token_tiles, tile_tokens;  // tile_tokens: multiple of 32, up to kPairTokens
+  int group;                                // token tiles that are walked through together
+};
+
+// Tile i of the walk: groups of `group` token tiles, within a group the token tiles of one row tile next to each
+// other, so that concurrent pairs share weight rows and a group's tokens stay in L2.
+__device__ __forceinline__ void pair_tile(const PairPlan& p, int i, int& row, int& token) {
+  const int per_group = p.group * p.row_tiles;
+  const int g = i / per_group, in = i - g * per_group;
+  const int width = min(p.group, p.token_tiles - g * p.group);
+  row = in / width;
+  token = g * p.group + in - row * width;
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    int8_pair_kernel(const Int8Args a, const PairPlan plan, const __grid_constant__ CUtensorMap tm_x,
+                     const __grid_constant__ CUtensorMap tm_w) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int failed;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = plan.row_tiles * plan.token_tiles;
+  const int blocks = (a.cols + kTileCols - 1) / kTileCols;
+  const int half_tokens = plan.tile_tokens / 2;
+  constexpr int kChannels = GATED ? 128 : 256;  // output channels of a tile, half of them in each CTA
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&tm_x);
+    tma_prefetch_map(&tm_w);
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 8);  // the four epilogue warps of both CTAs
+    }
+    failed = 0;
+    fence_barrier_init();
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // before tensor memory is taken, as in the stream kernel
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  if (threadIdx.x == 0) {
+    const uint64_t keep = policy_evict_last();
+    int n = 0;  // stage uses so far
+    bool ok = true;
+    for (int i = pair; i < tiles && ok; i += pairs) {
+      int row, token;
+      pair_tile(plan, i, row, token);
+      for (int b = 0; b < blocks; ++b, ++n) {
+        const int s = n % kPairStages;
+        if (n >= kPairStages && !mbar_wait_bounded(&empty[s], (n / kPairStages - 1) & 1, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        uint8_t* w = ring + s * kPairStage;
+        const uint32_t bar = cluster_addr(&full[s], 0);
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (128 + half_tokens) * kTileCols);
+        const int k = b * kTileCols;
+        if (GATED) {
+          const int n0 = row * kChannels + static_cast<int>(rank) * 64;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            tma_load_2d_pair(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, bar, keep);
+            tma_load_2d_pair(w + (q * 32 + 16) * kTileCols, &tm_w, k, a.channels + n0 + q * 16, bar, keep);
+          }
+        } else {
+          tma_load_2d_pair(w, &tm_w, k, row * kChannels + static_cast<int>(rank) * 128, bar, keep);
+        }
+        tma_load_2d_pair(w + 128 * kTileCols, &tm_x, k, token * plan.tile_tokens + static_cast<int>(rank) * half_tokens,
+                         bar, keep);
+      }
+    }
+    if (!ok) {
+      failed = 1;
+      // Copies in flight land before the cluster's last barrier: the even CTA's barriers count both CTAs' bytes.
+      if (rank == 0)
+        for (int i = max(0, n - kPairStages); i < n; ++i)
+          mbar_wait_bounded(&full[i % kPairStages], (i / kPairStages) & 1, kWaitNs);
+    }
+  } else if (threadIdx.x == 32 && rank == 0) {
+    const uint32_t idesc = idesc_s8(256, plan.tile_tokens);
+    int n = 0, done = 0;
+    bool ok = true;
+    for (int i = pair; i < tiles && ok; i += pairs, ++done) {
+      const int acc = done & 1;
+      if (done >= 2 && !mbar_wait_bounded(&acc_empty[acc], (done / 2 - 1) & 1, kWaitNs)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      for (int b = 0; b < blocks; ++b, ++n) {
+        const int s = n % kPairStages;
+        if (!mbar_wait_bounded(&full[s], (n / kPairStages) & 1, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t w = smem_addr(ring + s * kPairStage);
+        const uint64_t wd = smem_desc_sw128(w, 16, 1024), xd = smem_desc_sw128(w + 128 * kTileCols, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < kTileCols / 32; ++k)
+          tc_mma_i8_pair(tmem + acc * 256, wd + k * 2, xd + k * 2, idesc, (b | k) != 0 ? 1u : 0u);
+        tc_commit_pair(&empty[s]);
+      }
+      tc_commit_pair(&acc_full[acc]);
+    }
+    if (!ok) failed = 1;
+  } else if (warp >= 2) {
+    const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
+    int done = 0;
+    for (int i = pair; i < tiles; i += pairs, ++done) {
+      const int acc = done & 1;
+      if (failed || !mbar_wait_bounded(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) failed = 1;
+      tc_fence_after_sync();
+      int row, token;
+      pair_tile(plan, i, row, token);
+      const int t0 = token * plan.tile_tokens, tokens = min(plan.tile_tokens, a.tokens - t0);
+      const int n = row * kChannels + static_cast<int>(rank) * (kChannels / 2) +
+                    (GATED ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
+      const bool in = n < a.channels;
+      const int wrow = GATED && lane >= 16 ? a.channels + n : n;
+      const float ws = in ? a.ws[wrow] : 0.f;
+      const float bias = !GATED && in ? bias_value(a.bias, a.bias_dtype, n) : 0.f;
+      const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
+      for (int c = 0; c < tokens; c += 32) {
+        float v[32];
+        tmem_load32(from + c, v);
+        const float xs = c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
+        if (c + 32 >= tokens) {  // the accumulator's last columns are in registers
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[acc], 0));
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          v[j] = static_cast<float>(__float_as_int(v[j])) * (__shfl_sync(0xffffffffu, xs, j) * ws);
+        if (GATED) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            // Lanes 0-15 finish token j, lanes 16-31 token j + 1.
+            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[j + 1] : v[j], 16);
+            float h = silu(lane < 16 ? v[j] : other) * (lane < 16 ? other : v[j + 1]);
+            if (failed) h = NAN;
+            const int t = c + j + (lane >> 4);
+            if (in && t < tokens) store_as(a.y, static_cast<int64_t>(t0 + t) * a.ldy + n, a.y_dtype, h);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float y = v[j] + bias;
+            if (failed) y = NAN;
+            if (in && c + j < tokens) store_as(a.y, static_cast<int64_t>(t0 + c + j) * a.ldy + n, a.y_dtype, y);
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync();  // no barrier of this CTA is signalled and none of its memory read after this
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
@@ -313,13 +509,58 @@ int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
   return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a, tm_x, tm_w)) ? QCC_OK : QCC_ERR_CUDA;
 }
 
+// The token width of a tile: the one that needs the fewest columns of MMA work in the longest-running pair.
+int pair_tile_tokens(int tokens, int row_tiles, int pairs) {
+  int best = kPairTokens;
+  int64_t best_cost = INT64_MAX;
+  for (int width = kPairTokens; width >= 128; width -= 32) {
+    const int64_t tiles = static_cast<int64_t>(row_tiles) * ((tokens + width - 1) / width);
+    const int64_t cost = (tiles + pairs - 1) / pairs * width;
+    if (cost < best_cost) best = width, best_cost = cost;
+  }
+  return best;
+}
+
+template <bool GATED>
+int launch_pair(const Int8Args& a, int device, cudaStream_t stream) {
+  auto* kernel = int8_pair_kernel<GATED>;
+  const int channels = GATED ? 128 : 256;
+  const int pairs = device_info(device).num_sms / 2;
+  PairPlan plan;
+  plan.row_tiles = (a.channels + channels - 1) / channels;
+  plan.tile_tokens = pair_tile_tokens(a.tokens, plan.row_tiles, pairs);
+  plan.token_tiles = (a.tokens + plan.tile_tokens - 1) / plan.tile_tokens;
+  plan.group = 8;
+  CUtensorMap tm_x, tm_w;
+  if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, plan.tile_tokens / 2) ||
+      !make_map(&tm_w, a.w, GATED ? 2ll * a.channels : a.channels, a.cols, a.ldw, GATED ? 16 : 128))
+    return QCC_ERR_UNSUPPORTED;
+  if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(pairs, static_cast<int64_t>(plan.row_tiles) *
+                                                                            plan.token_tiles)));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a, plan, tm_x, tm_w)) ? QCC_OK : QCC_ERR_CUDA;
+}
+
 template <bool GATED>
 int launch(const Int8Args& a, int device, cudaStream_t stream) {
   if (a.tokens <= 16) return launch_stream<GATED, 16, 4>(a, device, stream);
   if (a.tokens <= 32) return launch_stream<GATED, 32, 4>(a, device, stream);
   if (a.tokens <= 64) return launch_stream<GATED, 64, 4>(a, device, stream);
   if (a.tokens <= 128) return launch_stream<GATED, 128, 3>(a, device, stream);
-  return launch_stream<GATED, 256, 4>(a, device, stream);
+  return launch_pair<GATED>(a, device, stream);
 }
 
 int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
