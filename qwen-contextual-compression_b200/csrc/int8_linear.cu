@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "qcc_common.cuh"
 #include "qcc_host.h"
@@ -33,10 +34,12 @@ struct Int8Args {
   void* y;
   int64_t ldy;
   int y_dtype;
-  bool y_vec4 = false;  // y's rows take stores of four values
 };
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + expf(-g)); }
+// silu with the fast exponential and quotient: exp's argument rounds once (an
+// error of |g| roundings in exp), exp and the quotient are off by 2 ulp each.
+// Below g = -87.3 the quotient, under 2^-119, becomes 0.
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
 __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) {
   if (bias == nullptr) return 0.f;
@@ -46,44 +49,91 @@ __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) 
 }
 
 // ---------------------------------------------------------------------------
-// Stream kernel: one CTA computes 128 weight rows x BN tokens of the product
-// over its share of the columns.  The weight rows are the M operand of
-// tcgen05.mma kind::i8 (TMEM lanes), the tokens its N operand (TMEM columns),
-// so one decoded token costs 16 columns of N, not 128 rows of M.  A cluster of
-// S CTAs splits the columns; every CTA leaves its int32 partial sums in its own
-// shared memory, and the cluster adds them over distributed shared memory --
-// integer sums, so the split changes no bit of the result, and no workspace.
-// Gated: the 128 rows are 64 gate rows and the 64 up rows of the same channels.
-//
+// Both kernels keep weight rows in TMEM lanes (the M operand of tcgen05.mma
+// kind::i8) and tokens in TMEM columns (the N operand), so one decoded token
+// costs 16 columns of N, not 128 rows of M.  Lane l of a warp finishes one
+// weight row's products with a run of tokens; a warp's store of one token is
+// 32 consecutive channels.
+// Gated: 32 lanes are 16 gate rows and the up rows of the same 16 channels, so
+// one shuffle brings two tokens' gate and up together and every lane has one
+// output of the two to finish.
 // Waits are bounded; a tile whose wait ran out is written as NaN.
 // ---------------------------------------------------------------------------
 
-constexpr int kTileRows = 128;   // TMEM lanes
-constexpr int kTileCols = 128;   // bytes of K per stage (one swizzled row)
+constexpr int kTileRows = 128;  // weight rows of a CTA's tile: TMEM lanes
+constexpr int kTileCols = 128;  // bytes of K per stage (one swizzled row)
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-template <int BN, int STAGES>
-struct StreamSmem {
-  static constexpr int kWBytes = kTileRows * kTileCols, kXBytes = BN * kTileCols;
-  static constexpr int kStage = kWBytes + kXBytes;
-  static constexpr int kPartial = BN * kTileRows * 4;
-  static constexpr int kRing = STAGES * kStage;
-  static constexpr int kBody = kRing > kPartial ? kRing : kPartial;
-  static constexpr int kBytes = 1024 + kBody;  // ring aligned to 1024
+// What one lane needs to finish its weight row's outputs.
+template <bool GATED, typename O>
+struct RowOutput {
+  O* y;  // the first token's output of this lane's channel
+  int64_t ldy;
+  float ws, ws_up, bias;
+  bool in;  // the channel exists
+
+  // row0: the first weight row (gated: channel) of the 32-lane group.  A tile whose wait ran out is `broken`: its
+  // scales become NaN, and so do its outputs.
+  __device__ __forceinline__ RowOutput(const Int8Args& a, int row0, int t0, int lane, bool broken) {
+    const int n = row0 + (GATED ? lane & 15 : lane);
+    in = n < a.channels;
+    ldy = a.ldy;
+    y = static_cast<O*>(a.y) + static_cast<int64_t>(t0) * a.ldy + n;
+    ws = broken ? NAN : in ? a.ws[n] : 0.f;
+    ws_up = GATED && in ? a.ws[a.channels + n] : 0.f;
+    bias = !GATED && in ? bias_value(a.bias, a.bias_dtype, n) : 0.f;
+  }
+
+  // Finishes tokens c .. c + J - 1 (those below `tokens`) from their sums; lane j holds token c + j's scale.
+  template <int J>
+  __device__ __forceinline__ void finish(const int (&acc)[J], int c, int tokens, float xs, int lane) const {
+    O* to = y + static_cast<int64_t>(c) * ldy;
+    if (GATED) {
+      // Lanes 0-15 finish the even tokens, lanes 16-31 the odd ones.
+      const bool low = lane < 16;
+      if (!low) to += ldy;
+      const int left = in ? tokens - c - (low ? 0 : 1) : 0;
+#pragma unroll
+      for (int j = 0; j < J; j += 2) {
+        const int other = __shfl_xor_sync(0xffffffffu, low ? acc[j + 1] : acc[j], 16);
+        const float scale = __shfl_sync(0xffffffffu, xs, j + (low ? 0 : 1));
+        const float g = static_cast<float>(low ? acc[j] : other) * (scale * ws);
+        const float u = static_cast<float>(low ? other : acc[j + 1]) * (scale * ws_up);
+        if (j < left) *to = static_cast<O>(silu(g) * u);
+        to += 2 * ldy;
+      }
+    } else {
+      const int left = in ? tokens - c : 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float v = static_cast<float>(acc[j]) * (__shfl_sync(0xffffffffu, xs, j) * ws);
+        if (j < left) *to = static_cast<O>(v + bias);
+        to += ldy;
+      }
+    }
+  }
 };
 
-__device__ __forceinline__ int4 cluster_load4(uint32_t smem, uint32_t rank) {
-  uint32_t remote;
-  int4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(remote)
-               : "memory");
-  return v;
-}
+// ---------------------------------------------------------------------------
+// Stream kernel: one CTA computes 128 weight rows x BN tokens over its share of
+// the columns; bound by the weight's bytes.  A cluster of S CTAs splits the
+// columns when there are few rows: every CTA leaves its int32 partial sums in
+// its own shared memory, and the cluster adds them over distributed shared
+// memory -- integer sums, so the split changes no bit of the result, and there
+// is no workspace that two calls could share.
+// ---------------------------------------------------------------------------
 
-__device__ __forceinline__ int cluster_load1(uint32_t smem, uint32_t rank) {
+template <int BN, int STAGES>
+struct StreamShape {
+  static constexpr int kWBytes = kTileRows * kTileCols, kXBytes = BN * kTileCols;
+  static constexpr int kStage = kWBytes + kXBytes;
+  static constexpr int kRing = STAGES * kStage;
+  static_assert(BN * kTileRows * 4 <= kRing, "the ring holds the partial sums as [token][row] int32");
+  static constexpr int kSmem = 1024 + kRing;  // ring aligned to 1024
+  static constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
+};
+
+__device__ __forceinline__ int cluster_load(uint32_t smem, uint32_t rank) {
   uint32_t remote;
   int v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(rank));
@@ -91,71 +141,49 @@ __device__ __forceinline__ int cluster_load1(uint32_t smem, uint32_t rank) {
   return v;
 }
 
-__device__ __forceinline__ void store4(const Int8Args& a, int t, int n, const float (&v)[4]) {
-  const int64_t at = static_cast<int64_t>(t) * a.ldy + n;
-  if (a.y_vec4 && n + 4 <= a.channels) {
-    if (a.y_dtype == QCC_DTYPE_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if (a.y_dtype == QCC_DTYPE_BF16) {
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.y) + at) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    } else {
-      const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
-      *reinterpret_cast<uint2*>(static_cast<__half*>(a.y) + at) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (n + j < a.channels) store_as(a.y, at + j, a.y_dtype, v[j]);
-}
-
-template <bool GATED, int BN, int STAGES>
-__global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, const __grid_constant__ CUtensorMap tm_x,
-                                                          const __grid_constant__ CUtensorMap tm_w) {
-  using S = StreamSmem<BN, STAGES>;
+template <bool GATED, typename O, int BN, int STAGES>
+__global__ void __launch_bounds__(128)
+    int8_stream_kernel(const Int8Args a, const __grid_constant__ CUtensorMap tm_x,
+                       const __grid_constant__ CUtensorMap tm_w) {
+  using S = StreamShape<BN, STAGES>;
   constexpr int kChannels = GATED ? kTileRows / 2 : kTileRows;
-  constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[STAGES], empty[STAGES], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int warp = threadIdx.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank, splits;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
   const int n0 = static_cast<int>(blockIdx.x / splits) * kChannels, t0 = static_cast<int>(blockIdx.y) * BN;
   const int blocks = (a.cols + kTileCols - 1) / kTileCols;
   const int first = static_cast<int>(static_cast<int64_t>(blocks) * rank / splits);
-  const int count = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / splits) - first;
+  const int count = static_cast<int>(static_cast<int64_t>(blocks) * (rank + 1) / splits) - first;  // >= 1
 
-  if (warp == 0) {
-    if (threadIdx.x == 0) {
-      tma_prefetch_map(&tm_x);
-      tma_prefetch_map(&tm_w);
-      for (int s = 0; s < STAGES; ++s) {
-        mbar_init(&full[s], 1);
-        mbar_init(&empty[s], 1);
-      }
-      mbar_init(&done, 1);
-      failed = 0;
-      fence_barrier_init();
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&tm_x);
+    tma_prefetch_map(&tm_w);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
+    mbar_init(&done, 1);
+    failed = 0;
+    fence_barrier_init();
   }
   // Tensor memory is taken only once the launches ahead have finished: a CTA
   // of theirs that still waits for its own columns must not wait for ours.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_dependency_wait();
   if (warp == 1) {
-    tmem_alloc(&tmem_slot, kTmemCols);
+    tmem_alloc(&tmem_slot, S::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  grid_dependency_trigger();
 
   if (threadIdx.x == 0) {
     const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
@@ -170,8 +198,9 @@ __global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, cons
       mbar_arrive_expect_tx(&full[s], S::kStage);
       const int k = (first + issued) * kTileCols;
       if (GATED) {
-        tma_load_2d_hint(w, &tm_w, k, n0, &full[s], stream);
-        tma_load_2d_hint(w + S::kWBytes / 2, &tm_w, k, a.channels + n0, &full[s], stream);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          tma_load_3d_hint(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, 0, &full[s], stream);
       } else {
         tma_load_2d_hint(w, &tm_w, k, n0, &full[s], stream);
       }
@@ -179,7 +208,7 @@ __global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, cons
     }
     // A copy must not land after this CTA has gone: after a wait that ran out, see the issued ones in.
     if (issued < count)
-      for (int i = issued - STAGES < 0 ? 0 : issued - STAGES; i < issued; ++i)
+      for (int i = max(0, issued - STAGES); i < issued; ++i)
         mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1, kWaitNs);
   } else if (threadIdx.x == 32) {
     constexpr uint32_t idesc = idesc_s8(kTileRows, BN);
@@ -202,74 +231,69 @@ __global__ void __launch_bounds__(128) int8_stream_kernel(const Int8Args a, cons
   __syncwarp();
   if (!mbar_wait_bounded(&done, 0, 4 * kWaitNs)) failed = 1;
   tc_fence_after_sync();
+  __syncthreads();
 
-  // TMEM -> this CTA's shared memory as [token][row] int32 (the ring is free: every MMA has completed).
-  int* partial = reinterpret_cast<int*>(ring);
   const int tokens = min(BN, a.tokens - t0);
+  const uint32_t from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  if (splits == 1) {
+    const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, failed != 0);
 #pragma unroll 1
-  for (int c = 0; c < tokens; c += 16) {
-    float v[16];
-    tmem_load16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, v);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) partial[(c + j) * kTileRows + threadIdx.x] = count > 0 ? __float_as_int(v[j]) : 0;
-  }
-  tc_fence_before_sync();
-  cluster_sync();
-  tc_fence_after_sync();
-  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
-
-  // Sum over the cluster, scale and store: 4 channels of one token a thread at a time.
-  constexpr int kVecs = kChannels / 4;
-  const uint32_t base = smem_addr(partial);
-  int broken = 0;
-  for (uint32_t r = 0; r < splits; ++r) broken |= cluster_load1(smem_addr(&failed), r);
-  for (int i = static_cast<int>(rank) * 128 + static_cast<int>(threadIdx.x); i < tokens * kVecs;
-       i += 128 * static_cast<int>(splits)) {
-    const int t = i / kVecs, c = i % kVecs * 4;
-    int g[4] = {}, u[4] = {};
-    for (uint32_t r = 0; r < splits; ++r) {
-      const int4 p = cluster_load4(base + (t * kTileRows + c) * 4, r);
-      g[0] += p.x, g[1] += p.y, g[2] += p.z, g[3] += p.w;
-      if (GATED) {
-        const int4 q = cluster_load4(base + (t * kTileRows + kChannels + c) * 4, r);
-        u[0] += q.x, u[1] += q.y, u[2] += q.z, u[3] += q.w;
-      }
+    for (int c = 0; c < tokens; c += 16) {
+      const float xs = c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
+      int acc[16];
+      tmem_load16(from + c, acc);
+      out.finish(acc, c, tokens, xs, lane);
     }
-    const float xs = a.xs[t0 + t];
-    float v[4];
+    tc_fence_before_sync();
+    __syncthreads();
+  } else {
+    // The ring is free (every MMA has completed).
+    int* partial = reinterpret_cast<int*>(ring);
+#pragma unroll 1
+    for (int c = 0; c < tokens; c += 16) {
+      int acc[16];
+      tmem_load16(from + c, acc);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = min(n0 + c + j, a.channels - 1);
-      v[j] = static_cast<float>(g[j]) * (xs * a.ws[n]);
-      if (GATED)
-        v[j] = silu(v[j]) * (static_cast<float>(u[j]) * (xs * a.ws[a.channels + n]));
-      else
-        v[j] += bias_value(a.bias, a.bias_dtype, n);
-      if (broken) v[j] = NAN;
+      for (int j = 0; j < 16; ++j) partial[(c + j) * kTileRows + threadIdx.x] = acc[j];
     }
-    store4(a, t0 + t, n0 + c, v);
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync();
+    tc_fence_after_sync();
+    int any = 0;
+    for (uint32_t r = 0; r < splits; ++r) any |= cluster_load(smem_addr(&failed), r);
+    const uint32_t base = smem_addr(partial) + threadIdx.x * 4;
+    const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, any != 0);
+    constexpr int kRun = 4;  // tokens a warp sums at a time; the cluster's CTAs take runs in turn
+    for (int c = static_cast<int>(rank) * kRun; c < tokens; c += static_cast<int>(splits) * kRun) {
+      const float xs = lane < kRun && c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
+      int acc[kRun] = {};
+      for (uint32_t r = 0; r < splits; ++r)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) acc[j] += cluster_load(base + (c + j) * kTileRows * 4, r);
+      out.finish(acc, c, tokens, xs, lane);
+    }
+    __syncwarp();
+    cluster_sync();  // the other CTAs have read this one's sums
   }
-  cluster_sync();  // the other CTAs have read this one's sums
+  if (warp == 1) tmem_dealloc(tmem, S::kTmemCols);
 }
 
 // ---------------------------------------------------------------------------
 // Pair kernel: persistent CTA pairs (cta_group::2), tiles of 256 weight rows x
 // up to 256 tokens over all columns, for token counts that make the product
 // compute bound.  Warp 0 loads, warp 1 of the even CTA issues the MMAs, warps
-// 2-5 drain the accumulators; two accumulators (2 x 256 of the 512 TMEM
+// 2-9 drain the accumulators; two accumulators (2 x 256 of the 512 TMEM
 // columns) let a tile's epilogue run beside the next tile's MMAs.  A pair reads
 // each operand byte of its tile once (128 rows of each per CTA), half of what
 // two single CTAs would.
-// Gated: the rows of a tile alternate 16 gate and 16 up rows, so that lane l
-// of a warp holds the gate and lane l + 16 the up product of one channel and
-// one shuffle brings two tokens' pairs together.
 // ---------------------------------------------------------------------------
 
 constexpr int kPairStages = 6;
 constexpr int kPairTokens = 256;                       // most tokens of a tile
 constexpr int kPairStage = 2 * 128 * kTileCols;        // bytes a CTA loads per stage, at most
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage;
-constexpr int kPairThreads = 192;
+constexpr int kPairThreads = 320;
 
 struct PairPlan {
   int row_tiles, token_tiles, tile_tokens;  // tile_tokens: multiple of 32, up to kPairTokens
@@ -286,7 +310,7 @@ __device__ __forceinline__ void pair_tile(const PairPlan& p, int i, int& row, in
   token = g * p.group + in - row * width;
 }
 
-template <bool GATED>
+template <bool GATED, typename O>
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const Int8Args a, const PairPlan plan, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_w) {
@@ -313,12 +337,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], 8);  // the four epilogue warps of both CTAs
+      mbar_init(&acc_empty[s], 16);  // the eight epilogue warps of both CTAs
     }
     failed = 0;
     fence_barrier_init();
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // before tensor memory is taken, as in the stream kernel
+  grid_dependency_wait();  // before tensor memory is taken, as in the stream kernel
   if (warp == 1) {
     tmem_alloc_pair(&tmem_slot, 512);
     tmem_relinquish_pair();
@@ -328,6 +352,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   cluster_sync();  // both CTAs' barriers are initialised
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  grid_dependency_trigger();
 
   if (threadIdx.x == 0) {
     const uint64_t keep = policy_evict_last();
@@ -349,10 +374,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (GATED) {
           const int n0 = row * kChannels + static_cast<int>(rank) * 64;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            tma_load_2d_pair(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, bar, keep);
-            tma_load_2d_pair(w + (q * 32 + 16) * kTileCols, &tm_w, k, a.channels + n0 + q * 16, bar, keep);
-          }
+          for (int q = 0; q < 4; ++q)
+            tma_load_3d_pair(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, 0, bar, keep);
         } else {
           tma_load_2d_pair(w, &tm_w, k, row * kChannels + static_cast<int>(rank) * 128, bar, keep);
         }
@@ -405,43 +428,25 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int row, token;
       pair_tile(plan, i, row, token);
       const int t0 = token * plan.tile_tokens, tokens = min(plan.tile_tokens, a.tokens - t0);
-      const int n = row * kChannels + static_cast<int>(rank) * (kChannels / 2) +
-                    (GATED ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
-      const bool in = n < a.channels;
-      const int wrow = GATED && lane >= 16 ? a.channels + n : n;
-      const float ws = in ? a.ws[wrow] : 0.f;
-      const float bias = !GATED && in ? bias_value(a.bias, a.bias_dtype, n) : 0.f;
+      const RowOutput<GATED, O> out(
+          a, row * kChannels + static_cast<int>(rank) * (kChannels / 2) + quarter * (GATED ? 16 : 32), t0, lane,
+          failed != 0);
       const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
-      for (int c = 0; c < tokens; c += 32) {
-        float v[32];
-        tmem_load32(from + c, v);
+      int c = (warp - 2) / 4 * 32;
+      for (; c < tokens; c += 64) {
+        int sums[32];
+        tmem_load32(from + c, sums);
         const float xs = c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
-        if (c + 32 >= tokens) {  // the accumulator's last columns are in registers
+        if (c + 64 >= tokens) {  // this warp's last columns are in registers
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[acc], 0));
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          v[j] = static_cast<float>(__float_as_int(v[j])) * (__shfl_sync(0xffffffffu, xs, j) * ws);
-        if (GATED) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            // Lanes 0-15 finish token j, lanes 16-31 token j + 1.
-            const float other = __shfl_xor_sync(0xffffffffu, lane < 16 ? v[j + 1] : v[j], 16);
-            float h = silu(lane < 16 ? v[j] : other) * (lane < 16 ? other : v[j + 1]);
-            if (failed) h = NAN;
-            const int t = c + j + (lane >> 4);
-            if (in && t < tokens) store_as(a.y, static_cast<int64_t>(t0 + t) * a.ldy + n, a.y_dtype, h);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float y = v[j] + bias;
-            if (failed) y = NAN;
-            if (in && c + j < tokens) store_as(a.y, static_cast<int64_t>(t0 + c + j) * a.ldy + n, a.y_dtype, y);
-          }
-        }
+        out.finish(sums, c, tokens, xs, lane);
+      }
+      if (tokens <= 32 && c == 32) {  // the second four warps had no column of this tile
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[acc], 0));
       }
     }
   }
@@ -477,90 +482,105 @@ bool make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t cols, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool GATED, int BN, int STAGES>
-int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
-  using S = StreamSmem<BN, STAGES>;
-  auto* kernel = int8_stream_kernel<GATED, BN, STAGES>;
-  CUtensorMap tm_x, tm_w;
-  const int64_t rows = GATED ? 2ll * a.channels : a.channels;
-  if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, BN) ||
-      !make_map(&tm_w, a.w, rows, a.cols, a.ldw, GATED ? kTileRows / 2 : kTileRows))
-    return QCC_ERR_UNSUPPORTED;
-  if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
-  const int channels = GATED ? kTileRows / 2 : kTileRows;
-  const int tiles = (a.channels + channels - 1) / channels, token_tiles = (a.tokens + BN - 1) / BN;
-  const int slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kBytes + 2048));
-  const int blocks = (a.cols + kTileCols - 1) / kTileCols;
-  const int split = std::max(1, std::min({8, blocks, static_cast<int>(slots / (static_cast<int64_t>(tiles) * token_tiles))}));
+// The gate and the up rows of a fused weight as two planes: a box holds box_rows rows of each.
+bool make_gated_map(CUtensorMap* map, const int8_t* base, int64_t channels, int64_t cols, int64_t ld, int box_rows) {
+  auto fn = encode_tiled();
+  if (fn == nullptr) return false;
+  const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(channels), 2};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(channels * ld)};
+  const uint32_t box[3] = {kTileCols, static_cast<uint32_t>(box_rows), 2}, elem[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A launch on `stream` as clusters of `cluster` CTAs that may start while the launch ahead of it finishes.
+template <typename... P, typename... A>
+int launch_clusters(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
+                    const A&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * split, token_tiles);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a, tm_x, tm_w)) ? QCC_OK : QCC_ERR_CUDA;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...)) ? QCC_OK : QCC_ERR_CUDA;
 }
 
-// The token width of a tile: the one that needs the fewest columns of MMA work in the longest-running pair.
-int pair_tile_tokens(int tokens, int row_tiles, int pairs) {
-  int best = kPairTokens;
-  int64_t best_cost = INT64_MAX;
-  for (int width = kPairTokens; width >= 128; width -= 32) {
-    const int64_t tiles = static_cast<int64_t>(row_tiles) * ((tokens + width - 1) / width);
-    const int64_t cost = (tiles + pairs - 1) / pairs * width;
-    if (cost < best_cost) best = width, best_cost = cost;
-  }
-  return best;
+template <bool GATED, typename O, int BN, int STAGES>
+int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
+  using S = StreamShape<BN, STAGES>;
+  constexpr int kChannels = GATED ? kTileRows / 2 : kTileRows;
+  auto* kernel = int8_stream_kernel<GATED, O, BN, STAGES>;
+  CUtensorMap tm_x, tm_w;
+  if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, BN) ||
+      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 16)
+              : make_map(&tm_w, a.w, a.channels, a.cols, a.ldw, kTileRows)))
+    return QCC_ERR_UNSUPPORTED;
+  if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
+  const int tiles = (a.channels + kChannels - 1) / kChannels, token_tiles = (a.tokens + BN - 1) / BN;
+  const int64_t slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kSmem + 2048));
+  const int blocks = (a.cols + kTileCols - 1) / kTileCols;
+  int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, blocks, slots * 85 / 100 / (static_cast<int64_t>(tiles) * token_tiles)})));
+  if (getenv("QS")) split = atoi(getenv("QS"));
+  return launch_clusters(kernel, dim3(tiles * split, token_tiles), 128, S::kSmem, split, stream, a, tm_x, tm_w);
 }
 
-template <bool GATED>
+template <bool GATED, typename O>
 int launch_pair(const Int8Args& a, int device, cudaStream_t stream) {
-  auto* kernel = int8_pair_kernel<GATED>;
+  auto* kernel = int8_pair_kernel<GATED, O>;
   const int channels = GATED ? 128 : 256;
   const int pairs = device_info(device).num_sms / 2;
   PairPlan plan;
   plan.row_tiles = (a.channels + channels - 1) / channels;
-  plan.tile_tokens = pair_tile_tokens(a.tokens, plan.row_tiles, pairs);
-  plan.token_tiles = (a.tokens + plan.tile_tokens - 1) / plan.tile_tokens;
+  // As few token tiles as fit, of equal width: a tile's time hardly falls with its width (its weight rows' loads stay).
+  plan.token_tiles = (a.tokens + kPairTokens - 1) / kPairTokens;
+  plan.tile_tokens = ((a.tokens + plan.token_tiles - 1) / plan.token_tiles + 31) / 32 * 32;
   plan.group = 8;
   CUtensorMap tm_x, tm_w;
   if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, plan.tile_tokens / 2) ||
-      !make_map(&tm_w, a.w, GATED ? 2ll * a.channels : a.channels, a.cols, a.ldw, GATED ? 16 : 128))
+      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 16)
+              : make_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 128)))
     return QCC_ERR_UNSUPPORTED;
   if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(pairs, static_cast<int64_t>(plan.row_tiles) *
-                                                                            plan.token_tiles)));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2] = {};
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a, plan, tm_x, tm_w)) ? QCC_OK : QCC_ERR_CUDA;
+  const unsigned grid = 2u * static_cast<unsigned>(std::min<int64_t>(pairs, static_cast<int64_t>(plan.row_tiles) * plan.token_tiles));
+  return launch_clusters(kernel, dim3(grid), kPairThreads, kPairSmem, 2, stream, a, plan, tm_x, tm_w);
+}
+
+template <bool GATED, typename O>
+int launch(const Int8Args& a, int device, cudaStream_t stream) {
+  const char* v = getenv("QV");
+  if (v) {
+    switch (atoi(v)) {
+      case 16: return launch_stream<GATED, O, 16, 4>(a, device, stream);
+      case 32: return launch_stream<GATED, O, 32, 4>(a, device, stream);
+      case 323: return launch_stream<GATED, O, 32, 3>(a, device, stream);
+      case 64: return launch_stream<GATED, O, 64, 4>(a, device, stream);
+      case 128: return launch_stream<GATED, O, 128, 3>(a, device, stream);
+      case 256: return launch_stream<GATED, O, 256, 4>(a, device, stream);
+      default: return launch_pair<GATED, O>(a, device, stream);
+    }
+  }
+  if (a.tokens <= 16) return launch_stream<GATED, O, 16, 4>(a, device, stream);
+  if (a.tokens <= 32) return launch_stream<GATED, O, 32, 4>(a, device, stream);
+  if (a.tokens <= 64) return launch_stream<GATED, O, 64, 4>(a, device, stream);
+  if (a.tokens <= 128) return launch_stream<GATED, O, 128, 3>(a, device, stream);
+  return launch_pair<GATED, O>(a, device, stream);
 }
 
 template <bool GATED>
 int launch(const Int8Args& a, int device, cudaStream_t stream) {
-  if (a.tokens <= 16) return launch_stream<GATED, 16, 4>(a, device, stream);
-  if (a.tokens <= 32) return launch_stream<GATED, 32, 4>(a, device, stream);
-  if (a.tokens <= 64) return launch_stream<GATED, 64, 4>(a, device, stream);
-  if (a.tokens <= 128) return launch_stream<GATED, 128, 3>(a, device, stream);
-  return launch_pair<GATED>(a, device, stream);
+  if (a.y_dtype == QCC_DTYPE_BF16) return launch<GATED, __nv_bfloat16>(a, device, stream);
+  if (a.y_dtype == QCC_DTYPE_F16) return launch<GATED, __half>(a, device, stream);
+  return launch<GATED, float>(a, device, stream);
 }
 
 int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
@@ -574,7 +594,6 @@ int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
   if (!aligned16(a.x) || !aligned16(a.w) || a.ldx % 16 != 0 || a.ldw % 16 != 0) return QCC_ERR_ALIGNMENT;
   int device = 0;
   if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
-  a.y_vec4 = reinterpret_cast<uintptr_t>(a.y) % (4 * dtype_bytes(a.y_dtype)) == 0 && a.ldy % 4 == 0;
   clear_stale_error();
   return gated ? launch<true>(a, device, stream) : launch<false>(a, device, stream);
 }

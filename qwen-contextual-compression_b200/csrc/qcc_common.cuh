@@ -64,6 +64,14 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// Programmatic dependent launch: waits until the launches ahead on the stream
+// have completed and their writes are visible (at once when this launch was not
+// allowed to start early); lets the next launch start.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // Cache policy for data that later reads of the same kernel should find in L2.
 __device__ __forceinline__ uint64_t policy_evict_last() {
   uint64_t p;

@@ -164,6 +164,15 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                                 uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+      "[%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(ncols)
                : "memory");
@@ -228,6 +237,20 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// The same for integer accumulators.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, int (&v)[32]) {
+  float f[32];
+  tmem_load32(taddr, f);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_int(f[i]);
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, int (&v)[16]) {
+  float f[16];
+  tmem_load16(taddr, f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __float_as_int(f[i]);
 }
 
 // ---------------------------------------------------------------------------
