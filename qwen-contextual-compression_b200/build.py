@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -55,8 +56,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     nvcc = nvcc_path()
     build_dir = PACKAGE_DIR / "_build"
     build_dir.mkdir(exist_ok=True)
-    objects = []
-    for src in sources():
+
+    def compile_one(src: Path) -> str:
         obj = build_dir / (src.stem + ".o")
         cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-I", str(INCLUDE), "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
         if ptxas_verbose:
@@ -68,7 +69,10 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             raise RuntimeError(f"nvcc failed for {src.name}:\n{result.stdout}\n{result.stderr}")
         if ptxas_verbose or verbose:
             sys.stdout.write(result.stdout + result.stderr)
-        objects.append(str(obj))
+        return str(obj)
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count()) as pool:
+        objects = list(pool.map(compile_one, sources()))
     tmp = LIBRARY.with_suffix(".so.tmp")
     cmd = [nvcc, *ARCH_FLAGS, "-shared", "-cudart", "static", "-o", str(tmp), *objects]
     if verbose:

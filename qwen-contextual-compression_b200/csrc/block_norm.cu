@@ -13,7 +13,18 @@
 //
 // One pass: a row's values stay in registers between the reductions (the
 // layer norm's variance is a second sum over centred values, not a difference
-// of moments), so DRAM sees each input once and each output once.
+// of moments), so DRAM sees each input once and each output once, and the
+// bytes are the bound.
+//
+// A row is cut into granules of 8 elements that start on 16 bytes; its first
+// and last granule may be partial (rows of odd width start anywhere).  Three
+// kernels share the arithmetic:
+//   warp_kernel   a warp a row, rows up to 128 granules;
+//   ring_kernel   a block a row, rows through a shared-memory ring of bulk
+//                 copies that runs ahead of the arithmetic;
+//   plain_kernel  single elements, read again in each pass: rows of tensors
+//                 that do not share their granules (mixed alignments), mixes of
+//                 three element types, and rows beyond the ring's.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,9 +36,8 @@
 namespace qcc {
 namespace {
 
-constexpr int kMaxThreads = 1024;
-constexpr int kMaxVecs = 4;                               // 8-element vectors a thread keeps
-constexpr int kMaxHidden = kMaxThreads * kMaxVecs * 8;    // 32768
+constexpr int kMaxHidden = 32768;
+constexpr uint64_t kWaitNs = 2000000000ull;
 // A row whose largest magnitude is below this is stored as zeros: its scale
 // (and 127 / amax) would leave the normal fp32 range.
 constexpr float kSmallestAmax = 1.504632769052528e-36f;   // 2^-119
@@ -47,40 +57,74 @@ struct BlockNormArgs {
   int64_t ld_out;
   int out_dtype;  // QCC_DTYPE_* or QCC_DTYPE_I8
   float* row_scale;
+  int shift0;             // elements of row 0 before its first 16-byte boundary's granule, 0..7
+  bool gate_in_granules;  // the gate's rows, in the branch's type, share its granules
+  float inv_hidden;       // 1 / hidden
 };
 
-// Element index of value j of vector v: vectors of 8 consecutive elements, or
-// (rows that are not 16-byte aligned) single elements a block width apart.
-template <bool VEC>
-__device__ __forceinline__ int element(int v, int j) {
-  const int bd = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
-  return VEC ? (v * bd + tid) * 8 + j : (v * 8 + j) * bd + tid;
-}
+// ---------------------------------------------------------------------------
+// Which elements a thread holds.
+// ---------------------------------------------------------------------------
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T* row, int v, int n, float (&f)[8]) {
-  if (VEC) {
-    const int e = element<true>(v, 0);
-    if (e + 8 <= n) {
-      widen(load_pack8<T>(row + e), f);
-      return;
-    }
+// Granule i of member `id` of a team of `width` threads: elements first(i) .. + 7.  EXACT: rows without a shift and
+// with a multiple of 8 elements, whose granules (and those of 16-byte aligned parameters) exist whole or not at all.
+template <bool EXACT>
+struct GranuleMap {
+  int n, shift, id, width;
+  __device__ __forceinline__ int first(int i) const { return (i * width + id) * 8 - (EXACT ? 0 : shift); }
+  __device__ __forceinline__ int element(int i, int j) const { return first(i) + j; }
+  __device__ __forceinline__ bool has(int i, int j) const {
+    return static_cast<unsigned>(element(i, j)) < static_cast<unsigned>(n);
   }
+  // All of the granule exists.
+  __device__ __forceinline__ bool whole(int i) const {
+    return EXACT ? first(i) < n : first(i) >= 0 && first(i) + 8 <= n;
+  }
+};
+
+template <typename T>
+struct alignas(16) Granule {
+  T e[8];
+};
+
+template <typename T>
+__device__ __forceinline__ void widen(const Granule<T>& g, float (&f)[8]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = element<VEC>(v, j);
-    f[j] = e < n ? to_f32<T>(row[e]) : 0.f;
+  for (int j = 0; j < 8; ++j) f[j] = to_f32<T>(g.e[j]);
+}
+
+// Granule i of a row (zeros outside of it): one wide load where all of it exists.
+template <typename T, bool EXACT>
+__device__ __forceinline__ Granule<T> load_granule(const T* row, const GranuleMap<EXACT>& m, int i) {
+  Granule<T> g;
+  if (m.whole(i)) {
+    g = *reinterpret_cast<const Granule<T>*>(row + m.first(i));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g.e[j] = !EXACT && m.has(i, j) ? row[m.element(i, j)] : T(0.f);
+  }
+  return g;
+}
+
+// A parameter vector's elements of granule i.  Without EXACT its alignment is not the row's: single elements.
+template <typename P, bool EXACT>
+__device__ __forceinline__ void load_param8(const P* p, const GranuleMap<EXACT>& m, int i, float (&f)[8]) {
+  if (EXACT) {
+    widen(load_granule(p, m, i), f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = m.has(i, j) ? to_f32<P>(p[m.element(i, j)]) : 0.f;
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void load_any8(const void* row, int dtype, int v, int n, float (&f)[8]) {
-  if (dtype == QCC_DTYPE_BF16)
-    load_row8<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(row), v, n, f);
-  else if (dtype == QCC_DTYPE_F16)
-    load_row8<__half, VEC>(static_cast<const __half*>(row), v, n, f);
+// The same for a parameter in T or fp32.
+template <typename T, bool EXACT>
+__device__ __forceinline__ void load_param8(const void* p, int dtype, const GranuleMap<EXACT>& m, int i,
+                                            float (&f)[8]) {
+  if (sizeof(T) == 4 || dtype == QCC_DTYPE_F32)
+    load_param8(static_cast<const float*>(p), m, i, f);
   else
-    load_row8<float, VEC>(static_cast<const float*>(row), v, n, f);
+    load_param8(static_cast<const T*>(p), m, i, f);
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
@@ -94,120 +138,127 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half*) {
 
 template <typename T>
 __device__ __forceinline__ void store_vec8(T* p, const float* f) {
-  uint4 w;
-  w.x = pack2(f[0], f[1], p);
-  w.y = pack2(f[2], f[3], p);
-  w.z = pack2(f[4], f[5], p);
-  w.w = pack2(f[6], f[7], p);
-  *reinterpret_cast<uint4*>(p) = w;
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack2(f[0], f[1], p), pack2(f[2], f[3], p), pack2(f[4], f[5], p), pack2(f[6], f[7], p));
 }
 __device__ __forceinline__ void store_vec8(float* p, const float* f) {
   reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_row8(T* row, int v, int n, const float* f) {
-  if (VEC) {
-    const int e = element<true>(v, 0);
-    if (e + 8 <= n) {
-      store_vec8(row + e, f);
-      return;
-    }
-  }
+template <typename T, bool EXACT>
+__device__ __forceinline__ void store_granule(T* row, const GranuleMap<EXACT>& m, int i, const float* f) {
+  if (m.whole(i)) {
+    store_vec8(row + m.first(i), f);
+  } else if (!EXACT) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = element<VEC>(v, j);
-    if (e < n) row[e] = static_cast<T>(f[j]);
+    for (int j = 0; j < 8; ++j)
+      if (m.has(i, j)) row[m.element(i, j)] = static_cast<T>(f[j]);
   }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store_any8(void* row, int dtype, int v, int n, const float* f) {
-  if (dtype == QCC_DTYPE_BF16)
-    store_row8<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(row), v, n, f);
-  else if (dtype == QCC_DTYPE_F16)
-    store_row8<__half, VEC>(static_cast<__half*>(row), v, n, f);
-  else
-    store_row8<float, VEC>(static_cast<float*>(row), v, n, f);
 }
 
 // |f| <= 127 / inverse by construction, so the rounded value fits int8.
-template <bool VEC>
-__device__ __forceinline__ void store_int8x8(int8_t* row, int v, int n, const float* f, float inverse) {
+__device__ __forceinline__ int8_t to_int8(float f, float inverse) {
+  return static_cast<int8_t>(__float2int_rn(f * inverse));
+}
+
+template <bool EXACT>
+__device__ __forceinline__ void store_int8x8(int8_t* row, const GranuleMap<EXACT>& m, int i, const float* f,
+                                             float inverse) {
   uint32_t q[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = static_cast<uint32_t>(__float2int_rn(f[j] * inverse)) & 0xFFu;
-  if (VEC) {
-    const int e = element<true>(v, 0);
-    if (e + 8 <= n) {
-      uint2 w;
-      w.x = q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24);
-      w.y = q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24);
-      *reinterpret_cast<uint2*>(row + e) = w;
-      return;
-    }
-  }
+  for (int j = 0; j < 8; ++j) q[j] = static_cast<uint8_t>(to_int8(f[j], inverse));
+  if (m.whole(i) && (EXACT || (reinterpret_cast<uintptr_t>(row + m.first(i)) & 7) == 0)) {
+    *reinterpret_cast<uint2*>(row + m.first(i)) =
+        make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+  } else if (!EXACT) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = element<VEC>(v, j);
-    if (e < n) row[e] = static_cast<int8_t>(q[j]);
+    for (int j = 0; j < 8; ++j)
+      if (m.has(i, j)) row[m.element(i, j)] = static_cast<int8_t>(q[j]);
   }
 }
 
-struct SumOp {
-  static __device__ __forceinline__ float apply(float a, float b) { return a + b; }
-};
-struct MaxOp {
-  static __device__ __forceinline__ float apply(float a, float b) { return fmaxf(a, b); }
+// Bits of |f|: ordered like the magnitudes, infinities and then NaNs above all finite values.
+__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
+
+// What a row's largest magnitude (its bits) makes of its int8 form.
+struct RowScale {
+  float scale, inverse;  // inverse 0: the row is stored as zeros
+  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+    const float amax = __uint_as_float(bits);
+    const bool finite = bits <= 0x7F7FFFFFu, kept = finite && amax >= kSmallestAmax;
+    inverse = kept ? 127.f / amax : 0.f;
+    scale = kept ? amax / 127.f : finite ? 0.f : NAN;
+  }
 };
 
-// Reduction over the block in a fixed order; every thread gets the result.
-template <typename Op>
-__device__ __forceinline__ float block_reduce(float v, float* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = Op::apply(v, __shfl_xor_sync(0xffffffffu, v, o));
-  const int warps = static_cast<int>(blockDim.x) >> 5;
-  if (warps == 1) return v;
-  __syncthreads();  // the previous reduction's readers are done
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = static_cast<int>(threadIdx.x & 31) < warps ? scratch[threadIdx.x & 31] : scratch[0];
-  if (static_cast<int>(threadIdx.x & 31) >= warps) s = Op::apply(0.f, 0.f);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s = Op::apply(s, __shfl_xor_sync(0xffffffffu, s, o));
-  return s;
-}
+// ---------------------------------------------------------------------------
+// Reductions over the team of a row, in a fixed order.
+// ---------------------------------------------------------------------------
 
-// v <- N(v) over the row's `n` values (entries past the row are 0 on entry and on exit).
-template <int VPT, bool VEC>
-__device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_params& a, int n, float* scratch) {
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+struct WarpTeam {
+  __device__ __forceinline__ float sum(float v) { return warp_sum(v); }
+  __device__ __forceinline__ uint32_t max(uint32_t v) { return warp_max(v); }
+};
+
+// One barrier a reduction: the halves of `scratch` [2][32] are used in turn, and a half's readers have passed the
+// next reduction's barrier before it is written again.
+struct BlockTeam {
+  float* scratch;
+  int half = 0;
+  __device__ __forceinline__ float exchange(float v) {
+    const int lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
+    float* s = scratch + half * 32;
+    half ^= 1;
+    if (lane == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return lane < warps ? s[lane] : 0.f;  // 0: neutral for sums and for maxima of magnitudes
+  }
+  __device__ __forceinline__ float sum(float v) { return warp_sum(exchange(warp_sum(v))); }
+  __device__ __forceinline__ uint32_t max(uint32_t v) {
+    return warp_max(__float_as_uint(exchange(__uint_as_float(warp_max(v)))));
+  }
+};
+
+// ---------------------------------------------------------------------------
+// The arithmetic of a row.
+// ---------------------------------------------------------------------------
+
+// v <- N(v) over the row's values (entries outside the row are 0 on entry, and stay so where they are summed).
+template <typename T, int VPT, bool EXACT, typename Team>
+__device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_params& a, float inv_n,
+                                          const GranuleMap<EXACT>& m, Team& team) {
   if (a.kind == QCC_NORM_NONE) return;
-  float mean = 0.f;
   if (a.kind == QCC_NORM_LAYER) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += v[i][j];
-    mean = block_reduce<SumOp>(s, scratch) / static_cast<float>(n);
+    const float mean = team.sum(s) * inv_n;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = element<VEC>(i, j) < n ? v[i][j] - mean : 0.f;
+      for (int j = 0; j < 8; ++j) v[i][j] -= mean;
+      if (!m.whole(i))
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (EXACT || !m.has(i, j)) v[i][j] = 0.f;
+    }
   }
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) s += v[i][j] * v[i][j];
-  s = block_reduce<SumOp>(s, scratch);
-  const float rstd = 1.f / sqrtf(s / static_cast<float>(n) + a.eps);
+  const float rstd = rsqrtf(team.sum(s) * inv_n + a.eps);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float w[8];
     if (a.weight != nullptr) {
-      load_any8<VEC>(a.weight, a.dtype, i, n, w);
+      load_param8<T>(a.weight, a.dtype, m, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] *= rstd * (a.weight_offset + w[j]);
     } else {
@@ -215,120 +266,392 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
       for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
     }
     if (a.bias != nullptr) {
-      load_any8<VEC>(a.bias, a.dtype, i, n, w);
+      load_param8<T>(a.bias, a.dtype, m, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] += w[j];
     }
   }
 }
 
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t e) {
+  if (dtype == QCC_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[e]);
+  if (dtype == QCC_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[e]);
+  return static_cast<const float*>(p)[e];
+}
+
 __device__ __forceinline__ float gate_value(float g, int act) {
-  if (act == QCC_GATE_SIGMOID) return 1.f / (1.f + expf(-g));
+  // The fast exponential and quotient are off by |g| + 8 roundings at most, and exact at the ends (0 and 1).
+  if (act == QCC_GATE_SIGMOID) return __fdividef(1.f, 1.f + __expf(-g));
   if (act == QCC_GATE_TANH) return tanhf(g);
   return g;
 }
 
-// One CTA a row.  T: the branch's type, R: the residual's.
-template <typename T, typename R, int VPT, bool VEC>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const BlockNormArgs a) {
-  __shared__ float scratch[32];
-  const int64_t t = blockIdx.x;
-  const int n = a.hidden;
-  float v[VPT][8];
+// v <- act(gate) * v.
+template <typename T, int VPT, bool EXACT>
+__device__ __forceinline__ void apply_gate(float (&v)[VPT][8], const BlockNormArgs& a, int64_t t,
+                                           const GranuleMap<EXACT>& m) {
+  if (a.gate.values == nullptr) return;
+  const int64_t row = (t / a.gate.rows_each) * a.gate.ld;
+  if (a.gate.cols == 1) {
+    const float s = gate_value(load_any(a.gate.values, a.gate.dtype, row), a.gate.act);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) load_row8<T, VEC>(static_cast<const T*>(a.y) + t * a.ldy, i, n, v[i]);
-  if (a.res != nullptr) {
-    normalise<VPT, VEC>(v, a.post, n, scratch);
-    if (a.gate.values != nullptr) {
-      const size_t gs = a.gate.dtype == QCC_DTYPE_F32 ? 4 : 2;
-      const char* row = static_cast<const char*>(a.gate.values) + (t / a.gate.rows_each) * a.gate.ld * gs;
-      if (a.gate.cols == 1) {
-        const float g = a.gate.dtype == QCC_DTYPE_BF16
-                            ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(row))
-                        : a.gate.dtype == QCC_DTYPE_F16 ? __half2float(*reinterpret_cast<const __half*>(row))
-                                                        : *reinterpret_cast<const float*>(row);
-        const float s = gate_value(g, a.gate.act);
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= s;
-      } else {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          float g[8];
-          load_any8<VEC>(row, a.gate.dtype, i, n, g);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= gate_value(g[j], a.gate.act);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      float r[8];
-      load_row8<R, VEC>(static_cast<const R*>(a.res) + t * a.ld_res, i, n, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[i][j] = element<VEC>(i, j) < n ? a.residual_scale * r[j] + a.branch_scale * v[i][j] : 0.f;
-      if (a.res_out != nullptr) store_row8<R, VEC>(static_cast<R*>(a.res_out) + t * a.ld_res_out, i, n, v[i]);
-    }
-  }
-  if (a.out == nullptr) return;
-  normalise<VPT, VEC>(v, a.next, n, scratch);
-  if (a.out_dtype != QCC_DTYPE_I8) {
-    char* row = static_cast<char*>(a.out) + t * a.ld_out * (a.out_dtype == QCC_DTYPE_F32 ? 4 : 2);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) store_any8<VEC>(row, a.out_dtype, i, n, v[i]);
+      for (int j = 0; j < 8; ++j) v[i][j] *= s;
     return;
   }
-  // amax with every non-finite value as +inf (fmaxf alone would drop a NaN).
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float m = fabsf(v[i][j]);
-      if (element<VEC>(i, j) < n) amax = fmaxf(amax, m <= FLT_MAX ? m : INFINITY);
-    }
-  amax = block_reduce<MaxOp>(amax, scratch);
-  const bool finite = amax <= FLT_MAX, kept = finite && amax >= kSmallestAmax;
-  const float inverse = kept ? 127.f / amax : 0.f;
-  if (threadIdx.x == 0) a.row_scale[t] = kept ? amax / 127.f : finite ? 0.f : NAN;
-  int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (!kept)
+    float g[8];
+    if (a.gate_in_granules)  // in T
+      widen(load_granule(static_cast<const T*>(a.gate.values) + row, m, i), g);
+    else
+      load_param8<T>(static_cast<const char*>(a.gate.values) + row * (a.gate.dtype == QCC_DTYPE_F32 ? 4 : 2),
+                     a.gate.dtype, m, i, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    store_int8x8<VEC>(row, i, n, v[i], inverse);
+    for (int j = 0; j < 8; ++j) v[i][j] *= gate_value(g[j], a.gate.act);
   }
 }
 
-bool row_vectors(const void* p, int64_t ld, int dtype_size) {
-  return p == nullptr || (aligned16(p) && (ld * dtype_size) % 16 == 0);
+// residual_out[t] <- v <- residual_scale * r + branch_scale * v, for granule i (0 outside of the row, as r and v are).
+template <typename R, bool EXACT>
+__device__ __forceinline__ void join8(float (&v)[8], const float (&r)[8], const BlockNormArgs& a, int64_t t,
+                                      const GranuleMap<EXACT>& m, int i) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = a.residual_scale * r[j] + a.branch_scale * v[j];
+  store_granule(static_cast<R*>(a.res_out) + t * a.ld_res_out, m, i, v);
 }
 
-int size_of(int dtype) { return dtype == QCC_DTYPE_I8 ? 1 : dtype_bytes(dtype); }
+// out[t] (T, fp32 or int8) from N_next(v).
+template <typename T, int VPT, bool EXACT, typename Team>
+__device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormArgs& a, int64_t t,
+                                           const GranuleMap<EXACT>& m, Team& team) {
+  if (a.out == nullptr) return;
+  normalise<T>(v, a.next, a.inv_hidden, m, team);
+  if (a.out_dtype == QCC_DTYPE_I8) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = max(amax, magnitude(v[i][j]));
+    const RowScale s(team.max(amax));
+    if (m.id == 0) a.row_scale[t] = s.scale;
+    int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (s.inverse == 0.f)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      store_int8x8(row, m, i, v[i], s.inverse);
+    }
+  } else if (a.out_dtype == QCC_DTYPE_F32) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) store_granule(static_cast<float*>(a.out) + t * a.ld_out, m, i, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) store_granule(static_cast<T*>(a.out) + t * a.ld_out, m, i, v[i]);
+  }
+}
 
-bool norm_vectors(const qcc_norm_params& a) { return row_vectors(a.weight, 0, 1) && row_vectors(a.bias, 0, 1); }
+// ---------------------------------------------------------------------------
+// Kernels.  T: the branch's (or x's) type, R: the residual's.
+// ---------------------------------------------------------------------------
 
-template <typename T, typename R>
-bool launch_block_norm(const BlockNormArgs& a, bool vec, cudaStream_t stream) {
-  const int vecs = (a.hidden + 7) / 8;
-  const int per = vecs <= 256 ? 1 : vecs <= 512 ? 2 : 4;
-  const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
-  const dim3 grid(static_cast<unsigned>(a.rows));
-  clear_stale_error();
-#define QCC_LAUNCH(V)                                                          \
-  (vec ? block_norm_kernel<T, R, V, true><<<grid, threads, 0, stream>>>(a)     \
-       : block_norm_kernel<T, R, V, false><<<grid, threads, 0, stream>>>(a))
-  if (per == 1)
-    QCC_LAUNCH(1);
-  else if (per == 2)
-    QCC_LAUNCH(2);
+__device__ __forceinline__ int row_shift(const BlockNormArgs& a, int64_t t) {
+  return static_cast<int>((a.shift0 + t * a.ldy) & 7);
+}
+
+constexpr int kWarpRows = 4;  // rows (warps) of a block
+
+template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
+__global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArgs a) {
+  grid_dependency_wait();
+  grid_dependency_trigger();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5);
+  if (t >= a.rows) return;
+  const GranuleMap<EXACT> m = {a.hidden, EXACT ? 0 : row_shift(a, t), static_cast<int>(threadIdx.x & 31), 32};
+  WarpTeam team;
+  Granule<T> y[VPT];
+  Granule<R> r[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) y[i] = load_granule(static_cast<const T*>(a.y) + t * a.ldy, m, i);
+  if (JOIN)
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) r[i] = load_granule(static_cast<const R*>(a.res) + t * a.ld_res, m, i);
+  float v[VPT][8];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) widen(y[i], v[i]);
+  if (JOIN) {
+    normalise<T>(v, a.post, a.inv_hidden, m, team);
+    apply_gate<T>(v, a, t, m);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[8];
+      widen(r[i], f);
+      join8<R>(v[i], f, a, t, m, i);
+    }
+  }
+  finish_row<T>(v, a, t, m, team);
+}
+
+// One norm's row statistics and an element's normed value.
+struct RowNorm {
+  float mean = 0.f, rstd = 1.f;
+  template <typename F>
+  __device__ __forceinline__ RowNorm(const qcc_norm_params& p, int n, BlockTeam& team, F value) {
+    if (p.kind == QCC_NORM_NONE) return;
+    float s = 0.f;
+    if (p.kind == QCC_NORM_LAYER) {
+      for (int e = threadIdx.x; e < n; e += blockDim.x) s += value(e);
+      mean = team.sum(s) / static_cast<float>(n);
+    }
+    s = 0.f;
+    for (int e = threadIdx.x; e < n; e += blockDim.x) {
+      const float d = value(e) - mean;
+      s += d * d;
+    }
+    rstd = 1.f / sqrtf(team.sum(s) / static_cast<float>(n) + p.eps);
+  }
+  __device__ __forceinline__ float apply(const qcc_norm_params& p, float v, int e) const {
+    if (p.kind == QCC_NORM_NONE) return v;
+    v = (v - mean) * rstd;
+    if (p.weight != nullptr) v *= p.weight_offset + load_any(p.weight, p.dtype, e);
+    return p.bias == nullptr ? v : v + load_any(p.bias, p.dtype, e);
+  }
+};
+
+// One block a row; outputs are written in the last pass, so they may be the inputs themselves.
+__global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int dtype, int res_dtype) {
+  __shared__ float scratch[64];
+  grid_dependency_wait();
+  grid_dependency_trigger();
+  const int64_t t = blockIdx.x;
+  const int n = a.hidden;
+  BlockTeam team = {scratch};
+  const auto branch = [&](int e) { return load_any(a.y, dtype, t * a.ldy + e); };
+  const RowNorm post(a.post, n, team, branch);
+  const auto joined = [&](int e) {
+    float v = branch(e);
+    if (a.res == nullptr) return v;
+    v = post.apply(a.post, v, e);
+    if (a.gate.values != nullptr)
+      v *= gate_value(load_any(a.gate.values, a.gate.dtype,
+                               (t / a.gate.rows_each) * a.gate.ld + (a.gate.cols == 1 ? 0 : e)), a.gate.act);
+    return a.residual_scale * load_any(a.res, res_dtype, t * a.ld_res + e) + a.branch_scale * v;
+  };
+  const RowNorm next(a.next, n, team, joined);
+  RowScale s(0u);
+  if (a.out != nullptr && a.out_dtype == QCC_DTYPE_I8) {
+    uint32_t amax = 0;
+    for (int e = threadIdx.x; e < n; e += blockDim.x) amax = max(amax, magnitude(next.apply(a.next, joined(e), e)));
+    s = RowScale(team.max(amax));
+    if (threadIdx.x == 0) a.row_scale[t] = s.scale;
+  }
+  for (int e = threadIdx.x; e < n; e += blockDim.x) {
+    const float r = joined(e);
+    if (a.res != nullptr) store_as(a.res_out, t * a.ld_res_out + e, res_dtype, r);
+    if (a.out == nullptr) continue;
+    const float x = next.apply(a.next, r, e);
+    if (a.out_dtype == QCC_DTYPE_I8)
+      static_cast<int8_t*>(a.out)[t * a.ld_out + e] = s.inverse == 0.f ? 0 : to_int8(x, s.inverse);
+    else
+      store_as(a.out, t * a.ld_out + e, a.out_dtype, x);
+  }
+}
+
+// Bytes of a ring slot's part for a row of es-byte elements: its granules.
+__host__ __device__ __forceinline__ int slot_bytes(int hidden, int es) { return (hidden + 14) / 8 * 8 * es; }
+
+constexpr int kMaxDepth = 8;
+// Rows up to this many granules give a thread 2 of them, wider ones 4.
+constexpr int kRingNarrow = 2048;
+
+// The granules of row t that a bulk copy brings, [lo, hi): all of them, except that the partial granules at the two
+// ends of the tensor would read outside of it (inside the tensor they read a neighbour's elements, ignored).
+struct RowCopy {
+  int lo, hi;
+  __device__ __forceinline__ RowCopy(const BlockNormArgs& a, int64_t t, int shift) {
+    lo = t == 0 && shift != 0 ? 1 : 0;
+    hi = t == a.rows - 1 ? (a.hidden + shift) / 8 : (a.hidden + shift + 7) / 8;
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ void copy_row(uint8_t* slot, const E* row, const RowCopy& c, int shift, uint64_t* bar,
+                                         uint64_t policy) {
+  if (c.lo < c.hi)
+    bulk_load(slot + c.lo * 8 * sizeof(E), row + (c.lo * 8 - shift), static_cast<uint32_t>((c.hi - c.lo) * 8 * sizeof(E)),
+              bar, policy);
+}
+
+// Granule i of the row from the ring slot; the tensor's partial end granules from global memory.
+template <typename E, bool EXACT>
+__device__ __forceinline__ void load_slot8(const uint8_t* slot, const E* row, const RowCopy& c,
+                                           const GranuleMap<EXACT>& m, int i, float (&f)[8]) {
+  const int g = i * m.width + m.id;
+  if (EXACT) {
+    widen(load_granule(reinterpret_cast<const E*>(slot), m, i), f);
+    return;
+  }
+  if (g >= c.lo && g < c.hi)
+    widen(reinterpret_cast<const Granule<E>*>(slot)[g], f);
   else
-    QCC_LAUNCH(4);
-#undef QCC_LAUNCH
-  return launch_ok();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = m.has(i, j) ? to_f32<E>(row[m.element(i, j)]) : 0.f;
+  if (!m.whole(i))
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!m.has(i, j)) f[j] = 0.f;
+}
+
+template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
+__global__ void __launch_bounds__(1024) ring_kernel(const BlockNormArgs a, int depth) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kMaxDepth];
+  __shared__ float scratch[64];
+  const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + (JOIN ? slot_bytes(a.hidden, sizeof(R)) : 0);
+  const uint64_t policy = policy_evict_first();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  grid_dependency_trigger();
+  const T* y = static_cast<const T*>(a.y);
+  const R* res = static_cast<const R*>(a.res);
+  const auto fetch = [&](int64_t t, int s) {
+    const int shift = EXACT ? 0 : row_shift(a, t);
+    const RowCopy c(a, t, shift);
+    mbar_arrive_expect_tx(&full[s], max(0, c.hi - c.lo) * 8 * static_cast<int>(sizeof(T) + (JOIN ? sizeof(R) : 0)));
+    copy_row(ring + s * bytes, y + t * a.ldy, c, shift, &full[s], policy);
+    if (JOIN) copy_row(ring + s * bytes + y_bytes, res + t * a.ld_res, c, shift, &full[s], policy);
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < depth; ++s) {
+      const int64_t t = blockIdx.x + static_cast<int64_t>(s) * gridDim.x;
+      if (t < a.rows) fetch(t, s);
+    }
+  BlockTeam team = {scratch};
+  int s = 0, phase = 0;
+  for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
+    const int shift = EXACT ? 0 : row_shift(a, t);
+    const GranuleMap<EXACT> m = {a.hidden, shift, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    const RowCopy c(a, t, shift);
+    const uint8_t* slot = ring + s * bytes;
+    const bool arrived = mbar_wait_bounded(&full[s], phase, kWaitNs);
+    float v[VPT][8];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) load_slot8(slot, y + t * a.ldy, c, m, i, v[i]);
+    if (!arrived) v[0][0] = NAN;  // a row whose wait ran out becomes NaN by its sums
+    if (JOIN) {
+      normalise<T>(v, a.post, a.inv_hidden, m, team);
+      apply_gate<T>(v, a, t, m);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float r[8];
+        load_slot8(slot + y_bytes, res + t * a.ld_res, c, m, i, r);
+        join8<R>(v[i], r, a, t, m, i);
+      }
+    }
+    __syncthreads();  // the slot has been read
+    const int64_t ahead = t + static_cast<int64_t>(depth) * gridDim.x;
+    if (threadIdx.x == 0 && ahead < a.rows) fetch(ahead, s);
+    finish_row<T>(v, a, t, m, team);
+    if (++s == depth) s = 0, phase ^= 1;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+
+bool element_aligned(const void* p, int es) { return reinterpret_cast<uintptr_t>(p) % es == 0; }
+
+// Whether a tensor's rows (es-byte elements, ld apart) start on 16 bytes in the granules of x's rows.
+bool same_granules(const void* p, int64_t ld, int es, const BlockNormArgs& a) {
+  return (reinterpret_cast<uintptr_t>(p) - static_cast<uintptr_t>(a.shift0) * es) % 16 == 0 &&
+         (a.rows == 1 || ((ld - a.ldy) * es) % 16 == 0);
+}
+
+// A launch that may start while the launch ahead of it finishes.
+template <typename K, typename... A>
+bool launch_early(K kernel, unsigned grid, int threads, size_t smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
+bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t stream) {
+  auto* kernel = ring_kernel<T, R, JOIN, VPT, EXACT>;
+  if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return false;
+  const int threads = ((granules + VPT - 1) / VPT + 31) / 32 * 32;
+  const int slot = slot_bytes(a.hidden, sizeof(T)) + (JOIN ? slot_bytes(a.hidden, sizeof(R)) : 0);
+  // Blocks an SM: as many as their registers allow, with at least two rows each in 200 KB of ring; what is left
+  // deepens the rings.
+  static const int regs = [&] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? (attr.numRegs + 7) / 8 * 8 : 64;
+  }();
+  const int resident = std::max(1, std::min(65536 / (regs * threads), 2048 / threads));
+  const int blocks = std::max(1, std::min(resident, (200 << 10) / (2 * slot)));
+  const int64_t grid = std::min<int64_t>(a.rows, static_cast<int64_t>(device_info(device).num_sms) * blocks);
+  const int64_t each = (a.rows + grid - 1) / grid;
+  const int depth = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, (200 << 10) / (static_cast<int64_t>(blocks) * slot), each})));
+  return launch_early(kernel, static_cast<unsigned>(grid), threads, static_cast<size_t>(depth) * slot, stream, a, depth);
+}
+
+template <typename T, typename R, bool JOIN, bool EXACT>
+bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((a.rows + kWarpRows - 1) / kWarpRows);
+  if (granules <= 32) return launch_early(warp_kernel<T, R, JOIN, 1, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= 64) return launch_early(warp_kernel<T, R, JOIN, 2, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= 128) return launch_early(warp_kernel<T, R, JOIN, 4, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= kRingNarrow) return launch_ring<T, R, JOIN, 2, EXACT>(a, granules, device, stream);
+  return launch_ring<T, R, JOIN, 4, EXACT>(a, granules, device, stream);
+}
+
+template <typename T, typename R, bool JOIN>
+bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStream_t stream) {
+  constexpr int es = sizeof(T), rs = sizeof(R);
+  // The granule kernels take parameters, gates and outputs in T or fp32.
+  const auto known = [&](int d) { return d == dtype || d == QCC_DTYPE_F32; };
+  const auto known_norm = [&](const qcc_norm_params& p) {
+    return (p.weight == nullptr && p.bias == nullptr) || known(p.dtype);
+  };
+  a.inv_hidden = 1.f / static_cast<float>(a.hidden);
+  a.shift0 = static_cast<int>(reinterpret_cast<uintptr_t>(a.y) / es % 8);
+  const bool row_gate = a.gate.values != nullptr && a.gate.cols > 1;
+  const bool together =
+      known_norm(a.post) && known_norm(a.next) && (!row_gate || known(a.gate.dtype)) && same_granules(a.y, a.ldy, es, a) &&
+      (!JOIN || (same_granules(a.res, a.ld_res, rs, a) && same_granules(a.res_out, a.ld_res_out, rs, a))) &&
+      (a.out == nullptr || a.out_dtype == QCC_DTYPE_I8 ||
+       (known(a.out_dtype) && same_granules(a.out, a.ld_out, dtype_bytes(a.out_dtype), a)));
+  const bool shifted = a.shift0 != 0 || (a.rows > 1 && a.ldy % 8 != 0);
+  const int granules = (a.hidden + (shifted ? 14 : 7)) / 8;
+  if (!together || granules > 4096) {
+    const int threads = std::min(512, (a.hidden + 31) / 32 * 32);
+    return launch_early(plain_kernel, static_cast<unsigned>(a.rows), threads, 0, stream, a, dtype, res_dtype);
+  }
+  a.gate_in_granules =
+      row_gate && a.gate.rows_each == 1 && a.gate.dtype == dtype && same_granules(a.gate.values, a.gate.ld, es, a);
+  const bool gate_exact = !row_gate || a.gate_in_granules ||
+                          (aligned16(a.gate.values) && (a.gate.ld * dtype_bytes(a.gate.dtype)) % 16 == 0);
+  const bool exact = !shifted && a.hidden % 8 == 0 && aligned16(a.post.weight) && aligned16(a.post.bias) &&
+                     aligned16(a.next.weight) && aligned16(a.next.bias) && gate_exact &&
+                     (a.out == nullptr || a.out_dtype != QCC_DTYPE_I8 || (aligned16(a.out) && a.ld_out % 8 == 0));
+  return exact ? launch_granules<T, R, JOIN, true>(a, granules, device, stream)
+               : launch_granules<T, R, JOIN, false>(a, granules, device, stream);
 }
 
 bool valid_norm(const qcc_norm_params* p) {
@@ -338,21 +661,34 @@ bool valid_norm(const qcc_norm_params* p) {
          ((p->weight == nullptr && p->bias == nullptr) || valid_dtype(p->dtype));
 }
 
+bool norm_aligned(const qcc_norm_params& p) {
+  const int es = dtype_bytes(p.dtype);
+  return element_aligned(p.weight, es) && element_aligned(p.bias, es);
+}
+
 int run_block_norm(const BlockNormArgs& a, int dtype, int res_dtype, cudaStream_t stream) {
-  const int es = dtype_bytes(dtype), rs = dtype_bytes(res_dtype);
-  const bool vec = row_vectors(a.y, a.ldy, es) && row_vectors(a.res, a.ld_res, rs) &&
-                   row_vectors(a.res_out, a.ld_res_out, rs) && norm_vectors(a.post) && norm_vectors(a.next) &&
-                   (a.gate.cols == 1 || row_vectors(a.gate.values, a.gate.ld, dtype_bytes(a.gate.dtype))) &&
-                   row_vectors(a.out, a.ld_out, size_of(a.out_dtype));
+  if (!element_aligned(a.y, dtype_bytes(dtype)) || !element_aligned(a.res, dtype_bytes(res_dtype)) ||
+      !element_aligned(a.res_out, dtype_bytes(res_dtype)) || !norm_aligned(a.post) || !norm_aligned(a.next) ||
+      (a.gate.values != nullptr && !element_aligned(a.gate.values, dtype_bytes(a.gate.dtype))) ||
+      (a.out_dtype != QCC_DTYPE_I8 && !element_aligned(a.out, dtype_bytes(a.out_dtype))) ||
+      !element_aligned(a.row_scale, 4))
+    return QCC_ERR_ALIGNMENT;
+  int device = 0;
+  if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
+  const bool join = a.res != nullptr;
   bool ok;
+#define QCC_ROWS(T, R, J) launch_rows<T, R, J>(a, dtype, res_dtype, device, stream)
   if (dtype == QCC_DTYPE_BF16)
-    ok = res_dtype == QCC_DTYPE_F32 ? launch_block_norm<__nv_bfloat16, float>(a, vec, stream)
-                                    : launch_block_norm<__nv_bfloat16, __nv_bfloat16>(a, vec, stream);
+    ok = !join                        ? QCC_ROWS(__nv_bfloat16, __nv_bfloat16, false)
+         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__nv_bfloat16, float, true)
+                                      : QCC_ROWS(__nv_bfloat16, __nv_bfloat16, true);
   else if (dtype == QCC_DTYPE_F16)
-    ok = res_dtype == QCC_DTYPE_F32 ? launch_block_norm<__half, float>(a, vec, stream)
-                                    : launch_block_norm<__half, __half>(a, vec, stream);
+    ok = !join                        ? QCC_ROWS(__half, __half, false)
+         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__half, float, true)
+                                      : QCC_ROWS(__half, __half, true);
   else
-    ok = launch_block_norm<float, float>(a, vec, stream);
+    ok = join ? QCC_ROWS(float, float, true) : QCC_ROWS(float, float, false);
+#undef QCC_ROWS
   return ok ? QCC_OK : QCC_ERR_CUDA;
 }
 
