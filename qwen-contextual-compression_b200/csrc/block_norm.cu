@@ -89,8 +89,7 @@ struct alignas(16) Granule {
 
 template <typename T>
 __device__ __forceinline__ void widen(const Granule<T>& g, float (&f)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = to_f32<T>(g.e[j]);
+  widen(*reinterpret_cast<const Pack8<T>*>(&g), f);
 }
 
 // Granule i of a row (zeros outside of it): one wide load where all of it exists.
@@ -259,8 +258,11 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
     float w[8];
     if (a.weight != nullptr) {
       load_param8<T>(a.weight, a.dtype, m, i, w);
+      if (a.weight_offset != 0.f)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= rstd * (a.weight_offset + w[j]);
+        for (int j = 0; j < 8; ++j) w[j] += a.weight_offset;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * w[j];
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
@@ -463,8 +465,14 @@ __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int d
 __host__ __device__ __forceinline__ int slot_bytes(int hidden, int es) { return (hidden + 14) / 8 * 8 * es; }
 
 constexpr int kMaxDepth = 8;
-// Rows up to this many granules give a thread 2 of them, wider ones 4.
-constexpr int kRingNarrow = 2048;
+constexpr int kRoom = 208 << 10;  // shared memory that a ring kernel's blocks on an SM share
+
+// Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.
+template <bool JOIN, int VPT, bool EXACT>
+struct RingShape {
+  static constexpr int kThreads = VPT == 2 ? 640 : VPT == 4 ? 576 : 512;
+  static constexpr int kBlocks = EXACT && (VPT == 2 || (VPT == 4 && !JOIN)) ? 2 : 1;
+};
 
 // The granules of row t that a bulk copy brings, [lo, hi): all of them, except that the partial granules at the two
 // ends of the tensor would read outside of it (inside the tensor they read a neighbour's elements, ignored).
@@ -505,7 +513,8 @@ __device__ __forceinline__ void load_slot8(const uint8_t* slot, const E* row, co
 }
 
 template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
-__global__ void __launch_bounds__(1024) ring_kernel(const BlockNormArgs a, int depth) {
+__global__ void __launch_bounds__(RingShape<JOIN, VPT, EXACT>::kThreads, RingShape<JOIN, VPT, EXACT>::kBlocks)
+    ring_kernel(const BlockNormArgs a, int depth) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMaxDepth];
   __shared__ float scratch[64];
@@ -539,7 +548,7 @@ __global__ void __launch_bounds__(1024) ring_kernel(const BlockNormArgs a, int d
     const GranuleMap<EXACT> m = {a.hidden, shift, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
     const RowCopy c(a, t, shift);
     const uint8_t* slot = ring + s * bytes;
-    const bool arrived = mbar_wait_bounded(&full[s], phase, kWaitNs);
+    const bool arrived = mbar_wait_suspended(&full[s], phase, kWaitNs);
     float v[VPT][8];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) load_slot8(slot, y + t * a.ldy, c, m, i, v[i]);
@@ -596,18 +605,18 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
   if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return false;
   const int threads = ((granules + VPT - 1) / VPT + 31) / 32 * 32;
   const int slot = slot_bytes(a.hidden, sizeof(T)) + (JOIN ? slot_bytes(a.hidden, sizeof(R)) : 0);
-  // Blocks an SM: as many as their registers allow, with at least two rows each in 200 KB of ring; what is left
+  // Blocks an SM: as many as their registers allow, with at least two rows each in the ring's room; what is left
   // deepens the rings.
   static const int regs = [&] {
     cudaFuncAttributes attr;
-    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? (attr.numRegs + 7) / 8 * 8 : 64;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? (attr.numRegs + 7) / 8 * 8 : 128;
   }();
   const int resident = std::max(1, std::min(65536 / (regs * threads), 2048 / threads));
-  const int blocks = std::max(1, std::min(resident, (200 << 10) / (2 * slot)));
+  const int blocks = std::max(1, std::min(resident, kRoom / (2 * slot)));
   const int64_t grid = std::min<int64_t>(a.rows, static_cast<int64_t>(device_info(device).num_sms) * blocks);
   const int64_t each = (a.rows + grid - 1) / grid;
   const int depth = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, (200 << 10) / (static_cast<int64_t>(blocks) * slot), each})));
+      std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, kRoom / (static_cast<int64_t>(blocks) * slot), each})));
   return launch_early(kernel, static_cast<unsigned>(grid), threads, static_cast<size_t>(depth) * slot, stream, a, depth);
 }
 
@@ -617,8 +626,11 @@ bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStrea
   if (granules <= 32) return launch_early(warp_kernel<T, R, JOIN, 1, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
   if (granules <= 64) return launch_early(warp_kernel<T, R, JOIN, 2, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
   if (granules <= 128) return launch_early(warp_kernel<T, R, JOIN, 4, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
-  if (granules <= kRingNarrow) return launch_ring<T, R, JOIN, 2, EXACT>(a, granules, device, stream);
-  return launch_ring<T, R, JOIN, 4, EXACT>(a, granules, device, stream);
+  if (granules <= 2 * RingShape<JOIN, 2, EXACT>::kThreads)
+    return launch_ring<T, R, JOIN, 2, EXACT>(a, granules, device, stream);
+  if (granules <= 4 * RingShape<JOIN, 4, EXACT>::kThreads)
+    return launch_ring<T, R, JOIN, 4, EXACT>(a, granules, device, stream);
+  return launch_ring<T, R, JOIN, 8, EXACT>(a, granules, device, stream);
 }
 
 template <typename T, typename R, bool JOIN>
@@ -639,7 +651,8 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
        (known(a.out_dtype) && same_granules(a.out, a.ld_out, dtype_bytes(a.out_dtype), a)));
   const bool shifted = a.shift0 != 0 || (a.rows > 1 && a.ldy % 8 != 0);
   const int granules = (a.hidden + (shifted ? 14 : 7)) / 8;
-  if (!together || granules > 4096) {
+  const bool fits = granules <= 4096 && slot_bytes(a.hidden, es) + (JOIN ? slot_bytes(a.hidden, rs) : 0) <= kRoom;
+  if (!together || !fits) {
     const int threads = std::min(512, (a.hidden + 31) / 32 * 32);
     return launch_early(plain_kernel, static_cast<unsigned>(a.rows), threads, 0, stream, a, dtype, res_dtype);
   }

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(128)
     int issued = 0;
     for (; issued < count; ++issued) {
       const int s = issued % STAGES;
-      if (issued >= STAGES && !mbar_wait_bounded(&empty[s], (issued / STAGES - 1) & 1, kWaitNs)) {
+      if (issued >= STAGES && !mbar_wait_suspended(&empty[s], (issued / STAGES - 1) & 1, kWaitNs)) {
         failed = 1;
         break;
       }
@@ -209,12 +209,12 @@ __global__ void __launch_bounds__(128)
     // A copy must not land after this CTA has gone: after a wait that ran out, see the issued ones in.
     if (issued < count)
       for (int i = max(0, issued - STAGES); i < issued; ++i)
-        mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1, kWaitNs);
+        mbar_wait_suspended(&full[i % STAGES], (i / STAGES) & 1, kWaitNs);
   } else if (threadIdx.x == 32) {
     constexpr uint32_t idesc = idesc_s8(kTileRows, BN);
     for (int i = 0; i < count; ++i) {
       const int s = i % STAGES;
-      if (!mbar_wait_bounded(&full[s], (i / STAGES) & 1, kWaitNs)) {
+      if (!mbar_wait_suspended(&full[s], (i / STAGES) & 1, kWaitNs)) {
         failed = 1;
         break;
       }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(128)
     tc_commit(&done);
   }
   __syncwarp();
-  if (!mbar_wait_bounded(&done, 0, 4 * kWaitNs)) failed = 1;
+  if (!mbar_wait_suspended(&done, 0, 4 * kWaitNs)) failed = 1;
   tc_fence_after_sync();
   __syncthreads();
 
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       pair_tile(plan, i, row, token);
       for (int b = 0; b < blocks; ++b, ++n) {
         const int s = n % kPairStages;
-        if (n >= kPairStages && !mbar_wait_bounded(&empty[s], (n / kPairStages - 1) & 1, kWaitNs)) {
+        if (n >= kPairStages && !mbar_wait_suspended(&empty[s], (n / kPairStages - 1) & 1, kWaitNs)) {
           ok = false;
           break;
         }
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // Copies in flight land before the cluster's last barrier: the even CTA's barriers count both CTAs' bytes.
       if (rank == 0)
         for (int i = max(0, n - kPairStages); i < n; ++i)
-          mbar_wait_bounded(&full[i % kPairStages], (i / kPairStages) & 1, kWaitNs);
+          mbar_wait_suspended(&full[i % kPairStages], (i / kPairStages) & 1, kWaitNs);
     }
   } else if (threadIdx.x == 32 && rank == 0) {
     const uint32_t idesc = idesc_s8(256, plan.tile_tokens);
@@ -396,14 +396,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     bool ok = true;
     for (int i = pair; i < tiles && ok; i += pairs, ++done) {
       const int acc = done & 1;
-      if (done >= 2 && !mbar_wait_bounded(&acc_empty[acc], (done / 2 - 1) & 1, kWaitNs)) {
+      if (done >= 2 && !mbar_wait_suspended(&acc_empty[acc], (done / 2 - 1) & 1, kWaitNs)) {
         ok = false;
         break;
       }
       tc_fence_after_sync();
       for (int b = 0; b < blocks; ++b, ++n) {
         const int s = n % kPairStages;
-        if (!mbar_wait_bounded(&full[s], (n / kPairStages) & 1, kWaitNs)) {
+        if (!mbar_wait_suspended(&full[s], (n / kPairStages) & 1, kWaitNs)) {
           ok = false;
           break;
         }
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int done = 0;
     for (int i = pair; i < tiles; i += pairs, ++done) {
       const int acc = done & 1;
-      if (failed || !mbar_wait_bounded(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) failed = 1;
+      if (failed || !mbar_wait_suspended(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) failed = 1;
       tc_fence_after_sync();
       int row, token;
       pair_tile(plan, i, row, token);

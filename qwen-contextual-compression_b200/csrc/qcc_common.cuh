@@ -72,6 +72,26 @@ __device__ __forceinline__ void grid_dependency_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// The same wait for threads that have nothing else to do: each try lets the
+// hardware suspend the thread (for up to 100 us), so that waiting warps leave
+// the issue slots to the working ones.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    if (done != 0) return true;
+    if (global_timer_ns() - start > limit_ns) return false;
+  }
+}
+
 // Cache policy for data that later reads of the same kernel should find in L2.
 __device__ __forceinline__ uint64_t policy_evict_last() {
   uint64_t p;

@@ -157,7 +157,7 @@ GATES = [None, "token", "channel", "full", "scalar"]
                                              (torch.float16, torch.float16), (torch.float16, torch.float32),
                                              (torch.float32, torch.float32)])
 @pytest.mark.parametrize("gate", GATES)
-@pytest.mark.parametrize("rows,hidden", [(1, 5120), (3, 1111), (65, 256), (2, 9000)])
+@pytest.mark.parametrize("rows,hidden", [(1, 5120), (3, 1111), (65, 256), (2, 9000), (2, 20000), (1, 32768)])
 def test_join_matches_formula(rows, hidden, gate, dtype, res_dtype):
     branch, residual = make((rows, hidden), dtype, 1), make((rows, hidden), res_dtype, 2, 3.0)
     shape = {None: None, "token": (rows, 1), "channel": (hidden,), "full": (rows, hidden), "scalar": (1,)}[gate]
