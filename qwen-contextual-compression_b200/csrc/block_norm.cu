@@ -82,27 +82,39 @@ struct GranuleMap {
   }
 };
 
-template <typename T>
-struct alignas(16) Granule {
-  T e[8];
-};
+__device__ __forceinline__ uint32_t half_bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ uint32_t half_bits(__half v) { return __half_as_ushort(v); }
 
+// Elements as a granule's words.
 template <typename T>
-__device__ __forceinline__ void widen(const Granule<T>& g, float (&f)[8]) {
-  widen(*reinterpret_cast<const Pack8<T>*>(&g), f);
+__device__ __forceinline__ Pack8<T> to_words(const T (&e)[8]) {
+  Pack8<T> p;
+  p.w[0] = make_uint4(half_bits(e[0]) | half_bits(e[1]) << 16, half_bits(e[2]) | half_bits(e[3]) << 16,
+                      half_bits(e[4]) | half_bits(e[5]) << 16, half_bits(e[6]) | half_bits(e[7]) << 16);
+  return p;
+}
+__device__ __forceinline__ Pack8<float> to_words(const float (&e)[8]) {
+  Pack8<float> p;
+  p.w[0] = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+  p.w[1] = make_uint4(__float_as_uint(e[4]), __float_as_uint(e[5]), __float_as_uint(e[6]), __float_as_uint(e[7]));
+  return p;
 }
 
-// Granule i of a row (zeros outside of it): one wide load where all of it exists.
+// Granule i of a row (zeros outside of it): one wide load where all of it exists.  Kept as words: 16-bit elements
+// held one by one would be taken apart and put together again.
 template <typename T, bool EXACT>
-__device__ __forceinline__ Granule<T> load_granule(const T* row, const GranuleMap<EXACT>& m, int i) {
-  Granule<T> g;
-  if (m.whole(i)) {
-    g = *reinterpret_cast<const Granule<T>*>(row + m.first(i));
-  } else {
+__device__ __forceinline__ Pack8<T> load_granule(const T* row, const GranuleMap<EXACT>& m, int i) {
+  if (m.whole(i)) return load_pack8<T>(row + m.first(i));
+  if (!EXACT) {
+    T e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g.e[j] = !EXACT && m.has(i, j) ? row[m.element(i, j)] : T(0.f);
+    for (int j = 0; j < 8; ++j) e[j] = m.has(i, j) ? row[m.element(i, j)] : T(0.f);
+    return to_words(e);
   }
-  return g;
+  Pack8<T> p;
+#pragma unroll
+  for (int k = 0; k < Pack8<T>::kWords; ++k) p.w[k] = make_uint4(0, 0, 0, 0);
+  return p;
 }
 
 // A parameter vector's elements of granule i.  Without EXACT its alignment is not the row's: single elements.
@@ -373,8 +385,8 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArg
   if (t >= a.rows) return;
   const GranuleMap<EXACT> m = {a.hidden, EXACT ? 0 : row_shift(a, t), static_cast<int>(threadIdx.x & 31), 32};
   WarpTeam team;
-  Granule<T> y[VPT];
-  Granule<R> r[VPT];
+  Pack8<T> y[VPT];
+  Pack8<R> r[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) y[i] = load_granule(static_cast<const T*>(a.y) + t * a.ldy, m, i);
   if (JOIN)
@@ -465,7 +477,9 @@ __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int d
 __host__ __device__ __forceinline__ int slot_bytes(int hidden, int es) { return (hidden + 14) / 8 * 8 * es; }
 
 constexpr int kMaxDepth = 8;
-constexpr int kRoom = 208 << 10;  // shared memory that a ring kernel's blocks on an SM share
+// Shared memory that a ring kernel's blocks on an SM share: two rows each in kRoom, more rows each only within
+// kDeepRoom (what is left caches the parameters: 208 KB of rings cost the norm of 8192 x 5120 rows 10 %).
+constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
 
 // Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.
 template <bool JOIN, int VPT, bool EXACT>
@@ -502,7 +516,7 @@ __device__ __forceinline__ void load_slot8(const uint8_t* slot, const E* row, co
     return;
   }
   if (g >= c.lo && g < c.hi)
-    widen(reinterpret_cast<const Granule<E>*>(slot)[g], f);
+    widen(load_pack8<E>(reinterpret_cast<const E*>(slot) + g * 8), f);
   else
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = m.has(i, j) ? to_f32<E>(row[m.element(i, j)]) : 0.f;
@@ -615,8 +629,8 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
   const int blocks = std::max(1, std::min(resident, kRoom / (2 * slot)));
   const int64_t grid = std::min<int64_t>(a.rows, static_cast<int64_t>(device_info(device).num_sms) * blocks);
   const int64_t each = (a.rows + grid - 1) / grid;
-  const int depth = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, kRoom / (static_cast<int64_t>(blocks) * slot), each})));
+  const int rows_each = std::max(kDeepRoom / (blocks * slot), std::min(2, kRoom / (blocks * slot)));
+  const int depth = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, rows_each, each})));
   return launch_early(kernel, static_cast<unsigned>(grid), threads, static_cast<size_t>(depth) * slot, stream, a, depth);
 }
 

@@ -9,7 +9,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "qcc_common.cuh"
 #include "qcc_host.h"
@@ -294,6 +293,7 @@ constexpr int kPairTokens = 256;                       // most tokens of a tile
 constexpr int kPairStage = 2 * 128 * kTileCols;        // bytes a CTA loads per stage, at most
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage;
 constexpr int kPairThreads = 320;
+constexpr int kPairGroup = 8;  // token tiles walked through together (4096 tokens: 4, 8 or 16 within 4 %)
 
 struct PairPlan {
   int row_tiles, token_tiles, tile_tokens;  // tile_tokens: multiple of 32, up to kPairTokens
@@ -482,13 +482,14 @@ bool make_map(CUtensorMap* map, const int8_t* base, int64_t rows, int64_t cols, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The gate and the up rows of a fused weight as two planes: a box holds box_rows rows of each.
-bool make_gated_map(CUtensorMap* map, const int8_t* base, int64_t channels, int64_t cols, int64_t ld, int box_rows) {
+// The gate and the up rows of a fused weight as two planes: a box holds 16 rows of each, one warp's 32 lanes (one copy
+// for both: two copies of 16 rows took 15 % longer at 4096 tokens).
+bool make_gated_map(CUtensorMap* map, const int8_t* base, int64_t channels, int64_t cols, int64_t ld) {
   auto fn = encode_tiled();
   if (fn == nullptr) return false;
   const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(channels), 2};
   const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(channels * ld)};
-  const uint32_t box[3] = {kTileCols, static_cast<uint32_t>(box_rows), 2}, elem[3] = {1, 1, 1};
+  const uint32_t box[3] = {kTileCols, 16, 2}, elem[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(base), dims, strides, box, elem,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -522,15 +523,18 @@ int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
   auto* kernel = int8_stream_kernel<GATED, O, BN, STAGES>;
   CUtensorMap tm_x, tm_w;
   if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, BN) ||
-      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 16)
+      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw)
               : make_map(&tm_w, a.w, a.channels, a.cols, a.ldw, kTileRows)))
     return QCC_ERR_UNSUPPORTED;
   if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
   const int tiles = (a.channels + kChannels - 1) / kChannels, token_tiles = (a.tokens + BN - 1) / BN;
-  const int64_t slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kSmem + 2048));
+  // Columns are split while all CTAs still run at once: a second wave costs more than the split brings (17408 columns
+  // to 5120 channels, 32 tokens, two CTAs an SM: 240 CTAs 19.1 us, 320 CTAs 25.2 us).  Clusters leave part of a
+  // GPC's slots empty, hence 85 %.
+  const int slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kSmem + 2048)) * 85 / 100;
   const int blocks = (a.cols + kTileCols - 1) / kTileCols;
-  int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, blocks, slots * 85 / 100 / (static_cast<int64_t>(tiles) * token_tiles)})));
-  if (getenv("QS")) split = atoi(getenv("QS"));
+  const int split = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>({8, blocks, slots / (static_cast<int64_t>(tiles) * token_tiles)})));
   return launch_clusters(kernel, dim3(tiles * split, token_tiles), 128, S::kSmem, split, stream, a, tm_x, tm_w);
 }
 
@@ -541,39 +545,42 @@ int launch_pair(const Int8Args& a, int device, cudaStream_t stream) {
   const int pairs = device_info(device).num_sms / 2;
   PairPlan plan;
   plan.row_tiles = (a.channels + channels - 1) / channels;
-  // As few token tiles as fit, of equal width: a tile's time hardly falls with its width (its weight rows' loads stay).
+  // As few token tiles as fit, of equal width: a tile's time hardly falls with its width (4096 tokens of the 34816 x
+  // 5120 gated product: 702 us at 256 wide, 889 at 192, 1240 at 128), its weight rows' loads stay.
   plan.token_tiles = (a.tokens + kPairTokens - 1) / kPairTokens;
   plan.tile_tokens = ((a.tokens + plan.token_tiles - 1) / plan.token_tiles + 31) / 32 * 32;
-  plan.group = 8;
+  plan.group = kPairGroup;
   CUtensorMap tm_x, tm_w;
   if (!make_map(&tm_x, a.x, a.tokens, a.cols, a.ldx, plan.tile_tokens / 2) ||
-      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 16)
+      !(GATED ? make_gated_map(&tm_w, a.w, a.channels, a.cols, a.ldw)
               : make_map(&tm_w, a.w, a.channels, a.cols, a.ldw, 128)))
     return QCC_ERR_UNSUPPORTED;
   if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return QCC_ERR_CUDA;
-  const unsigned grid = 2u * static_cast<unsigned>(std::min<int64_t>(pairs, static_cast<int64_t>(plan.row_tiles) * plan.token_tiles));
+  const unsigned grid = 2u * static_cast<unsigned>(std::min<int64_t>(
+                                 pairs, static_cast<int64_t>(plan.row_tiles) * plan.token_tiles));
   return launch_clusters(kernel, dim3(grid), kPairThreads, kPairSmem, 2, stream, a, plan, tm_x, tm_w);
+}
+
+// Bytes that the stream kernel's CTAs load with tiles of `bn` tokens.
+int64_t stream_loads(const Int8Args& a, bool gated, int bn) {
+  const int64_t tiles = static_cast<int64_t>((a.channels + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((a.tokens + bn - 1) / bn);
+  return tiles * ((a.cols + kTileCols - 1) / kTileCols) * (kTileRows + bn) * kTileCols;
 }
 
 template <bool GATED, typename O>
 int launch(const Int8Args& a, int device, cudaStream_t stream) {
-  const char* v = getenv("QV");
-  if (v) {
-    switch (atoi(v)) {
-      case 16: return launch_stream<GATED, O, 16, 4>(a, device, stream);
-      case 32: return launch_stream<GATED, O, 32, 4>(a, device, stream);
-      case 323: return launch_stream<GATED, O, 32, 3>(a, device, stream);
-      case 64: return launch_stream<GATED, O, 64, 4>(a, device, stream);
-      case 128: return launch_stream<GATED, O, 128, 3>(a, device, stream);
-      case 256: return launch_stream<GATED, O, 256, 4>(a, device, stream);
-      default: return launch_pair<GATED, O>(a, device, stream);
-    }
-  }
   if (a.tokens <= 16) return launch_stream<GATED, O, 16, 4>(a, device, stream);
   if (a.tokens <= 32) return launch_stream<GATED, O, 32, 4>(a, device, stream);
   if (a.tokens <= 64) return launch_stream<GATED, O, 64, 4>(a, device, stream);
-  if (a.tokens <= 128) return launch_stream<GATED, O, 128, 3>(a, device, stream);
-  return launch_pair<GATED, O>(a, device, stream);
+  // Pairs where their tiles fill at least half of the SMs (512 tokens, 17408 columns to 5120 channels, 40 tiles: pairs
+  // 55 us, stream 60 us; 256 tokens, 20 tiles: 58 and 33 us).
+  const int channels = GATED ? 128 : 256;
+  const int64_t pair_tiles = static_cast<int64_t>((a.channels + channels - 1) / channels) * ((a.tokens + kPairTokens - 1) / kPairTokens);
+  if (a.tokens > 128 && 4 * pair_tiles >= device_info(device).num_sms) return launch_pair<GATED, O>(a, device, stream);
+  // Narrow token tiles make more CTAs, wide ones load the weight less often (200 tokens of a 4000 x 4000 weight, 98 MB
+  // of loads at 64: 13.2 us, at 128 15.1 us; 256 tokens of 17408 columns to 5120 channels, 522 MB: 52 and 33 us).
+  if (stream_loads(a, GATED, 64) <= (128 << 20)) return launch_stream<GATED, O, 64, 4>(a, device, stream);
+  return launch_stream<GATED, O, 128, 3>(a, device, stream);
 }
 
 template <bool GATED>
@@ -591,7 +598,11 @@ int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
   if (a.tokens == 0) return QCC_OK;
   if (a.x == nullptr || a.xs == nullptr || a.w == nullptr || a.ws == nullptr || a.y == nullptr)
     return QCC_ERR_INVALID_ARGUMENT;
-  if (!aligned16(a.x) || !aligned16(a.w) || a.ldx % 16 != 0 || a.ldw % 16 != 0) return QCC_ERR_ALIGNMENT;
+  const auto misaligned = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
+  if (!aligned16(a.x) || !aligned16(a.w) || a.ldx % 16 != 0 || a.ldw % 16 != 0 || misaligned(a.xs, 4) ||
+      misaligned(a.ws, 4) || misaligned(a.y, dtype_bytes(a.y_dtype)) ||
+      (a.bias != nullptr && misaligned(a.bias, dtype_bytes(a.bias_dtype))))
+    return QCC_ERR_ALIGNMENT;
   int device = 0;
   if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
   clear_stale_error();

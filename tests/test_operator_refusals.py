@@ -34,6 +34,9 @@ def norm_args(**changed):
     (dict(hidden=0), _lib.ERR_SHAPE), (dict(ldx=63), _lib.ERR_SHAPE), (dict(ld_out=63), _lib.ERR_SHAPE),
     (dict(hidden=32769, ldx=32769, ld_out=32769), _lib.ERR_UNSUPPORTED), (dict(x=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(out=None), _lib.ERR_INVALID_ARGUMENT), (dict(out_dtype=I8), _lib.ERR_INVALID_ARGUMENT),
+    (dict(x=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT), (dict(out=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
+    (dict(norm=params(weight=65)), _lib.ERR_ALIGNMENT), (dict(norm=params(bias=66, dtype=F32)), _lib.ERR_ALIGNMENT),
+    (dict(out_dtype=I8, scale=ctypes.c_void_p(66)), _lib.ERR_ALIGNMENT),
     (dict(rows=0, x=None, out=None, norm=None), _lib.OK)])
 def test_norm_rows_status(changed, status):
     assert _lib.library().qcc_norm_rows(*norm_args(**changed)) == status
@@ -59,7 +62,8 @@ def join_args(**changed):
     (dict(gate=gate(dtype=I8)), _lib.ERR_DTYPE), (dict(gate=gate(act=3)), _lib.ERR_INVALID_ARGUMENT),
     (dict(gate=gate(each=0)), _lib.ERR_SHAPE), (dict(gate=gate(cols=32)), _lib.ERR_SHAPE),
     (dict(gate=gate(ld=-1)), _lib.ERR_SHAPE), (dict(gate=gate(values=None)), _lib.ERR_INVALID_ARGUMENT),
-    (dict(out=P, ld_out=60), _lib.ERR_SHAPE),
+    (dict(out=P, ld_out=60), _lib.ERR_SHAPE), (dict(gate=gate(values=65)), _lib.ERR_ALIGNMENT),
+    (dict(residual=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT), (dict(residual_out=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
     (dict(out=P, ld_out=64, out_dtype=I8), _lib.ERR_INVALID_ARGUMENT), (dict(residual=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(residual_out=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(hidden=40000, ld_branch=40000, ld_residual=40000, ld_residual_out=40000), _lib.ERR_UNSUPPORTED),
@@ -84,6 +88,8 @@ def linear_args(**changed):
     (dict(x=None), _lib.ERR_INVALID_ARGUMENT), (dict(ws=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(y=None), _lib.ERR_INVALID_ARGUMENT), (dict(ldx=72), _lib.ERR_ALIGNMENT), (dict(ldw=72), _lib.ERR_ALIGNMENT),
     (dict(x=ctypes.c_void_p(72)), _lib.ERR_ALIGNMENT), (dict(w=ctypes.c_void_p(72)), _lib.ERR_ALIGNMENT),
+    (dict(xs=ctypes.c_void_p(66)), _lib.ERR_ALIGNMENT), (dict(ws=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
+    (dict(y=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
     (dict(tokens=0, x=None, y=None), _lib.OK)])
 def test_int8_linear_status(changed, status):
     lib = _lib.library()
