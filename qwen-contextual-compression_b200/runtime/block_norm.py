@@ -62,8 +62,9 @@ def _out_rows(out: torch.Tensor, shape: torch.Size, rows: int, dtype: torch.dtyp
 def int8_rows(rows: int, cols: int, device: torch.device) -> torch.Tensor:
     """Uninitialised int8 [rows, cols] whose rows start on multiples of 16 bytes."""
     pad = -cols % 16
-    q = torch.empty((rows, cols + pad), dtype=torch.int8, device=device)
-    return q[:, :cols] if pad else q
+    if pad:
+        return torch.empty_strided((rows, cols), (cols + pad, 1), dtype=torch.int8, device=device)
+    return torch.empty(rows, cols, dtype=torch.int8, device=device)
 
 
 class BlockNorm:

@@ -28,30 +28,30 @@ MAX_TOKENS = 1 << 20
 MAX_CHANNELS = 1 << 19
 
 
-def _int8_operand(q: torch.Tensor, scale: torch.Tensor, what: str) -> int:
-    """Checks an int8 matrix with its row scales; returns the row stride."""
+def _int8_operand(q: torch.Tensor, scale: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """Checks an int8 matrix with its row scales; returns its rows, columns and row stride."""
     if q.dim() != 2 or q.dtype != torch.int8:
         raise ValueError(f"{what} must be an int8 matrix")
-    (rows, cols), (ld, step) = q.shape, q.stride()
+    rows, cols = q.shape
+    ld, step = q.stride()
     if step != 1 and cols != 1:
         raise ValueError(f"{what} must be contiguous along its columns")
-    if scale.dtype != torch.float32 or scale.dim() != 1 or scale.shape[0] != rows or not scale.is_contiguous():
+    if scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous():
         raise ValueError(f"the scales of {what} must be a contiguous float32 tensor with one value per row")
     if rows <= 1:
         ld = cols + -cols % 16
     if ld % 16 or q.data_ptr() % 16 or ld < cols:
         raise ValueError(f"the rows of {what} must start on multiples of 16 bytes (quantize_rows stores them so)")
-    return ld
+    return rows, cols, ld
 
 
 def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
-    ldx, ldw = _int8_operand(xq, x_scale, "x"), _int8_operand(wq, w_scale, "w")
+    tokens, cols, ldx = _int8_operand(xq, x_scale, "x")
+    rows, w_cols, ldw = _int8_operand(wq, w_scale, "w")
     index = xq.get_device()
     if (index < 0 or x_scale.get_device() != index or wq.get_device() != index or w_scale.get_device() != index
             or (bias is not None and bias.get_device() != index) or (out is not None and out.get_device() != index)):
         _lib.require_cuda(xq, x_scale, wq, w_scale, bias, out)
-    tokens, cols = xq.shape
-    rows, w_cols = wq.shape
     if w_cols != cols:
         raise ValueError(f"x has {cols} columns, w {w_cols}")
     if gated and rows % 2:
@@ -65,7 +65,7 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
     if out is None:
         out_dtype = out_dtype or torch.bfloat16
         y_code = _lib.dtype_code(out_dtype)
-        out = torch.empty((tokens, channels), dtype=out_dtype, device=xq.device)
+        out = torch.empty(tokens, channels, dtype=out_dtype, device=xq.device)
         ldy = channels
     else:
         y_code = _lib.dtype_code(out.dtype)

@@ -26,12 +26,9 @@ DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 def int8_matrix(rows, cols, seed, low=-128, high=127):
     gen = torch.Generator().manual_seed(seed)
-    q = int8_rows(rows, cols, torch.device("cuda"))
-    if q.numel():
-        whole = q.as_strided((rows, q.stride(0)), (q.stride(0), 1))
-        whole.copy_(torch.randint(-128, 128, whole.shape, generator=gen, dtype=torch.int8))  # the padding holds values
-        q.copy_(torch.randint(low, high + 1, (rows, cols), generator=gen, dtype=torch.int8))
-    return q
+    whole = torch.randint(-128, 128, (rows, (cols + 15) // 16 * 16), generator=gen, dtype=torch.int8)
+    whole[:, :cols] = torch.randint(low, high + 1, (rows, cols), generator=gen, dtype=torch.int8)
+    return whole.cuda()[:, :cols]  # the padding holds values
 
 
 def scales(n, seed, size=1.0):
