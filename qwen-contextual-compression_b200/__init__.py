@@ -10,6 +10,8 @@ surface:
   ``validate_selected_ids`` (reference runtime/cuda_indexed.py)
 * ``qcc_b200.runtime.ffn``           -- ``TorchDynamicSparseFFN`` (reference runtime/ffn.py)
 * ``qcc_b200.runtime.selector``      -- deterministic top-K selection (reference runtime/selector.py)
+* ``qcc_b200.runtime.block_norm``, ``.int8_dense``, ``.block`` -- the norms around an FFN block, the dense FFN in
+  8-bit integers, and a layer's FFN half built from them
 * ``qcc_b200.runtime.sharded``       -- intermediate-dimension sharding over GPUs
 * ``qcc_b200.end_to_end``            -- ``OracleSparseMLP``, ``OracleMLPPatcher``
 

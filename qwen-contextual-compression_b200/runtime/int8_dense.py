@@ -21,7 +21,7 @@ import torch
 
 from .. import _lib
 from .block_norm import int8_rows, quantize_rows
-from .packing import validate_weight_shapes
+from .packing import PackedFFNWeights, validate_weight_shapes
 
 MAX_COLS = 131071       # |q| <= 128: the int32 sums cannot overflow
 MAX_TOKENS = 1 << 20
@@ -175,6 +175,12 @@ class Int8GatedLinear(Int8Linear):
             weight[begin:begin + n] = q
             scale[begin:begin + n] = s
         return cls(weight, scale)
+
+    @classmethod
+    def from_packed(cls, weights: PackedFFNWeights) -> "Int8GatedLinear":
+        """From the gate and up parts of packed records (``OracleModeFFN(..., gate_up=...)`` takes the result)."""
+        h, hp = weights.hidden, weights.hidden_pad
+        return cls.from_weights(weights.packed[:, :h], weights.packed[:, hp:hp + h])
 
     @classmethod
     def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Int8GatedLinear":

@@ -21,6 +21,10 @@ Here one layer is three kinds of launch per chunk of tokens:
 
 So a token reads 2/3 of the layer plus K/N of the last third, instead of the
 whole layer twice over as the masked-dense formulation does.
+
+With ``gate_up=Int8GatedLinear.from_packed(weights)`` step 1 is the int8 gated
+product (``runtime.int8_dense``): every token of the call in one launch, from
+half of the bytes, with activations within int8's error of the records' own.
 """
 from __future__ import annotations
 
@@ -28,6 +32,7 @@ import torch
 
 from .. import _lib
 from .engine import _current_stream, stream_workspace
+from .int8_dense import Int8GatedLinear
 from .packing import PackedFFNWeights
 from .selector import activation_topk, build_union, retention_count
 
@@ -46,12 +51,20 @@ def down_column_norms(weights: PackedFFNWeights) -> torch.Tensor:
 
 
 class OracleModeFFN:
-    """``(y, ids) = OracleModeFFN(weights, retention)(x)`` for x [T, hidden]."""
+    """``(y, ids) = OracleModeFFN(weights, retention)(x)`` for x [T, hidden].
+
+    ``gate_up``: optional int8 form of the same gate and up rows, which then
+    makes the activations (the down pass keeps the packed records).
+    """
 
     def __init__(self, weights: PackedFFNWeights, retention: float, score: str = "weighted_activation",
-                 column_weights: torch.Tensor | None = None):
+                 column_weights: torch.Tensor | None = None, gate_up: Int8GatedLinear | None = None):
         if score not in SCORES:
             raise ValueError(f"score must be one of {SCORES}")
+        if gate_up is not None and (not gate_up.gated or gate_up.cols != weights.hidden
+                                    or gate_up.rows != 2 * weights.n_records):
+            raise ValueError(f"gate_up must be a gated int8 weight [{2 * weights.n_records}, {weights.hidden}]")
+        self.gate_up = gate_up
         self.weights = weights
         self.retention = float(retention)
         self.k = retention_count(weights.n_records, retention)
@@ -74,6 +87,8 @@ class OracleModeFFN:
         if x.ndim != 2 or x.shape[1] != w.hidden or x.dtype != w.dtype:
             raise ValueError(f"x must be [tokens, {w.hidden}] in {w.dtype}")
         _lib.require_cuda(x, w.packed)
+        if self.gate_up is not None:
+            return self.gate_up(x, out_dtype=torch.float32)
         x = x.contiguous()
         n = w.n_records
         acts = torch.empty((x.shape[0], n), dtype=torch.float32, device=x.device)
