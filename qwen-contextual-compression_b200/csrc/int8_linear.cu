@@ -61,6 +61,7 @@ __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) 
 
 constexpr int kTileRows = 128;  // weight rows of a CTA's tile: TMEM lanes
 constexpr int kTileCols = 128;  // bytes of K per stage (one swizzled row)
+constexpr uint32_t kMaxSplit = 8;  // CTAs of a stream kernel's cluster, at most
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 // What one lane needs to finish its weight row's outputs.
@@ -259,17 +260,29 @@ __global__ void __launch_bounds__(128)
     __syncwarp();
     cluster_sync();
     tc_fence_after_sync();
-    int any = 0;
-    for (uint32_t r = 0; r < splits; ++r) any |= cluster_load(smem_addr(&failed), r);
+    // Remote loads take about 250 cycles: those of all ranks are in flight together.
     const uint32_t base = smem_addr(partial) + threadIdx.x * 4;
-    const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, any != 0);
+    int flags[kMaxSplit];
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxSplit; ++r) flags[r] = r < splits ? cluster_load(smem_addr(&failed), r) : 0;
+    int any = 0;
     constexpr int kRun = 4;  // tokens a warp sums at a time; the cluster's CTAs take runs in turn
     for (int c = static_cast<int>(rank) * kRun; c < tokens; c += static_cast<int>(splits) * kRun) {
       const float xs = lane < kRun && c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
-      int acc[kRun] = {};
-      for (uint32_t r = 0; r < splits; ++r)
+      int part[kMaxSplit][kRun];
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) acc[j] += cluster_load(base + (c + j) * kTileRows * 4, r);
+      for (uint32_t r = 0; r < kMaxSplit; ++r)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j)
+          part[r][j] = r < splits && c + j < tokens ? cluster_load(base + (c + j) * kTileRows * 4, r) : 0;
+      int acc[kRun] = {};
+#pragma unroll
+      for (uint32_t r = 0; r < kMaxSplit; ++r) {
+        any |= flags[r];
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) acc[j] += part[r][j];
+      }
+      const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, any != 0);
       out.finish(acc, c, tokens, xs, lane);
     }
     __syncwarp();
@@ -534,7 +547,7 @@ int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
   const int slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kSmem + 2048)) * 85 / 100;
   const int blocks = (a.cols + kTileCols - 1) / kTileCols;
   const int split = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>({8, blocks, slots / (static_cast<int64_t>(tiles) * token_tiles)})));
+      std::max<int64_t>(1, std::min<int64_t>({kMaxSplit, blocks, slots / (static_cast<int64_t>(tiles) * token_tiles)})));
   return launch_clusters(kernel, dim3(tiles * split, token_tiles), 128, S::kSmem, split, stream, a, tm_x, tm_w);
 }
 
