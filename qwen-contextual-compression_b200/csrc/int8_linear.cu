@@ -323,6 +323,13 @@ __device__ __forceinline__ void pair_tile(const PairPlan& p, int i, int& row, in
   token = g * p.group + in - row * width;
 }
 
+// Notes a wait that ran out in both CTAs of the pair, before the commits that follow.
+__device__ __forceinline__ void note_failure(int* failed, uint32_t rank) {
+  *static_cast<volatile int*>(failed) = 1;
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(cluster_addr(failed, rank ^ 1u)), "r"(1)
+               : "memory");
+}
+
 template <bool GATED, typename O>
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const Int8Args a, const PairPlan plan, const __grid_constant__ CUtensorMap tm_x,
@@ -330,7 +337,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int failed;
+  __shared__ int failed;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
@@ -397,7 +404,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
     if (!ok) {
-      failed = 1;
+      note_failure(&failed, rank);
       // Copies in flight land before the cluster's last barrier: the even CTA's barriers count both CTAs' bytes.
       if (rank == 0)
         for (int i = max(0, n - kPairStages); i < n; ++i)
@@ -410,6 +417,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int i = pair; i < tiles && ok; i += pairs, ++done) {
       const int acc = done & 1;
       if (done >= 2 && !mbar_wait_suspended(&acc_empty[acc], (done / 2 - 1) & 1, kWaitNs)) {
+        note_failure(&failed, rank);
         ok = false;
         break;
       }
@@ -417,6 +425,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int b = 0; b < blocks; ++b, ++n) {
         const int s = n % kPairStages;
         if (!mbar_wait_suspended(&full[s], (n / kPairStages) & 1, kWaitNs)) {
+          note_failure(&failed, rank);
           ok = false;
           break;
         }
@@ -430,20 +439,21 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_commit_pair(&acc_full[acc]);
     }
-    if (!ok) failed = 1;
   } else if (warp >= 2) {
     const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
     int done = 0;
+    bool broken = false;
     for (int i = pair; i < tiles; i += pairs, ++done) {
       const int acc = done & 1;
-      if (failed || !mbar_wait_suspended(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) failed = 1;
+      if (!broken && !mbar_wait_suspended(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) note_failure(&failed, rank);
+      broken = *static_cast<volatile int*>(&failed) != 0;  // and all tiles after it: their waits would run out too
       tc_fence_after_sync();
       int row, token;
       pair_tile(plan, i, row, token);
       const int t0 = token * plan.tile_tokens, tokens = min(plan.tile_tokens, a.tokens - t0);
       const RowOutput<GATED, O> out(
           a, row * kChannels + static_cast<int>(rank) * (kChannels / 2) + quarter * (GATED ? 16 : 32), t0, lane,
-          failed != 0);
+          broken);
       const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
       int c = (warp - 2) / 4 * 32;
       for (; c < tokens; c += 64) {
