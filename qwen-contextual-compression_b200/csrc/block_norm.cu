@@ -502,8 +502,8 @@ template <typename E>
 __device__ __forceinline__ void copy_row(uint8_t* slot, const E* row, const RowCopy& c, int shift, uint64_t* bar,
                                          uint64_t policy) {
   if (c.lo < c.hi)
-    bulk_load(slot + c.lo * 8 * sizeof(E), row + (c.lo * 8 - shift), static_cast<uint32_t>((c.hi - c.lo) * 8 * sizeof(E)),
-              bar, policy);
+    bulk_load(slot + c.lo * 8 * sizeof(E), row + (c.lo * 8 - shift),
+              static_cast<uint32_t>((c.hi - c.lo) * 8 * sizeof(E)), bar, policy);
 }
 
 // Granule i of the row from the ring slot; the tensor's partial end granules from global memory.
@@ -631,7 +631,8 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
   const int64_t each = (a.rows + grid - 1) / grid;
   const int rows_each = std::max(kDeepRoom / (blocks * slot), std::min(2, kRoom / (blocks * slot)));
   const int depth = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxDepth, rows_each, each})));
-  return launch_early(kernel, static_cast<unsigned>(grid), threads, static_cast<size_t>(depth) * slot, stream, a, depth);
+  return launch_early(kernel, static_cast<unsigned>(grid), threads, static_cast<size_t>(depth) * slot, stream, a,
+                      depth);
 }
 
 template <typename T, typename R, bool JOIN, bool EXACT>
@@ -659,7 +660,8 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
   a.shift0 = static_cast<int>(reinterpret_cast<uintptr_t>(a.y) / es % 8);
   const bool row_gate = a.gate.values != nullptr && a.gate.cols > 1;
   const bool together =
-      known_norm(a.post) && known_norm(a.next) && (!row_gate || known(a.gate.dtype)) && same_granules(a.y, a.ldy, es, a) &&
+      known_norm(a.post) && known_norm(a.next) && (!row_gate || known(a.gate.dtype)) &&
+      same_granules(a.y, a.ldy, es, a) &&
       (!JOIN || (same_granules(a.res, a.ld_res, rs, a) && same_granules(a.res_out, a.ld_res_out, rs, a))) &&
       (a.out == nullptr || a.out_dtype == QCC_DTYPE_I8 ||
        (known(a.out_dtype) && same_granules(a.out, a.ld_out, dtype_bytes(a.out_dtype), a)));

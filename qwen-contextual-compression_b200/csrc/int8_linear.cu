@@ -326,8 +326,8 @@ __device__ __forceinline__ void pair_tile(const PairPlan& p, int i, int& row, in
 // Notes a wait that ran out in both CTAs of the pair, before the commits that follow.
 __device__ __forceinline__ void note_failure(int* failed, uint32_t rank) {
   *static_cast<volatile int*>(failed) = 1;
-  asm volatile("st.shared::cluster.s32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(cluster_addr(failed, rank ^ 1u)), "r"(1)
-               : "memory");
+  const uint32_t other = cluster_addr(failed, rank ^ 1u);
+  asm volatile("st.shared::cluster.s32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(other), "r"(1) : "memory");
 }
 
 template <bool GATED, typename O>
@@ -557,7 +557,7 @@ int launch_stream(const Int8Args& a, int device, cudaStream_t stream) {
   const int slots = device_info(device).num_sms * std::max(1, (225 << 10) / (S::kSmem + 2048)) * 85 / 100;
   const int blocks = (a.cols + kTileCols - 1) / kTileCols;
   const int split = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>({kMaxSplit, blocks, slots / (static_cast<int64_t>(tiles) * token_tiles)})));
+      std::max<int64_t>(1, std::min<int64_t>({kMaxSplit, blocks, slots / (1ll * tiles * token_tiles)})));
   return launch_clusters(kernel, dim3(tiles * split, token_tiles), 128, S::kSmem, split, stream, a, tm_x, tm_w);
 }
 
@@ -586,7 +586,8 @@ int launch_pair(const Int8Args& a, int device, cudaStream_t stream) {
 
 // Bytes that the stream kernel's CTAs load with tiles of `bn` tokens.
 int64_t stream_loads(const Int8Args& a, bool gated, int bn) {
-  const int64_t tiles = static_cast<int64_t>((a.channels + (gated ? 63 : 127)) / (gated ? 64 : 128)) * ((a.tokens + bn - 1) / bn);
+  const int channels = gated ? kTileRows / 2 : kTileRows;
+  const int64_t tiles = static_cast<int64_t>((a.channels + channels - 1) / channels) * ((a.tokens + bn - 1) / bn);
   return tiles * ((a.cols + kTileCols - 1) / kTileCols) * (kTileRows + bn) * kTileCols;
 }
 
@@ -598,7 +599,8 @@ int launch(const Int8Args& a, int device, cudaStream_t stream) {
   // Pairs where their tiles fill at least half of the SMs (512 tokens, 17408 columns to 5120 channels, 40 tiles: pairs
   // 55 us, stream 60 us; 256 tokens, 20 tiles: 58 and 33 us).
   const int channels = GATED ? 128 : 256;
-  const int64_t pair_tiles = static_cast<int64_t>((a.channels + channels - 1) / channels) * ((a.tokens + kPairTokens - 1) / kPairTokens);
+  const int64_t pair_tiles = static_cast<int64_t>((a.channels + channels - 1) / channels) *
+                             ((a.tokens + kPairTokens - 1) / kPairTokens);
   if (a.tokens > 128 && 4 * pair_tiles >= device_info(device).num_sms) return launch_pair<GATED, O>(a, device, stream);
   // Narrow token tiles make more CTAs, wide ones load the weight less often (200 tokens of a 4000 x 4000 weight, 98 MB
   // of loads at 64: 13.2 us, at 128 15.1 us; 256 tokens of 17408 columns to 5120 channels, 522 MB: 52 and 33 us).

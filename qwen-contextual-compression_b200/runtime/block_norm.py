@@ -23,6 +23,7 @@ from .. import _lib
 KINDS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 GATES = {None: _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
 MAX_HIDDEN = 32768
+MAX_ROWS = 2 ** 31 - 1
 
 
 def _check_hidden(x: torch.Tensor, what: str) -> None:
@@ -77,7 +78,7 @@ class BlockNorm:
     for models that store the weight's difference from one.
     """
 
-    __slots__ = ("weight", "bias", "hidden", "_index", "_params", "_ref", "_pointers")
+    __slots__ = ("weight", "bias", "hidden", "_index", "_params", "_ref", "_weight_ptr", "_bias_ptr")
 
     def __init__(self, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, kind: str = "rms",
                  eps: float = 1e-6, weight_offset: float = 0.0):
@@ -101,8 +102,8 @@ class BlockNorm:
                 raise TypeError("weight and bias must share a dtype")
             _lib.require_cuda(weight, bias)
         self.weight, self.bias = weight, bias
-        self._pointers = (_lib.ptr(weight), _lib.ptr(bias))
-        self._params = _lib.NormParams(*self._pointers, code, KINDS[kind], weight_offset, eps)
+        self._weight_ptr, self._bias_ptr = _lib.ptr(weight), _lib.ptr(bias)
+        self._params = _lib.NormParams(self._weight_ptr, self._bias_ptr, code, KINDS[kind], weight_offset, eps)
         self._ref = ctypes.byref(self._params)
 
     @property
@@ -124,11 +125,17 @@ class BlockNorm:
                 raise ValueError(f"the norm has {self.hidden} weights, its input {hidden} values a row")
             if self._index != index:
                 raise RuntimeError("all tensors must share a device")
-            _lib.refuse_grad("BlockNorm", self.weight, self.bias)
-            pointers = (_lib.ptr(self.weight), _lib.ptr(self.bias))
-            if pointers != self._pointers:  # the parameters' storage was replaced
-                self._pointers = pointers
-                self._params.weight, self._params.bias = pointers
+            weight, bias = self.weight, self.bias
+            if weight is not None:
+                if weight.requires_grad:
+                    _lib.refuse_grad("BlockNorm", weight)
+                if weight.data_ptr() != self._weight_ptr:  # the parameter's storage was replaced
+                    self._params.weight = self._weight_ptr = weight.data_ptr()
+            if bias is not None:
+                if bias.requires_grad:
+                    _lib.refuse_grad("BlockNorm", bias)
+                if bias.data_ptr() != self._bias_ptr:
+                    self._params.bias = self._bias_ptr = bias.data_ptr()
         return self._ref
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
@@ -153,6 +160,8 @@ def _run_norm(x, norm, out, out_dtype, quantize):
     norm_ref = None if norm is None else norm._for(hidden, index)
     rows, ld = _rows(x)
     t = x.numel() // hidden
+    if t > MAX_ROWS:
+        raise ValueError(f"x has {t} rows: at most {MAX_ROWS}")
     scale, ld_out = None, hidden
     if quantize:
         if out is not None or out_dtype is not None:
@@ -186,7 +195,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale = amax / 127 and q = round_half_even(x * (127 / amax)).  A row with
     amax < 2^-119 gets scale 0 and zeros; one that holds a NaN or an infinity
     gets scale NaN and zeros, so every product with it is NaN.  The int8 rows
-    are padded to a multiple of 16 bytes, as ``runtime.int8_dense`` wants them.
+    start on multiples of 16 bytes, as ``runtime.int8_dense`` wants them.  At
+    most 32768 columns.
     """
     return _run_norm(x, None, None, None, True)
 
@@ -249,13 +259,16 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
         raise ValueError(f"gate_activation must be one of {tuple(GATES)}")
     if next_norm is None and (quantize or out is not None or out_dtype is not None):
         raise ValueError("quantize, out and out_dtype need a next_norm")
-    _lib.refuse_grad("residual_norm", branch, residual, gate)
+    if branch.requires_grad or residual.requires_grad or (gate is not None and gate.requires_grad):
+        _lib.refuse_grad("residual_norm", branch, residual, gate)
     post_ref = None if post is None else post._for(hidden, index)
     next_ref = None if next_norm is None else next_norm._for(hidden, index)
     gate_rows, gate_ref = (None, None) if gate is None else _gate_params(gate, gate_activation, shape)
     rows, ld = _rows(branch)
     res_rows, ld_res = _rows(residual)
     t = branch.numel() // hidden
+    if t > MAX_ROWS:
+        raise ValueError(f"branch has {t} rows: at most {MAX_ROWS}")
     if residual_out is None:
         residual_out = torch.empty_like(residual) if res_rows is residual else residual.new_empty(shape)
         ld_res_out = hidden

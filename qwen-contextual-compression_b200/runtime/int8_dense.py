@@ -61,7 +61,8 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
         raise ValueError("w must have rows and columns")
     if cols > MAX_COLS or tokens > MAX_TOKENS or channels > MAX_CHANNELS:
         raise ValueError(f"at most {MAX_TOKENS} tokens, {MAX_CHANNELS} channels and {MAX_COLS} columns")
-    _lib.refuse_grad("the int8 product", x_scale, w_scale, bias)
+    if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
+        _lib.refuse_grad("the int8 product", x_scale, w_scale, bias)
     if out is None:
         out_dtype = out_dtype or torch.bfloat16
         y_code = _lib.dtype_code(out_dtype)
@@ -212,7 +213,8 @@ class Int8GatedFFN:
                      transposed_down: bool = False) -> "Int8GatedFFN":
         """From gate, up [N, H] and down [H, N] (or its transpose), as ``pack_neuron_major`` takes them."""
         validate_weight_shapes(gate, up, down, transposed_down)
-        return cls(Int8GatedLinear.from_weights(gate, up), Int8Linear.from_weight(down.t() if transposed_down else down))
+        return cls(Int8GatedLinear.from_weights(gate, up),
+                   Int8Linear.from_weight(down.t() if transposed_down else down))
 
     @property
     def hidden(self) -> int:

@@ -214,7 +214,8 @@ def quantized_plain(v):
     keep = amax >= 2.0 ** -119
     most = torch.full_like(amax, 127.0)
     inverse = torch.where(keep, torch.div(most, amax), torch.zeros_like(amax))
-    return torch.round(v * inverse).to(torch.int8), torch.where(keep, torch.div(amax, most), torch.zeros_like(amax))[:, 0]
+    scale = torch.where(keep, torch.div(amax, most), torch.zeros_like(amax))
+    return torch.round(v * inverse).to(torch.int8), scale[:, 0]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -233,7 +233,8 @@ def test_layer_run_together(tokens, dtype):
     scale = want.abs().amax(1, keepdim=True) + branch.abs().amax(1, keepdim=True)
     assert bool(((r.double() - want).abs() <= half * want.abs() + 256 * U32 * scale).all())
     want_x = rms(want, following)
-    assert bool(((x.double() - want_x).abs() <= half * want_x.abs() + 1024 * U32 * want_x.abs().amax(1, keepdim=True)).all())
+    assert bool(((x.double() - want_x).abs()
+                 <= half * want_x.abs() + 1024 * U32 * want_x.abs().amax(1, keepdim=True)).all())
 
     # The whole layer is near the dense layer in float64: int8's errors, about 1% each in the 2-norm.
     n = rms(residual.double(), pre)

@@ -63,7 +63,8 @@ def join_args(**changed):
     (dict(gate=gate(each=0)), _lib.ERR_SHAPE), (dict(gate=gate(cols=32)), _lib.ERR_SHAPE),
     (dict(gate=gate(ld=-1)), _lib.ERR_SHAPE), (dict(gate=gate(values=None)), _lib.ERR_INVALID_ARGUMENT),
     (dict(out=P, ld_out=60), _lib.ERR_SHAPE), (dict(gate=gate(values=65)), _lib.ERR_ALIGNMENT),
-    (dict(residual=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT), (dict(residual_out=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
+    (dict(residual=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
+    (dict(residual_out=ctypes.c_void_p(65)), _lib.ERR_ALIGNMENT),
     (dict(out=P, ld_out=64, out_dtype=I8), _lib.ERR_INVALID_ARGUMENT), (dict(residual=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(residual_out=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(hidden=40000, ld_branch=40000, ld_residual=40000, ld_residual_out=40000), _lib.ERR_UNSUPPORTED),
@@ -84,7 +85,8 @@ def linear_args(**changed):
     (dict(y_dtype=I8), _lib.ERR_DTYPE), (dict(tokens=-1), _lib.ERR_SHAPE), (dict(channels=0), _lib.ERR_SHAPE),
     (dict(cols=0), _lib.ERR_SHAPE), (dict(ldx=48), _lib.ERR_SHAPE), (dict(ldw=48), _lib.ERR_SHAPE),
     (dict(ldy=7), _lib.ERR_SHAPE), (dict(cols=131072, ldx=131072, ldw=131072), _lib.ERR_UNSUPPORTED),
-    (dict(tokens=(1 << 20) + 1), _lib.ERR_UNSUPPORTED), (dict(channels=(1 << 19) + 1, ldy=1 << 20), _lib.ERR_UNSUPPORTED),
+    (dict(tokens=(1 << 20) + 1), _lib.ERR_UNSUPPORTED),
+    (dict(channels=(1 << 19) + 1, ldy=1 << 20), _lib.ERR_UNSUPPORTED),
     (dict(x=None), _lib.ERR_INVALID_ARGUMENT), (dict(ws=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(y=None), _lib.ERR_INVALID_ARGUMENT), (dict(ldx=72), _lib.ERR_ALIGNMENT), (dict(ldw=72), _lib.ERR_ALIGNMENT),
     (dict(x=ctypes.c_void_p(72)), _lib.ERR_ALIGNMENT), (dict(w=ctypes.c_void_p(72)), _lib.ERR_ALIGNMENT),
