@@ -536,8 +536,9 @@ QCC_API int qcc_indexed_ffn_prefill(const void* x, int64_t ldx, int n_tokens, in
  * host framework (end_to_end/model_patcher.py:12-33 replaces only the MLPs).
  *
  * Outputs of type QCC_DTYPE_I8 are int8 rows with one scale each:
- *   row_scale[t] = amax / 127,  q = round_half_even(v * (127 / amax)),
- * amax the row's largest magnitude.  A row with amax < 2^-119 gets scale 0
+ *   row_scale[t] = amax / 127,  q = round_half_even(127 * v / amax),
+ * amax the row's largest magnitude; of the exact quotient where rows are taken
+ * as they are (no norm), of the fp32 quotient after a norm.  A row with amax < 2^-119 gets scale 0
  * and zeros; a row that holds a NaN or an infinity gets scale NaN and zeros,
  * so that every product with it is NaN.
  * ------------------------------------------------------------------------- */

@@ -168,17 +168,61 @@ __device__ __forceinline__ void store_granule(T* row, const GranuleMap<EXACT>& m
   }
 }
 
-// |f| <= 127 / inverse by construction, so the rounded value fits int8.
-__device__ __forceinline__ int8_t to_int8(float f, float inverse) {
-  return static_cast<int8_t>(__float2int_rn(f * inverse));
+// Bits of |f|: ordered like the magnitudes, infinities and then NaNs above all finite values.
+__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
+
+// What a row's largest magnitude (its bits) makes of its int8 form.
+struct RowScale {
+  float amax, scale, inverse, inverse_rest;  // inverse 0: the row is stored as zeros
+  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+    amax = __uint_as_float(bits);
+    const bool finite = bits <= 0x7F7FFFFFu, kept = finite && amax >= kSmallestAmax;
+    inverse = kept ? 127.f / amax : 0.f;
+    inverse_rest = kept ? fmaf(-inverse, amax, 127.f) / amax : 0.f;
+    scale = kept ? amax / 127.f : finite ? 0.f : NAN;
+  }
+};
+
+// round_half_even(127 x / amax) from the remainder 127 x - q amax of a rounding q that may be one off: an exact pair
+// d + e, since q amax and 127 x are multiples of amax's last place and d is at most amax.
+__device__ __forceinline__ int settle_border(float x, float amax, int q) {
+  if (amax > 0x1p100f) x *= 0x1p-20f, amax *= 0x1p-20f;  // keeps 127 x finite; exact
+  const float p = 127.f * x, e = fmaf(127.f, x, -p);
+  const float d = fmaf(-static_cast<float>(q), amax, p);
+  const float side = d < 0.f ? -1.f : 1.f;
+  const float over = fmaf(2.f, fabsf(d), -amax) + 2.f * side * e;  // twice the remainder's size beyond half a step
+  return over > 0.f || (over == 0.f && (q & 1) != 0) ? q + static_cast<int>(side) : q;
+}
+
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, held in the low bits
+
+// int8 of computed values (norms): the rounding of x * inverse, within 1.6e-5 of a step of the quotient.
+__device__ __forceinline__ uint32_t quantize(float x, const RowScale& s) {
+  return __float_as_uint(fmaf(x, s.inverse, kMagic)) & 0xFFu;
+}
+
+// int8 of rows as they are: round_half_even(127 x / amax), of the exact quotient, for |x| <= amax.  The quotient with
+// the reciprocal's remainder is within 2^-47 of itself before its one rounding to fp32, so a border k + 1/2 comes out
+// as such.  Values of 16-bit types lie on borders in earnest (small whole numbers times powers of two), and no other
+// quotient of theirs rounds to one: 2^-12 is the least distance of those beyond 1.  fp32 values that round to a border
+// need the exact remainder.
+template <typename T>
+__device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
+  bool border = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float t = fmaf(f[j], s.inverse, f[j] * s.inverse_rest), m = t + kMagic;
+    q[j] = __float_as_uint(m) & 0xFFu;
+    if (sizeof(T) == 4) border |= fabsf(t - (m - kMagic)) == 0.5f;
+  }
+  if (sizeof(T) == 4 && border)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      q[j] = static_cast<uint8_t>(settle_border(f[j], s.amax, __float2int_rn(f[j] * s.inverse)));
 }
 
 template <bool EXACT>
-__device__ __forceinline__ void store_int8x8(int8_t* row, const GranuleMap<EXACT>& m, int i, const float* f,
-                                             float inverse) {
-  uint32_t q[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = static_cast<uint8_t>(to_int8(f[j], inverse));
+__device__ __forceinline__ void store_int8x8(int8_t* row, const GranuleMap<EXACT>& m, int i, const uint32_t (&q)[8]) {
   if (m.whole(i) && (EXACT || (reinterpret_cast<uintptr_t>(row + m.first(i)) & 7) == 0)) {
     *reinterpret_cast<uint2*>(row + m.first(i)) =
         make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
@@ -188,20 +232,6 @@ __device__ __forceinline__ void store_int8x8(int8_t* row, const GranuleMap<EXACT
       if (m.has(i, j)) row[m.element(i, j)] = static_cast<int8_t>(q[j]);
   }
 }
-
-// Bits of |f|: ordered like the magnitudes, infinities and then NaNs above all finite values.
-__device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
-
-// What a row's largest magnitude (its bits) makes of its int8 form.
-struct RowScale {
-  float scale, inverse;  // inverse 0: the row is stored as zeros
-  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
-    const float amax = __uint_as_float(bits);
-    const bool finite = bits <= 0x7F7FFFFFu, kept = finite && amax >= kSmallestAmax;
-    inverse = kept ? 127.f / amax : 0.f;
-    scale = kept ? amax / 127.f : finite ? 0.f : NAN;
-  }
-};
 
 // ---------------------------------------------------------------------------
 // Reductions over the team of a row, in a fixed order.
@@ -353,10 +383,13 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
     int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      if (s.inverse == 0.f)
+      if (s.inverse == 0.f)  // also takes the NaNs and infinities out
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      store_int8x8(row, m, i, v[i], s.inverse);
+      uint32_t q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = quantize(v[i][j], s);
+      store_int8x8(row, m, i, q);
     }
   } else if (a.out_dtype == QCC_DTYPE_F32) {
 #pragma unroll
@@ -368,8 +401,71 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
 }
 
 // ---------------------------------------------------------------------------
+// Rows as they are to int8: the words stay as they came, and 16-bit magnitudes are compared two at a time.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t w, __nv_bfloat16*) {  // NaN if either is
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t w, __half*) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), __habs2(*reinterpret_cast<__half2*>(&w)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void widen2(uint32_t w, float& lo, float& hi, __nv_bfloat16*) { bf16x2_to_f32(w, lo, hi); }
+__device__ __forceinline__ void widen2(uint32_t w, float& lo, float& hi, __half*) { half2_to_f32(w, lo, hi); }
+
+// Bits of the largest magnitude of the words.
+template <typename T, int VPT>
+__device__ __forceinline__ uint32_t largest(const Pack8<T> (&y)[VPT]) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        top = max(max(max(top, y[i].w[k].x & 0x7FFFFFFFu), max(y[i].w[k].y & 0x7FFFFFFFu, y[i].w[k].z & 0x7FFFFFFFu)),
+                  y[i].w[k].w & 0x7FFFFFFFu);
+    return top;
+  } else {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      top = larger2(top, y[i].w[0].x, static_cast<T*>(nullptr));
+      top = larger2(top, y[i].w[0].y, static_cast<T*>(nullptr));
+      top = larger2(top, y[i].w[0].z, static_cast<T*>(nullptr));
+      top = larger2(top, y[i].w[0].w, static_cast<T*>(nullptr));
+    }
+    float lo, hi;
+    widen2(top, lo, hi, static_cast<T*>(nullptr));
+    return max(magnitude(lo), magnitude(hi));
+  }
+}
+
+template <typename T, int VPT, bool EXACT, typename Team>
+__device__ __forceinline__ void quantize_row(const Pack8<T> (&y)[VPT], const BlockNormArgs& a, int64_t t,
+                                             const GranuleMap<EXACT>& m, Team& team) {
+  const RowScale s(team.max(largest(y)));
+  if (m.id == 0) a.row_scale[t] = s.scale;
+  int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float f[8];
+    uint32_t q[8];
+    widen(y[i], f);
+    if (s.inverse == 0.f)  // also takes the NaNs and infinities out
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    quantize8_exact<T>(f, s, q);
+    store_int8x8(row, m, i, q);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Kernels.  T: the branch's (or x's) type, R: the residual's.
 // ---------------------------------------------------------------------------
+
+enum Mode { kNorm, kJoin, kQuantize };
 
 __device__ __forceinline__ int row_shift(const BlockNormArgs& a, int64_t t) {
   return static_cast<int>((a.shift0 + t * a.ldy) & 7);
@@ -377,7 +473,7 @@ __device__ __forceinline__ int row_shift(const BlockNormArgs& a, int64_t t) {
 
 constexpr int kWarpRows = 4;  // rows (warps) of a block
 
-template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
+template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArgs a) {
   grid_dependency_wait();
   grid_dependency_trigger();
@@ -389,13 +485,17 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArg
   Pack8<R> r[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) y[i] = load_granule(static_cast<const T*>(a.y) + t * a.ldy, m, i);
-  if (JOIN)
+  if (MODE == kQuantize) {
+    quantize_row(y, a, t, m, team);
+    return;
+  }
+  if (MODE == kJoin)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) r[i] = load_granule(static_cast<const R*>(a.res) + t * a.ld_res, m, i);
   float v[VPT][8];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) widen(y[i], v[i]);
-  if (JOIN) {
+  if (MODE == kJoin) {
     normalise<T>(v, a.post, a.inv_hidden, m, team);
     apply_gate<T>(v, a, t, m);
 #pragma unroll
@@ -467,7 +567,10 @@ __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int d
     if (a.out == nullptr) continue;
     const float x = next.apply(a.next, r, e);
     if (a.out_dtype == QCC_DTYPE_I8)
-      static_cast<int8_t*>(a.out)[t * a.ld_out + e] = s.inverse == 0.f ? 0 : to_int8(x, s.inverse);
+      static_cast<int8_t*>(a.out)[t * a.ld_out + e] = static_cast<int8_t>(
+          s.inverse == 0.f                                      ? 0
+          : a.res == nullptr && a.next.kind == QCC_NORM_NONE ? settle_border(x, s.amax, __float2int_rn(x * s.inverse))
+                                                             : static_cast<int>(quantize(x, s)));
     else
       store_as(a.out, t * a.ld_out + e, a.out_dtype, x);
   }
@@ -482,10 +585,10 @@ constexpr int kMaxDepth = 8;
 constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
 
 // Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.
-template <bool JOIN, int VPT, bool EXACT>
+template <Mode MODE, int VPT, bool EXACT>
 struct RingShape {
   static constexpr int kThreads = VPT == 2 ? 640 : VPT == 4 ? 576 : 512;
-  static constexpr int kBlocks = EXACT && (VPT == 2 || (VPT == 4 && !JOIN)) ? 2 : 1;
+  static constexpr int kBlocks = EXACT && (VPT == 2 || (VPT == 4 && MODE != kJoin)) ? 2 : 1;
 };
 
 // The granules of row t that a bulk copy brings, [lo, hi): all of them, except that the partial granules at the two
@@ -508,31 +611,26 @@ __device__ __forceinline__ void copy_row(uint8_t* slot, const E* row, const RowC
 
 // Granule i of the row from the ring slot; the tensor's partial end granules from global memory.
 template <typename E, bool EXACT>
-__device__ __forceinline__ void load_slot8(const uint8_t* slot, const E* row, const RowCopy& c,
-                                           const GranuleMap<EXACT>& m, int i, float (&f)[8]) {
+__device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row, const RowCopy& c,
+                                              const GranuleMap<EXACT>& m, int i) {
+  const E* const there = reinterpret_cast<const E*>(slot);
+  if (EXACT) return load_granule(there, m, i);
   const int g = i * m.width + m.id;
-  if (EXACT) {
-    widen(load_granule(reinterpret_cast<const E*>(slot), m, i), f);
-    return;
-  }
-  if (g >= c.lo && g < c.hi)
-    widen(load_pack8<E>(reinterpret_cast<const E*>(slot) + g * 8), f);
-  else
+  if (m.whole(i)) return load_pack8<E>(there + g * 8);  // copied: only partial granules are left out
+  const E* const from = g >= c.lo && g < c.hi ? there + m.shift : row;
+  E e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = m.has(i, j) ? to_f32<E>(row[m.element(i, j)]) : 0.f;
-  if (!m.whole(i))
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (!m.has(i, j)) f[j] = 0.f;
+  for (int j = 0; j < 8; ++j) e[j] = m.has(i, j) ? from[m.element(i, j)] : E(0.f);
+  return to_words(e);
 }
 
-template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
-__global__ void __launch_bounds__(RingShape<JOIN, VPT, EXACT>::kThreads, RingShape<JOIN, VPT, EXACT>::kBlocks)
+template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
+__global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)
     ring_kernel(const BlockNormArgs a, int depth) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMaxDepth];
   __shared__ float scratch[64];
-  const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + (JOIN ? slot_bytes(a.hidden, sizeof(R)) : 0);
+  const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + (MODE == kJoin ? slot_bytes(a.hidden, sizeof(R)) : 0);
   const uint64_t policy = policy_evict_first();
   if (threadIdx.x == 0) {
     for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1);
@@ -546,9 +644,9 @@ __global__ void __launch_bounds__(RingShape<JOIN, VPT, EXACT>::kThreads, RingSha
   const auto fetch = [&](int64_t t, int s) {
     const int shift = EXACT ? 0 : row_shift(a, t);
     const RowCopy c(a, t, shift);
-    mbar_arrive_expect_tx(&full[s], max(0, c.hi - c.lo) * 8 * static_cast<int>(sizeof(T) + (JOIN ? sizeof(R) : 0)));
+    mbar_arrive_expect_tx(&full[s], max(0, c.hi - c.lo) * 8 * static_cast<int>(sizeof(T) + (MODE == kJoin ? sizeof(R) : 0)));
     copy_row(ring + s * bytes, y + t * a.ldy, c, shift, &full[s], policy);
-    if (JOIN) copy_row(ring + s * bytes + y_bytes, res + t * a.ld_res, c, shift, &full[s], policy);
+    if (MODE == kJoin) copy_row(ring + s * bytes + y_bytes, res + t * a.ld_res, c, shift, &full[s], policy);
   };
   if (threadIdx.x == 0)
     for (int s = 0; s < depth; ++s) {
@@ -563,24 +661,31 @@ __global__ void __launch_bounds__(RingShape<JOIN, VPT, EXACT>::kThreads, RingSha
     const RowCopy c(a, t, shift);
     const uint8_t* slot = ring + s * bytes;
     const bool arrived = mbar_wait_suspended(&full[s], phase, kWaitNs);
-    float v[VPT][8];
+    Pack8<T> words[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) load_slot8(slot, y + t * a.ldy, c, m, i, v[i]);
-    if (!arrived) v[0][0] = NAN;  // a row whose wait ran out becomes NaN by its sums
-    if (JOIN) {
+    for (int i = 0; i < VPT; ++i) words[i] = load_slot(slot, y + t * a.ldy, c, m, i);
+    if (!arrived) words[0].w[0].x = 0xFFFFFFFFu;  // a NaN in every type: the row becomes NaN by its sums or its scale
+    float v[VPT][8];
+    if (MODE != kQuantize)
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) widen(words[i], v[i]);
+    if (MODE == kJoin) {
       normalise<T>(v, a.post, a.inv_hidden, m, team);
       apply_gate<T>(v, a, t, m);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         float r[8];
-        load_slot8(slot + y_bytes, res + t * a.ld_res, c, m, i, r);
+        widen(load_slot(slot + y_bytes, res + t * a.ld_res, c, m, i), r);
         join8<R>(v[i], r, a, t, m, i);
       }
     }
     __syncthreads();  // the slot has been read
     const int64_t ahead = t + static_cast<int64_t>(depth) * gridDim.x;
     if (threadIdx.x == 0 && ahead < a.rows) fetch(ahead, s);
-    finish_row<T>(v, a, t, m, team);
+    if (MODE == kQuantize)
+      quantize_row(words, a, t, m, team);
+    else
+      finish_row<T>(v, a, t, m, team);
     if (++s == depth) s = 0, phase ^= 1;
   }
 }
@@ -613,12 +718,12 @@ bool launch_early(K kernel, unsigned grid, int threads, size_t smem, cudaStream_
   return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-template <typename T, typename R, bool JOIN, int VPT, bool EXACT>
+template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t stream) {
-  auto* kernel = ring_kernel<T, R, JOIN, VPT, EXACT>;
+  auto* kernel = ring_kernel<T, R, MODE, VPT, EXACT>;
   if (!ensure_max_dynamic_smem(reinterpret_cast<const void*>(kernel), device)) return false;
   const int threads = ((granules + VPT - 1) / VPT + 31) / 32 * 32;
-  const int slot = slot_bytes(a.hidden, sizeof(T)) + (JOIN ? slot_bytes(a.hidden, sizeof(R)) : 0);
+  const int slot = slot_bytes(a.hidden, sizeof(T)) + (MODE == kJoin ? slot_bytes(a.hidden, sizeof(R)) : 0);
   // Blocks an SM: as many as their registers allow, with at least two rows each in the ring's room; what is left
   // deepens the rings.
   static const int regs = [&] {
@@ -635,20 +740,20 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
                       depth);
 }
 
-template <typename T, typename R, bool JOIN, bool EXACT>
+template <typename T, typename R, Mode MODE, bool EXACT>
 bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>((a.rows + kWarpRows - 1) / kWarpRows);
-  if (granules <= 32) return launch_early(warp_kernel<T, R, JOIN, 1, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
-  if (granules <= 64) return launch_early(warp_kernel<T, R, JOIN, 2, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
-  if (granules <= 128) return launch_early(warp_kernel<T, R, JOIN, 4, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
-  if (granules <= 2 * RingShape<JOIN, 2, EXACT>::kThreads)
-    return launch_ring<T, R, JOIN, 2, EXACT>(a, granules, device, stream);
-  if (granules <= 4 * RingShape<JOIN, 4, EXACT>::kThreads)
-    return launch_ring<T, R, JOIN, 4, EXACT>(a, granules, device, stream);
-  return launch_ring<T, R, JOIN, 8, EXACT>(a, granules, device, stream);
+  if (granules <= 32) return launch_early(warp_kernel<T, R, MODE, 1, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= 64) return launch_early(warp_kernel<T, R, MODE, 2, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= 128) return launch_early(warp_kernel<T, R, MODE, 4, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
+  if (granules <= 2 * RingShape<MODE, 2, EXACT>::kThreads)
+    return launch_ring<T, R, MODE, 2, EXACT>(a, granules, device, stream);
+  if (granules <= 4 * RingShape<MODE, 4, EXACT>::kThreads)
+    return launch_ring<T, R, MODE, 4, EXACT>(a, granules, device, stream);
+  return launch_ring<T, R, MODE, 8, EXACT>(a, granules, device, stream);
 }
 
-template <typename T, typename R, bool JOIN>
+template <typename T, typename R, Mode MODE>
 bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStream_t stream) {
   constexpr int es = sizeof(T), rs = sizeof(R);
   // The granule kernels take parameters, gates and outputs in T or fp32.
@@ -662,12 +767,12 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
   const bool together =
       known_norm(a.post) && known_norm(a.next) && (!row_gate || known(a.gate.dtype)) &&
       same_granules(a.y, a.ldy, es, a) &&
-      (!JOIN || (same_granules(a.res, a.ld_res, rs, a) && same_granules(a.res_out, a.ld_res_out, rs, a))) &&
+      (MODE != kJoin || (same_granules(a.res, a.ld_res, rs, a) && same_granules(a.res_out, a.ld_res_out, rs, a))) &&
       (a.out == nullptr || a.out_dtype == QCC_DTYPE_I8 ||
        (known(a.out_dtype) && same_granules(a.out, a.ld_out, dtype_bytes(a.out_dtype), a)));
   const bool shifted = a.shift0 != 0 || (a.rows > 1 && a.ldy % 8 != 0);
   const int granules = (a.hidden + (shifted ? 14 : 7)) / 8;
-  const bool fits = granules <= 4096 && slot_bytes(a.hidden, es) + (JOIN ? slot_bytes(a.hidden, rs) : 0) <= kRoom;
+  const bool fits = granules <= 4096 && slot_bytes(a.hidden, es) + (MODE == kJoin ? slot_bytes(a.hidden, rs) : 0) <= kRoom;
   if (!together || !fits) {
     const int threads = std::min(512, (a.hidden + 31) / 32 * 32);
     return launch_early(plain_kernel, static_cast<unsigned>(a.rows), threads, 0, stream, a, dtype, res_dtype);
@@ -679,8 +784,8 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
   const bool exact = !shifted && a.hidden % 8 == 0 && aligned16(a.post.weight) && aligned16(a.post.bias) &&
                      aligned16(a.next.weight) && aligned16(a.next.bias) && gate_exact &&
                      (a.out == nullptr || a.out_dtype != QCC_DTYPE_I8 || (aligned16(a.out) && a.ld_out % 8 == 0));
-  return exact ? launch_granules<T, R, JOIN, true>(a, granules, device, stream)
-               : launch_granules<T, R, JOIN, false>(a, granules, device, stream);
+  return exact ? launch_granules<T, R, MODE, true>(a, granules, device, stream)
+               : launch_granules<T, R, MODE, false>(a, granules, device, stream);
 }
 
 bool valid_norm(const qcc_norm_params* p) {
@@ -706,17 +811,22 @@ int run_block_norm(const BlockNormArgs& a, int dtype, int res_dtype, cudaStream_
   if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
   const bool join = a.res != nullptr;
   bool ok;
-#define QCC_ROWS(T, R, J) launch_rows<T, R, J>(a, dtype, res_dtype, device, stream)
+  const bool quantize = !join && a.out_dtype == QCC_DTYPE_I8 && a.next.kind == QCC_NORM_NONE;
+#define QCC_ROWS(T, R, M) launch_rows<T, R, M>(a, dtype, res_dtype, device, stream)
   if (dtype == QCC_DTYPE_BF16)
-    ok = !join                        ? QCC_ROWS(__nv_bfloat16, __nv_bfloat16, false)
-         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__nv_bfloat16, float, true)
-                                      : QCC_ROWS(__nv_bfloat16, __nv_bfloat16, true);
+    ok = quantize                     ? QCC_ROWS(__nv_bfloat16, __nv_bfloat16, kQuantize)
+         : !join                      ? QCC_ROWS(__nv_bfloat16, __nv_bfloat16, kNorm)
+         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__nv_bfloat16, float, kJoin)
+                                      : QCC_ROWS(__nv_bfloat16, __nv_bfloat16, kJoin);
   else if (dtype == QCC_DTYPE_F16)
-    ok = !join                        ? QCC_ROWS(__half, __half, false)
-         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__half, float, true)
-                                      : QCC_ROWS(__half, __half, true);
+    ok = quantize                     ? QCC_ROWS(__half, __half, kQuantize)
+         : !join                      ? QCC_ROWS(__half, __half, kNorm)
+         : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__half, float, kJoin)
+                                      : QCC_ROWS(__half, __half, kJoin);
   else
-    ok = join ? QCC_ROWS(float, float, true) : QCC_ROWS(float, float, false);
+    ok = quantize ? QCC_ROWS(float, float, kQuantize)
+         : join   ? QCC_ROWS(float, float, kJoin)
+                  : QCC_ROWS(float, float, kNorm);
 #undef QCC_ROWS
   return ok ? QCC_OK : QCC_ERR_CUDA;
 }

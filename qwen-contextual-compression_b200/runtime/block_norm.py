@@ -192,7 +192,7 @@ def _run_norm(x, norm, out, out_dtype, quantize):
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [..., cols] in bf16 / fp16 / fp32 -> (int8 [T, cols], fp32 scales [T]), one symmetric scale a row.
 
-    scale = amax / 127 and q = round_half_even(x * (127 / amax)).  A row with
+    scale = amax / 127 and q = round_half_even(127 * x / amax), of the exact quotient.  A row with
     amax < 2^-119 gets scale 0 and zeros; one that holds a NaN or an infinity
     gets scale NaN and zeros, so every product with it is NaN.  The int8 rows
     start on multiples of 16 bytes, as ``runtime.int8_dense`` wants them.  At

@@ -207,15 +207,13 @@ def test_join_gate_of_sequences_and_in_place():
 
 
 def quantized_plain(v):
-    """The documented rule, in fp32 on the CPU (quotients of two tensors: torch multiplies by a reciprocal in
-    ``127 / amax``, which rounds twice)."""
-    v = v.float().cpu()
-    amax = v.abs().amax(-1, keepdim=True) if v.shape[1] else torch.zeros(v.shape[0], 1)
+    """The documented rule.  In float64 127 v is exact and its quotient by amax rounds to a border (k + 1/2) only where
+    it is one: another quotient of a 31-bit by a 24-bit number is at least 2^-25 away."""
+    v = v.double().cpu()
+    amax = v.abs().amax(-1, keepdim=True)
     keep = amax >= 2.0 ** -119
-    most = torch.full_like(amax, 127.0)
-    inverse = torch.where(keep, torch.div(most, amax), torch.zeros_like(amax))
-    scale = torch.where(keep, torch.div(amax, most), torch.zeros_like(amax))
-    return torch.round(v * inverse).to(torch.int8), scale[:, 0]
+    q = torch.where(keep, torch.round(127 * v / amax), torch.zeros_like(v))
+    return q.to(torch.int8), torch.where(keep, amax / 127, torch.zeros_like(amax)).float()[:, 0]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -232,6 +230,32 @@ def test_quantize_rows(rows, cols, dtype):
     assert bool((q.abs().amax(1) == 127).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_rows_on_borders(dtype):
+    """Rows full of values on or next to a border between two steps, at ordinary, tiny and huge magnitudes."""
+    cols = 2 * 127 + 2
+    for amax in (254.0, 127.0, 3 * 127.0, 1.0, 0.7, 254 * 2.0 ** -20, 254 * 2.0 ** -60, 2.0 ** 127 * 1.984):
+        if dtype == torch.float16 and not 2.0 ** -14 <= amax < 65504:
+            continue
+        a = float(torch.tensor(amax).to(dtype))
+        steps = torch.arange(-127, 127, dtype=torch.float64) + 0.5
+        x = torch.cat([steps * a / 127, torch.tensor([a, -a], dtype=torch.float64)]).to(dtype)
+        bits = x.float().view(torch.int32)
+        unit = 1 if dtype == torch.float32 else 1 << (16 if dtype == torch.bfloat16 else 13)
+        rows = [x]
+        for shift in (-unit, unit):  # the neighbours of each value in its type, kept below amax
+            rows.append(torch.where(x.float().abs() < a, (bits + shift).view(torch.float32), x.float()).to(dtype))
+        x = torch.stack(rows).cuda()
+        assert x.shape[1] == cols
+        for y in (x, x[:, :cols - 1].flip(1)):  # with and without the granule kernels' alignment
+            q, s = quantize_rows(y.contiguous())
+            want_q, want_s = quantized_plain(y)
+            assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s), amax
+        q, s = quantize_rows(x.contiguous().view(-1)[3:3 + cols].view(1, cols))
+        want_q, want_s = quantized_plain(x.contiguous().view(-1)[3:3 + cols].view(1, cols))
+        assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
 def test_quantize_rows_extremes():
     x = torch.zeros((8, 40), device="cuda")
     x[1] = 2.0 ** -119
@@ -239,7 +263,7 @@ def test_quantize_rows_extremes():
     x[3, 1] = float("nan")
     x[4, 2] = float("-inf")
     x[5] = 3e38
-    x[6, 0], x[6, 1] = -1.0, 127.5 / 127 * 0.5
+    x[6, 0], x[6, 1] = -1.0, 0.5
     q, s = quantize_rows(x)
     assert s[0] == 0 and bool((q[0] == 0).all())
     assert s[1] > 0 and bool((q[1] == 127).all())
@@ -247,7 +271,7 @@ def test_quantize_rows_extremes():
     for row in (3, 4):
         assert s[row].isnan() and bool((q[row] == 0).all())
     assert s[5].isfinite() and bool((q[5] == 127).all())
-    assert q[6, 0] == -127
+    assert q[6, 0] == -127 and q[6, 1] == 64  # 63.5 to the even side
     assert bool((q[7] == 0).all())
 
 
