@@ -121,6 +121,9 @@ struct RowOutput {
 // its own shared memory, and the cluster adds them over distributed shared
 // memory -- integer sums, so the split changes no bit of the result, and there
 // is no workspace that two calls could share.
+// Measured: gate|up 34816 x 5120, 1 token 28.9 us (6.2 of 6.45 TB/s), 64 tokens
+// 33.3 us; down 5120 x 17408, 1 token 16.8 us (5.3 TB/s: filling the rings and
+// joining the cluster take 3 us), 128 tokens 23.9 us.
 // ---------------------------------------------------------------------------
 
 template <int BN, int STAGES>
@@ -299,6 +302,10 @@ __global__ void __launch_bounds__(128)
 // columns) let a tile's epilogue run beside the next tile's MMAs.  A pair reads
 // each operand byte of its tile once (128 rows of each per CTA), half of what
 // two single CTAs would.
+// Measured at 4096 tokens: gate|up 34816 x 5120 529 to 570 us (2.8 to 2.6
+// POP/s), down 5120 x 17408 274 to 290 us (320 tiles are 4.3 rounds of 74
+// pairs).  A long run sits at the card's 1000 W with the SMs near 1.5 GHz, as
+// cuBLAS's bf16 product does (1.4 PFLOP/s sustained): power bounds it.
 // ---------------------------------------------------------------------------
 
 constexpr int kPairStages = 6;
