@@ -193,21 +193,21 @@ def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
             raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or detach its inputs")
 
 
-def launch(device_index: int, fn, *args) -> int:
-    """fn(*args, current stream of the device), with the device current (a launch needs its stream's device)."""
-    if _get_device() == device_index:
-        return fn(*args, _raw_stream(device_index))
-    with torch.cuda.device(device_index):
-        return fn(*args, _raw_stream(device_index))
-
-
 try:  # the raw queries avoid building a torch.cuda.Stream and the lazy-initialisation check per call
-    _raw_stream, _get_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    raw_stream, current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 except AttributeError:  # pragma: no cover  (a torch build without CUDA)
-    def _raw_stream(device_index: int) -> int:
+    def raw_stream(device_index: int) -> int:
         return torch.cuda.current_stream(device_index).cuda_stream
 
-    _get_device = torch.cuda.current_device
+    current_device = torch.cuda.current_device
+
+
+def launch(device_index: int, fn, *args) -> int:
+    """fn(*args, current stream of the device), with the device current (a launch needs its stream's device)."""
+    if current_device() == device_index:
+        return fn(*args, raw_stream(device_index))
+    with torch.cuda.device(device_index):
+        return fn(*args, raw_stream(device_index))
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

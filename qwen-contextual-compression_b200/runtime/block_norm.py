@@ -20,6 +20,7 @@ import torch
 
 from .. import _lib
 
+_raw_stream, _current_device = _lib.raw_stream, _lib.current_device
 KINDS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 GATES = {None: _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
 MAX_HIDDEN = 32768
@@ -182,8 +183,10 @@ def _run_norm(x, norm, out, out_dtype, quantize):
         out_code = _lib.dtype_code(out_dtype)
         ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
     lib = _lib.library()
-    status = _lib.launch(index, lib.qcc_norm_rows, rows.data_ptr(), ld, code, t, hidden, norm_ref, out.data_ptr(),
-                         ld_out, out_code, None if scale is None else scale.data_ptr())
+    args = (rows.data_ptr(), ld, code, t, hidden, norm_ref, out.data_ptr(), ld_out, out_code,
+            None if scale is None else scale.data_ptr())
+    fn = lib.qcc_norm_rows
+    status = fn(*args, _raw_stream(index)) if _current_device() == index else _lib.launch(index, fn, *args)
     if status:
         _lib.check(status, "qcc_norm_rows")
     return (out, scale) if quantize else out
@@ -295,9 +298,11 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
             ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
         out_ptr = out.data_ptr()
     lib = _lib.library()
-    status = _lib.launch(index, lib.qcc_residual_norm, rows.data_ptr(), ld, code, res_rows.data_ptr(), ld_res,
-                         res_code, t, hidden, post_ref, gate_ref, residual_scale, branch_scale,
-                         residual_out.data_ptr(), ld_res_out, next_ref, out_ptr, ld_out, out_code, scale_ptr)
+    args = (rows.data_ptr(), ld, code, res_rows.data_ptr(), ld_res, res_code, t, hidden, post_ref, gate_ref,
+            residual_scale, branch_scale, residual_out.data_ptr(), ld_res_out, next_ref, out_ptr, ld_out, out_code,
+            scale_ptr)
+    fn = lib.qcc_residual_norm
+    status = fn(*args, _raw_stream(index)) if _current_device() == index else _lib.launch(index, fn, *args)
     if status:
         _lib.check(status, "qcc_residual_norm")
     if next_norm is None:

@@ -23,24 +23,28 @@ from .. import _lib
 from .block_norm import int8_rows, quantize_rows
 from .packing import PackedFFNWeights, validate_weight_shapes
 
+_raw_stream, _current_device = _lib.raw_stream, _lib.current_device
 MAX_COLS = 131071       # |q| <= 128: the int32 sums cannot overflow
 MAX_TOKENS = 1 << 20
 MAX_CHANNELS = 1 << 19
 
 
+_INT8, _FLOAT32 = torch.int8, torch.float32
+
+
 def _int8_operand(q: torch.Tensor, scale: torch.Tensor, what: str) -> tuple[int, int, int]:
     """Checks an int8 matrix with its row scales; returns its rows, columns and row stride."""
-    if q.dim() != 2 or q.dtype != torch.int8:
+    if q.dim() != 2 or q.dtype is not _INT8:
         raise ValueError(f"{what} must be an int8 matrix")
     rows, cols = q.shape
     ld, step = q.stride()
     if step != 1 and cols != 1:
         raise ValueError(f"{what} must be contiguous along its columns")
-    if scale.dtype != torch.float32 or scale.shape != (rows,) or not scale.is_contiguous():
+    if scale.dtype is not _FLOAT32 or scale.shape != (rows,) or not scale.is_contiguous():
         raise ValueError(f"the scales of {what} must be a contiguous float32 tensor with one value per row")
     if rows <= 1:
         ld = cols + -cols % 16
-    if ld % 16 or q.data_ptr() % 16 or ld < cols:
+    if ld & 15 or q.data_ptr() & 15 or ld < cols:
         raise ValueError(f"the rows of {what} must start on multiples of 16 bytes (quantize_rows stores them so)")
     return rows, cols, ld
 
@@ -54,9 +58,9 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
         _lib.require_cuda(xq, x_scale, wq, w_scale, bias, out)
     if w_cols != cols:
         raise ValueError(f"x has {cols} columns, w {w_cols}")
-    if gated and rows % 2:
+    if gated and rows & 1:
         raise ValueError("a gated weight has as many up rows as gate rows")
-    channels = rows // 2 if gated else rows
+    channels = rows >> 1 if gated else rows
     if channels < 1 or cols < 1:
         raise ValueError("w must have rows and columns")
     if cols > MAX_COLS or tokens > MAX_TOKENS or channels > MAX_CHANNELS:
@@ -64,7 +68,8 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
     if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
         _lib.refuse_grad("the int8 product", x_scale, w_scale, bias)
     if out is None:
-        out_dtype = out_dtype or torch.bfloat16
+        if out_dtype is None:
+            out_dtype = torch.bfloat16
         y_code = _lib.dtype_code(out_dtype)
         out = torch.empty(tokens, channels, dtype=out_dtype, device=xq.device)
         ldy = channels
@@ -76,17 +81,19 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
         ldy = max(out.stride(0), channels)
     lib = _lib.library()
     if gated:
-        status = _lib.launch(index, lib.qcc_int8_gated_linear, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(),
-                             ldw, w_scale.data_ptr(), tokens, channels, cols, out.data_ptr(), ldy, y_code)
+        args = (xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(), tokens, channels, cols,
+                out.data_ptr(), ldy, y_code)
+        fn = lib.qcc_int8_gated_linear
     else:
         bias_ptr, bias_code = None, _lib.DTYPE_F32
         if bias is not None:
             if bias.dim() != 1 or bias.shape[0] != channels or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous tensor with one value per channel")
             bias_ptr, bias_code = bias.data_ptr(), _lib.dtype_code(bias.dtype)
-        status = _lib.launch(index, lib.qcc_int8_linear, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw,
-                             w_scale.data_ptr(), bias_ptr, bias_code, tokens, channels, cols, out.data_ptr(), ldy,
-                             y_code)
+        args = (xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(), bias_ptr, bias_code,
+                tokens, channels, cols, out.data_ptr(), ldy, y_code)
+        fn = lib.qcc_int8_linear
+    status = fn(*args, _raw_stream(index)) if _current_device() == index else _lib.launch(index, fn, *args)
     if status:
         _lib.check(status, "qcc_int8_gated_linear" if gated else "qcc_int8_linear")
     return out
