@@ -62,6 +62,7 @@ __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) 
 constexpr int kTileRows = 128;  // weight rows of a CTA's tile: TMEM lanes
 constexpr int kTileCols = 128;  // bytes of K per stage (one swizzled row)
 constexpr uint32_t kMaxSplit = 8;  // CTAs of a stream kernel's cluster, at most
+constexpr int kAhead = 6;       // blocks of the weight that a stream kernel's CTA brings to L2 before it waits
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 // What one lane needs to finish its weight row's outputs.
@@ -174,6 +175,18 @@ __global__ void __launch_bounds__(128)
     mbar_init(&done, 1);
     failed = 0;
     fence_barrier_init();
+    // The weight's first blocks start for L2 while the launches ahead finish (usually the one that makes x): a
+    // prefetch moves no value into this kernel, so it may run ahead of a launch that writes the weight.  Norm and
+    // gate|up of one token: 32.2 us without it, 30.9 with 4 or 8 blocks, 32.8 with 16.
+    for (int i = 0; i < min(count, kAhead); ++i) {
+      const int k = (first + i) * kTileCols;
+      if (GATED) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tma_prefetch_3d(&tm_w, k, n0 + q * 16, 0);
+      } else {
+        tma_prefetch_2d(&tm_w, k, n0);
+      }
+    }
   }
   // Tensor memory is taken only once the launches ahead have finished: a CTA
   // of theirs that still waits for its own columns must not wait for ours.
