@@ -28,7 +28,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cfloat>
+#include <type_traits>
 
 #include "qcc_common.cuh"
 #include "qcc_host.h"
@@ -128,14 +128,14 @@ __device__ __forceinline__ void load_param8(const P* p, const GranuleMap<EXACT>&
   }
 }
 
-// The same for a parameter in T or fp32.
-template <typename T, bool EXACT>
+// The same for a parameter in P or fp32.
+template <typename P, bool EXACT>
 __device__ __forceinline__ void load_param8(const void* p, int dtype, const GranuleMap<EXACT>& m, int i,
                                             float (&f)[8]) {
-  if (sizeof(T) == 4 || dtype == QCC_DTYPE_F32)
+  if (sizeof(P) == 4 || dtype == QCC_DTYPE_F32)
     load_param8(static_cast<const float*>(p), m, i, f);
   else
-    load_param8(static_cast<const T*>(p), m, i, f);
+    load_param8(static_cast<const P*>(p), m, i, f);
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
@@ -204,8 +204,8 @@ __device__ __forceinline__ uint32_t quantize(float x, const RowScale& s) {
 // int8 of rows as they are: round_half_even(127 x / amax), of the exact quotient, for |x| <= amax.  The quotient with
 // the reciprocal's remainder is within 2^-47 of itself before its one rounding to fp32, so a border k + 1/2 comes out
 // as such.  Values of 16-bit types lie on borders in earnest (small whole numbers times powers of two), and no other
-// quotient of theirs rounds to one: 2^-12 is the least distance of those beyond 1.  fp32 values that round to a border
-// need the exact remainder.
+// quotient of theirs rounds to one: with 11-bit significands those in [2^k, 2^(k+1)) are 2^(k-20) or more away from a
+// border, and fp32 is off by 2^(k-24) there.  fp32 values that round to a border need the exact remainder.
 template <typename T>
 __device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
   bool border = false;
@@ -268,7 +268,7 @@ struct BlockTeam {
 // ---------------------------------------------------------------------------
 
 // v <- N(v) over the row's values (entries outside the row are 0 on entry, and stay so where they are summed).
-template <typename T, int VPT, bool EXACT, typename Team>
+template <typename P, int VPT, bool EXACT, typename Team>
 __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_params& a, float inv_n,
                                           const GranuleMap<EXACT>& m, Team& team) {
   if (a.kind == QCC_NORM_NONE) return;
@@ -299,7 +299,7 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
   for (int i = 0; i < VPT; ++i) {
     float w[8];
     if (a.weight != nullptr) {
-      load_param8<T>(a.weight, a.dtype, m, i, w);
+      load_param8<P>(a.weight, a.dtype, m, i, w);
       if (a.weight_offset != 0.f)
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] += a.weight_offset;
@@ -310,7 +310,7 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
       for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
     }
     if (a.bias != nullptr) {
-      load_param8<T>(a.bias, a.dtype, m, i, w);
+      load_param8<P>(a.bias, a.dtype, m, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] += w[j];
     }
@@ -366,12 +366,12 @@ __device__ __forceinline__ void join8(float (&v)[8], const float (&r)[8], const 
   store_granule(static_cast<R*>(a.res_out) + t * a.ld_res_out, m, i, v);
 }
 
-// out[t] (T, fp32 or int8) from N_next(v).
-template <typename T, int VPT, bool EXACT, typename Team>
+// out[t] (P, fp32 or int8) from N_next(v).
+template <typename P, int VPT, bool EXACT, typename Team>
 __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormArgs& a, int64_t t,
                                            const GranuleMap<EXACT>& m, Team& team) {
   if (a.out == nullptr) return;
-  normalise<T>(v, a.next, a.inv_hidden, m, team);
+  normalise<P>(v, a.next, a.inv_hidden, m, team);
   if (a.out_dtype == QCC_DTYPE_I8) {
     uint32_t amax = 0;
 #pragma unroll
@@ -396,7 +396,7 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
     for (int i = 0; i < VPT; ++i) store_granule(static_cast<float*>(a.out) + t * a.ld_out, m, i, v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) store_granule(static_cast<T*>(a.out) + t * a.ld_out, m, i, v[i]);
+    for (int i = 0; i < VPT; ++i) store_granule(static_cast<P*>(a.out) + t * a.ld_out, m, i, v[i]);
   }
 }
 
@@ -405,7 +405,8 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t w, __nv_bfloat16*) {  // NaN if either is
-  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&w)));
+  const __nv_bfloat162 r =
+      __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&w)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t w, __half*) {
@@ -462,10 +463,15 @@ __device__ __forceinline__ void quantize_row(const Pack8<T> (&y)[VPT], const Blo
 }
 
 // ---------------------------------------------------------------------------
-// Kernels.  T: the branch's (or x's) type, R: the residual's.
+// Kernels.  T: the branch's (or x's) type, R: the residual's in a join.
 // ---------------------------------------------------------------------------
 
 enum Mode { kNorm, kJoin, kQuantize };
+
+// The 16-bit type that parameters and outputs may have besides fp32: T, or for the norm of fp32 rows R (an fp32
+// residual stream normed for 16-bit weights).
+template <typename T, typename R, Mode MODE>
+using ParamType = std::conditional_t<sizeof(T) == 4 && MODE == kNorm, R, T>;
 
 __device__ __forceinline__ int row_shift(const BlockNormArgs& a, int64_t t) {
   return static_cast<int>((a.shift0 + t * a.ldy) & 7);
@@ -477,6 +483,7 @@ constexpr int kWarpRows = 4;  // rows (warps) of a block
 // bf16: 2.4 us, 1.7 TB/s).
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArgs a) {
+  using P = ParamType<T, R, MODE>;
   grid_dependency_wait();
   grid_dependency_trigger();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarpRows + (threadIdx.x >> 5);
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArg
 #pragma unroll
   for (int i = 0; i < VPT; ++i) widen(y[i], v[i]);
   if (MODE == kJoin) {
-    normalise<T>(v, a.post, a.inv_hidden, m, team);
+    normalise<P>(v, a.post, a.inv_hidden, m, team);
     apply_gate<T>(v, a, t, m);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArg
       join8<R>(v[i], f, a, t, m, i);
     }
   }
-  finish_row<T>(v, a, t, m, team);
+  finish_row<P>(v, a, t, m, team);
 }
 
 // One norm's row statistics and an element's normed value.
@@ -638,10 +645,12 @@ __device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row,
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)
     ring_kernel(const BlockNormArgs a, int depth) {
+  using P = ParamType<T, R, MODE>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMaxDepth];
   __shared__ float scratch[64];
-  const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + (MODE == kJoin ? slot_bytes(a.hidden, sizeof(R)) : 0);
+  constexpr int kResidual = MODE == kJoin ? sizeof(R) : 0;
+  const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + slot_bytes(a.hidden, kResidual);
   const uint64_t policy = policy_evict_first();
   if (threadIdx.x == 0) {
     for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1);
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
   const auto fetch = [&](int64_t t, int s) {
     const int shift = EXACT ? 0 : row_shift(a, t);
     const RowCopy c(a, t, shift);
-    mbar_arrive_expect_tx(&full[s], max(0, c.hi - c.lo) * 8 * static_cast<int>(sizeof(T) + (MODE == kJoin ? sizeof(R) : 0)));
+    mbar_arrive_expect_tx(&full[s], max(0, c.hi - c.lo) * 8 * (static_cast<int>(sizeof(T)) + kResidual));
     copy_row(ring + s * bytes, y + t * a.ldy, c, shift, &full[s], policy);
     if (MODE == kJoin) copy_row(ring + s * bytes + y_bytes, res + t * a.ld_res, c, shift, &full[s], policy);
   };
@@ -696,7 +705,7 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     if (MODE == kQuantize)
       quantize_row(words, a, t, m, team);
     else
-      finish_row<T>(v, a, t, m, team);
+      finish_row<P>(v, a, t, m, team);
     if (++s == depth) s = 0, phase ^= 1;
   }
 }
@@ -753,7 +762,7 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
 
 template <typename T, typename R, Mode MODE, bool EXACT>
 bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>((a.rows + kWarpRows - 1) / kWarpRows);
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kWarpRows - 1) / kWarpRows);
   if (granules <= 32) return launch_early(warp_kernel<T, R, MODE, 1, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
   if (granules <= 64) return launch_early(warp_kernel<T, R, MODE, 2, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
   if (granules <= 128) return launch_early(warp_kernel<T, R, MODE, 4, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
@@ -764,11 +773,17 @@ bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStrea
   return launch_ring<T, R, MODE, 8, EXACT>(a, granules, device, stream);
 }
 
+template <typename T>
+constexpr int code_of() {
+  return std::is_same_v<T, __nv_bfloat16> ? QCC_DTYPE_BF16 : std::is_same_v<T, __half> ? QCC_DTYPE_F16 : QCC_DTYPE_F32;
+}
+
 template <typename T, typename R, Mode MODE>
 bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStream_t stream) {
   constexpr int es = sizeof(T), rs = sizeof(R);
-  // The granule kernels take parameters, gates and outputs in T or fp32.
-  const auto known = [&](int d) { return d == dtype || d == QCC_DTYPE_F32; };
+  // The granule kernels take parameters and outputs in ParamType or fp32, gates in T or fp32.
+  constexpr int kParams = code_of<ParamType<T, R, MODE>>();
+  const auto known = [&](int d) { return d == kParams || d == QCC_DTYPE_F32; };
   const auto known_norm = [&](const qcc_norm_params& p) {
     return (p.weight == nullptr && p.bias == nullptr) || known(p.dtype);
   };
@@ -783,7 +798,8 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
        (known(a.out_dtype) && same_granules(a.out, a.ld_out, dtype_bytes(a.out_dtype), a)));
   const bool shifted = a.shift0 != 0 || (a.rows > 1 && a.ldy % 8 != 0);
   const int granules = (a.hidden + (shifted ? 14 : 7)) / 8;
-  const bool fits = granules <= 4096 && slot_bytes(a.hidden, es) + (MODE == kJoin ? slot_bytes(a.hidden, rs) : 0) <= kRoom;
+  const int slot = slot_bytes(a.hidden, es) + (MODE == kJoin ? slot_bytes(a.hidden, rs) : 0);
+  const bool fits = granules <= 4096 && slot <= kRoom;
   if (!together || !fits) {
     const int threads = std::min(512, (a.hidden + 31) / 32 * 32);
     return launch_early(plain_kernel, static_cast<unsigned>(a.rows), threads, 0, stream, a, dtype, res_dtype);
@@ -834,10 +850,12 @@ int run_block_norm(const BlockNormArgs& a, int dtype, int res_dtype, cudaStream_
          : !join                      ? QCC_ROWS(__half, __half, kNorm)
          : res_dtype == QCC_DTYPE_F32 ? QCC_ROWS(__half, float, kJoin)
                                       : QCC_ROWS(__half, __half, kJoin);
+  else if (quantize || join)
+    ok = quantize ? QCC_ROWS(float, float, kQuantize) : QCC_ROWS(float, float, kJoin);
   else
-    ok = quantize ? QCC_ROWS(float, float, kQuantize)
-         : join   ? QCC_ROWS(float, float, kJoin)
-                  : QCC_ROWS(float, float, kNorm);
+    ok = a.out_dtype == QCC_DTYPE_BF16 || a.next.dtype == QCC_DTYPE_BF16  ? QCC_ROWS(float, __nv_bfloat16, kNorm)
+         : a.out_dtype == QCC_DTYPE_F16 || a.next.dtype == QCC_DTYPE_F16 ? QCC_ROWS(float, __half, kNorm)
+                                                                         : QCC_ROWS(float, float, kNorm);
 #undef QCC_ROWS
   return ok ? QCC_OK : QCC_ERR_CUDA;
 }

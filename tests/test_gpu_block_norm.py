@@ -80,6 +80,26 @@ def test_norm_types_and_offset(param_dtype, out_dtype):
     assert_rows_close(bare(x, out_dtype=out_dtype), norm64(x.double(), bare))
 
 
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(1, 64), (5, 333), (3, 1000), (2, 5120), (700, 1111), (9, 20001)])
+def test_fp32_rows_for_16_bit_weights(rows, hidden, low):
+    """An fp32 residual stream normed with 16-bit parameters, into 16 bits, fp32 and int8."""
+    x = make((rows, hidden), torch.float32, 1, 2.0)
+    for kind, param_dtype in (("rms", low), ("layer", low), ("layer", torch.float32)):
+        norm = make_norm(hidden, kind, param_dtype, 2)
+        want = norm64(x.double(), norm)
+        for out_dtype in (low, torch.float32):
+            y = norm(x, out_dtype=out_dtype)
+            assert y.dtype == out_dtype
+            assert_rows_close(y, want, norm.bias.expand(rows, hidden))
+        q, s = norm(x, quantize=True)
+        amax = want.abs().amax(-1, keepdim=True)
+        bound = 260 * U32 * (amax + norm.bias.double().abs().max())
+        assert bool(((s.double()[:, None] * 127 - amax).abs() <= bound).all())
+        assert bool(((q.double() * s.double()[:, None] - want).abs() <= 0.5 * amax / 127 + 127 * 4 * U32 * amax
+                     + 2 * bound).all())
+
+
 def test_norm_strides_views_and_in_place():
     base = make((7, 1300), torch.bfloat16, 4)
     norm = make_norm(640, "rms", torch.bfloat16, 5, bias=False)
@@ -254,6 +274,19 @@ def test_quantize_rows_on_borders(dtype):
         q, s = quantize_rows(x.contiguous().view(-1)[3:3 + cols].view(1, cols))
         want_q, want_s = quantized_plain(x.contiguous().view(-1)[3:3 + cols].view(1, cols))
         assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantize_rows_over_a_whole_type(dtype):
+    """Every value of the type up to amax, for a few amax of each significand's parity."""
+    positive = torch.arange(1 << 15, dtype=torch.int32).to(torch.int16).view(dtype).float()
+    for amax in (1.0, 1.5, 1.0078125, 1.9921875, 240.0, 1.25 * 2.0 ** -10, 127.0, 0.99609375):
+        x = positive[positive <= amax].to(dtype)
+        assert float(x.float().max()) == amax
+        for y in (x, -x):
+            q, s = quantize_rows(y.cuda()[None])
+            want_q, want_s = quantized_plain(y[None])
+            assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s), amax
 
 
 def test_quantize_rows_extremes():
