@@ -117,11 +117,46 @@ __device__ __forceinline__ Pack8<T> load_granule(const T* row, const GranuleMap<
   return p;
 }
 
-// A parameter vector's elements of granule i.  Without EXACT its alignment is not the row's: single elements.
+// Elements 8 - shift .. 15 - shift of two granules that follow each other, shift 1..7: words are selected two steps
+// down, 16-bit elements then brought together across words.
+template <typename P>
+__device__ __forceinline__ Pack8<P> straddle(const Pack8<P>& lo, const Pack8<P>& hi, int shift) {
+  constexpr int kWords = sizeof(P) * 2;  // of a granule
+  uint32_t w[2 * kWords];
+#pragma unroll
+  for (int k = 0; k < Pack8<P>::kWords; ++k) {
+    w[4 * k] = lo.w[k].x, w[4 * k + 1] = lo.w[k].y, w[4 * k + 2] = lo.w[k].z, w[4 * k + 3] = lo.w[k].w;
+    w[kWords + 4 * k] = hi.w[k].x, w[kWords + 4 * k + 1] = hi.w[k].y;
+    w[kWords + 4 * k + 2] = hi.w[k].z, w[kWords + 4 * k + 3] = hi.w[k].w;
+  }
+  const int first = sizeof(P) == 4 ? 8 - shift : (8 - shift) >> 1;  // the first word wanted
+#pragma unroll
+  for (int step = kWords / 2; step > 0; step >>= 1)
+#pragma unroll
+    for (int j = 0; j + step < 2 * kWords; ++j) w[j] = (first & step) != 0 ? w[j + step] : w[j];
+  if (sizeof(P) == 2) {
+    const int bits = (shift & 1) * 16;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], bits);
+  }
+  Pack8<P> r;
+#pragma unroll
+  for (int k = 0; k < Pack8<P>::kWords; ++k) r.w[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  return r;
+}
+
+// A parameter vector's elements of granule i.  Without EXACT they straddle two of its own granules (when it starts on
+// 16 bytes and both lie inside of it), or are single elements.
 template <typename P, bool EXACT>
 __device__ __forceinline__ void load_param8(const P* p, const GranuleMap<EXACT>& m, int i, float (&f)[8]) {
   if (EXACT) {
     widen(load_granule(p, m, i), f);
+    return;
+  }
+  const int e = m.first(i) + m.shift;  // the later granule's first element
+  if (m.first(i) >= 0 && e + 8 <= m.n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const Pack8<P> hi = load_pack8<P>(p + e);
+    widen(m.shift == 0 ? hi : straddle(load_pack8<P>(p + e - 8), hi, m.shift), f);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = m.has(i, j) ? to_f32<P>(p[m.element(i, j)]) : 0.f;
