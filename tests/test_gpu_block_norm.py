@@ -342,6 +342,24 @@ def test_streams_and_graph():
     assert torch.equal(captured[0], want[0]) and torch.equal(captured[1], want[1])
 
 
+@pytest.mark.parametrize("rows,hidden", [(2048, 1400), (2049, 1536), (2051, 2048), (2048, 1401)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_of_middling_width(rows, hidden, dtype):
+    x, residual = make((rows, hidden), dtype, 1), make((rows, hidden), dtype, 2)
+    norm = make_norm(hidden, "layer", dtype, 3)
+    assert_rows_close(norm(x), norm64(x.double(), norm), norm.bias.expand(rows, hidden))
+    bare = make_norm(hidden, "rms", dtype, 5, bias=False)
+    r, (q, s) = residual_norm(x, residual, next_norm=bare, quantize=True)
+    want = x.double() + residual.double()
+    assert_rows_close(r, want, torch.maximum(x.abs(), residual.abs()))
+    want = norm64(want, bare)
+    amax = want.abs().amax(-1, keepdim=True)
+    assert bool(((q.double() * s.double()[:, None] - want).abs() <= 0.5 * amax / 127 + (520 + 127 * 4) * U32 * amax).all())
+    q, s = quantize_rows(x)
+    want_q, want_s = quantized_plain(x)
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
 def test_many_rows():
     """More rows than one launch dimension of 65535 would hold."""
     rows = 70001

@@ -8,6 +8,7 @@ import torch
 
 import conftest  # noqa: F401
 from qcc_b200 import _lib
+from qcc_b200.runtime.block import FFNBlock
 from qcc_b200.runtime.block_norm import BlockNorm, quantize_rows, residual_norm
 from qcc_b200.runtime.int8_dense import Int8GatedFFN, Int8GatedLinear, Int8Linear, int8_gated_linear, int8_linear
 
@@ -121,6 +122,8 @@ def test_no_cpu_fallback():
 
 
 def test_python_argument_errors():
+    with pytest.raises(ValueError, match="next_norm"):
+        FFNBlock(lambda x: x, BlockNorm(), quantize_next=True)
     with pytest.raises(ValueError, match="kind"):
         BlockNorm(kind="batch")
     with pytest.raises(ValueError, match="eps"):
