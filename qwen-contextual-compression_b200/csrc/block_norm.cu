@@ -204,6 +204,13 @@ __device__ __forceinline__ void store_granule(T* row, const GranuleMap<EXACT>& m
   }
 }
 
+// max(a, |f|), NaN if either is.
+__device__ __forceinline__ float larger(float a, float f) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(f)));
+  return r;
+}
+
 // Bits of |f|: ordered like the magnitudes, infinities and then NaNs above all finite values.
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
 
@@ -232,9 +239,15 @@ __device__ __forceinline__ int settle_border(float x, float amax, int q) {
 
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, held in the low bits
 
-// int8 of computed values (norms): the rounding of x * inverse, within 1.6e-5 of a step of the quotient.
+// int8 of computed values (norms), in the low byte: the rounding of x * inverse, within 1.6e-5 of a step of the
+// quotient.
 __device__ __forceinline__ uint32_t quantize(float x, const RowScale& s) {
-  return __float_as_uint(fmaf(x, s.inverse, kMagic)) & 0xFFu;
+  return __float_as_uint(fmaf(x, s.inverse, kMagic));
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // int8 of rows as they are: round_half_even(127 x / amax), of the exact quotient, for |x| <= amax.  The quotient with
@@ -248,20 +261,20 @@ __device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowSc
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float t = fmaf(f[j], s.inverse, f[j] * s.inverse_rest), m = t + kMagic;
-    q[j] = __float_as_uint(m) & 0xFFu;
+    q[j] = __float_as_uint(m);
     if (sizeof(T) == 4) border |= fabsf(t - (m - kMagic)) == 0.5f;
   }
   if (sizeof(T) == 4 && border)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      q[j] = static_cast<uint8_t>(settle_border(f[j], s.amax, __float2int_rn(f[j] * s.inverse)));
+      q[j] = static_cast<uint32_t>(settle_border(f[j], s.amax, __float2int_rn(f[j] * s.inverse)));
 }
 
 template <bool EXACT>
 __device__ __forceinline__ void store_int8x8(int8_t* row, const GranuleMap<EXACT>& m, int i, const uint32_t (&q)[8]) {
   if (m.whole(i) && (EXACT || (reinterpret_cast<uintptr_t>(row + m.first(i)) & 7) == 0)) {
     *reinterpret_cast<uint2*>(row + m.first(i)) =
-        make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+        make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
   } else if (!EXACT) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -409,12 +422,12 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
   if (a.out == nullptr) return;
   normalise<P>(v, a.next, a.inv_hidden, m, team);
   if (a.out_dtype == QCC_DTYPE_I8) {
-    uint32_t amax = 0;
+    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, magnitude(v[i][j]));
-    const RowScale s(team.max(amax));
+      for (int j = 0; j < 8; ++j) amax = larger(amax, v[i][j]);
+    const RowScale s(team.max(__float_as_uint(amax)));
     if (m.id == 0) a.row_scale[t] = s.scale;
     int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
 #pragma unroll
@@ -633,7 +646,7 @@ constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
 
 // Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.  Two
 // granules a thread up to 640 threads for norms (8192 x 5120 bf16: 31.8 us, 34.4 us with four; fp32 60.6 and 76.2 us),
-// four from 192 threads on for plain quantisation, whose threads do little else (4096 x 5120: 13.5 us, 17.1 us).
+// four from 192 threads on for plain quantisation, whose threads do little else (4096 x 5120: 13.1 us, 17 with two).
 template <Mode MODE, int VPT, bool EXACT>
 struct RingShape {
   static constexpr int kThreads = VPT == 2 ? (MODE == kQuantize ? 192 : 640) : VPT == 4 ? 576 : 512;
@@ -675,9 +688,9 @@ __device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row,
 
 // A block a row at a time, rows gridDim.x apart; thread 0 keeps `depth` rows of bulk copies ahead, so DRAM is busy
 // while the block reduces.  Several small blocks an SM hide each other's reductions.  Measured (bf16): norm of
-// 8192 x 5120 31.8 us (5.3 of 6.45 TB/s), join 62.6 us (5.4 TB/s), int8 rows of 4096 x 17408 38.7 us (5.5 TB/s).
+// 8192 x 5120 31.8 us (5.3 of 6.45 TB/s), join 62.6 us (5.4 TB/s), int8 rows of 4096 x 17408 37.5 us (5.7 TB/s).
 // The issue slots are 70 to 75 % busy then, about 20 instructions an element of the join: they bound it, not DRAM.
-// Layer norms take a third reduction and odd widths single loads of their parameters (4096 x 8001: 37.6 us, 8000:
+// Layer norms take a third reduction and odd widths two loads for eight parameters (4096 x 8001: 34.4 us, 8000:
 // 28.0 us).
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)

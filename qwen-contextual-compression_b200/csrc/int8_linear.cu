@@ -190,6 +190,9 @@ __global__ void __launch_bounds__(128)
   }
   // Tensor memory is taken only once the launches ahead have finished: a CTA
   // of theirs that still waits for its own columns must not wait for ours.
+  // Beside launches of other streams an SM's 512 columns suffice: shared memory
+  // admits three of these CTAs at most (two with 128 columns each), and neither
+  // the pair kernel nor the prefill (197 and 205 KB) beside one.
   grid_dependency_wait();
   if (warp == 1) {
     tmem_alloc(&tmem_slot, S::kTmemCols);

@@ -323,6 +323,20 @@ def test_norm_quantized(rows, hidden, dtype):
                      <= 0.5 * amax / 127 + (260 + 127 * 4) * U32 * amax).all())
 
 
+@pytest.mark.parametrize("hidden", [8, 100, 1111, 5120])
+def test_norm_quantized_extremes(hidden):
+    x = make((5, hidden), torch.float32, 1)
+    x[1, hidden // 2] = float("nan")
+    x[2, 0] = float("inf")
+    x[3] = 0
+    for norm in (make_norm(hidden, "rms", torch.float32, 2, bias=False), make_norm(hidden, "layer", torch.float32, 3)):
+        q, s = norm(x, quantize=True)
+        assert bool(s[1:3].isnan().all()) and bool((q[1:3] == 0).all())
+        assert bool(s[[0, 4]].isfinite().all())
+        if norm.bias is None:
+            assert s[3] == 0 and bool((q[3] == 0).all())
+
+
 def test_streams_and_graph():
     x, residual = make((9, 5120), torch.bfloat16, 1), make((9, 5120), torch.bfloat16, 2)
     norm = make_norm(5120, "rms", torch.bfloat16, 3)
