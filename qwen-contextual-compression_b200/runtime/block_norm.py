@@ -79,7 +79,8 @@ class BlockNorm:
     for models that store the weight's difference from one.
     """
 
-    __slots__ = ("weight", "bias", "hidden", "_index", "_params", "_ref", "_weight_ptr", "_bias_ptr")
+    __slots__ = ("weight", "bias", "hidden", "_index", "_dtype", "_params", "_ref", "_weight_ptr",
+                 "_bias_ptr")
 
     def __init__(self, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, kind: str = "rms",
                  eps: float = 1e-6, weight_offset: float = 0.0):
@@ -89,23 +90,35 @@ class BlockNorm:
             raise ValueError("eps must be finite and not negative")
         if weight is None and weight_offset != 0.0:
             raise ValueError("weight_offset needs a weight")
-        self.hidden, self._index, code = None, None, _lib.DTYPE_F32
-        for p in (weight, bias):
+        self.weight, self.bias = weight, bias
+        self._params = _lib.NormParams(None, None, _lib.DTYPE_F32, KINDS[kind], weight_offset, eps)
+        self._ref = ctypes.byref(self._params)
+        self._bind()
+
+    def _bind(self) -> None:
+        """Checks weight and bias as they are now and writes them into the C argument."""
+        hidden, index, dtype, code = None, None, None, _lib.DTYPE_F32
+        for p in (self.weight, self.bias):
             if p is None:
                 continue
             if p.get_device() < 0:
                 _lib.require_cuda(p)
-            if p.dim() != 1 or not p.is_contiguous() or self.hidden not in (None, p.shape[0]):
+            if p.dim() != 1 or not p.is_contiguous() or hidden not in (None, p.shape[0]):
                 raise ValueError("weight and bias must be contiguous one-dimensional tensors of one length")
-            self.hidden, self._index, code = p.shape[0], p.get_device(), _lib.dtype_code(p.dtype)
-        if weight is not None and bias is not None:
-            if weight.dtype != bias.dtype:
+            if dtype not in (None, p.dtype):
                 raise TypeError("weight and bias must share a dtype")
-            _lib.require_cuda(weight, bias)
-        self.weight, self.bias = weight, bias
-        self._weight_ptr, self._bias_ptr = _lib.ptr(weight), _lib.ptr(bias)
-        self._params = _lib.NormParams(self._weight_ptr, self._bias_ptr, code, KINDS[kind], weight_offset, eps)
-        self._ref = ctypes.byref(self._params)
+            if index not in (None, p.get_device()):
+                raise RuntimeError("all tensors must share a device")
+            hidden, index, dtype, code = p.shape[0], p.get_device(), p.dtype, _lib.dtype_code(p.dtype)
+        self.hidden, self._index, self._dtype = hidden, index, dtype
+        self._weight_ptr, self._bias_ptr = _lib.ptr(self.weight), _lib.ptr(self.bias)
+        self._params.weight, self._params.bias = self._weight_ptr, self._bias_ptr
+        self._params.dtype = code
+
+    def _changed(self, p: torch.Tensor, ptr: int) -> bool:
+        """Whether a parameter's data was replaced (``p.data = ...``, ``module.to(...)``) since _bind."""
+        return (p.data_ptr() != ptr or p.dtype is not self._dtype or p.numel() != self.hidden
+                or p.get_device() != self._index or not p.is_contiguous())
 
     @property
     def kind(self) -> str:
@@ -121,22 +134,22 @@ class BlockNorm:
 
     def _for(self, hidden: int, index: int):
         """The norm as a C argument for rows of `hidden` values on a device, after its checks against them."""
+        weight, bias = self.weight, self.bias
+        if weight is not None:
+            if weight.requires_grad:
+                _lib.refuse_grad("BlockNorm", weight)
+            if self._changed(weight, self._weight_ptr):
+                self._bind()
+        if bias is not None:
+            if bias.requires_grad:
+                _lib.refuse_grad("BlockNorm", bias)
+            if self._changed(bias, self._bias_ptr):
+                self._bind()
         if self.hidden is not None:
             if self.hidden != hidden:
                 raise ValueError(f"the norm has {self.hidden} weights, its input {hidden} values a row")
             if self._index != index:
                 raise RuntimeError("all tensors must share a device")
-            weight, bias = self.weight, self.bias
-            if weight is not None:
-                if weight.requires_grad:
-                    _lib.refuse_grad("BlockNorm", weight)
-                if weight.data_ptr() != self._weight_ptr:  # the parameter's storage was replaced
-                    self._params.weight = self._weight_ptr = weight.data_ptr()
-            if bias is not None:
-                if bias.requires_grad:
-                    _lib.refuse_grad("BlockNorm", bias)
-                if bias.data_ptr() != self._bias_ptr:
-                    self._params.bias = self._bias_ptr = bias.data_ptr()
         return self._ref
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,

@@ -337,6 +337,35 @@ def test_norm_quantized_extremes(hidden):
             assert s[3] == 0 and bool((q[3] == 0).all())
 
 
+def test_replaced_parameters():
+    """A norm follows its parameters when a module replaces their data, and refuses what no longer fits."""
+    x = make((5, 512), torch.float32, 1)
+    weight, bias = make((512,), torch.float32, 2), make((512,), torch.float32, 3)
+    layer = torch.nn.LayerNorm(512, device="cuda").requires_grad_(False)
+    layer.weight.data, layer.bias.data = weight.clone(), bias.clone()
+    norm = BlockNorm(layer.weight, layer.bias, kind="layer")
+    assert torch.equal(norm(x), BlockNorm(weight, bias, kind="layer")(x))
+    layer.half()
+    assert torch.equal(norm(x), BlockNorm(weight.half(), bias.half(), kind="layer")(x))
+    layer.float()
+    layer.weight.data = layer.weight.data[:100]  # the same address, fewer values
+    with pytest.raises(ValueError):
+        norm(x)
+    layer.bias.data = layer.bias.data[:100]
+    with pytest.raises(ValueError):
+        norm(x)
+    assert torch.equal(norm(x[:, :100]), BlockNorm(layer.weight, layer.bias, kind="layer")(x[:, :100]))
+    layer.weight.data = torch.ones(200, device="cuda")[::2]
+    with pytest.raises(ValueError):
+        norm(x[:, :100])
+    layer.weight.data = torch.ones(100, device="cuda", dtype=torch.float16)
+    with pytest.raises(TypeError):
+        norm(x[:, :100])
+    layer.cpu()
+    with pytest.raises(RuntimeError):
+        norm(x[:, :100])
+
+
 def test_streams_and_graph():
     x, residual = make((9, 5120), torch.bfloat16, 1), make((9, 5120), torch.bfloat16, 2)
     norm = make_norm(5120, "rms", torch.bfloat16, 3)
