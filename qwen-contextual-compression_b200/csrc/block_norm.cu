@@ -83,6 +83,32 @@ struct GranuleMap {
   }
 };
 
+// Two elements an instruction, each rounded as the single one: the kernels are short of issue slots, not of
+// arithmetic (join of 8192 x 5120 bf16: 63.3 us with single instructions, 61.5 with these).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 a, b, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 a, b, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 a, b, c, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7};"
+      " fma.rn.f32x2 r, a, b, c; mov.b64 {%0, %1}, r;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// Elements 2 j and 2 j + 1 of a granule.
+__device__ __forceinline__ float2 pair(const float (&v)[8], int j) { return make_float2(v[2 * j], v[2 * j + 1]); }
+__device__ __forceinline__ void set_pair(float (&v)[8], int j, float2 p) { v[2 * j] = p.x, v[2 * j + 1] = p.y; }
+
 __device__ __forceinline__ uint32_t half_bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint32_t half_bits(__half v) { return __half_as_ushort(v); }
 
@@ -244,6 +270,13 @@ constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole n
 __device__ __forceinline__ uint32_t quantize(float x, const RowScale& s) {
   return __float_as_uint(fmaf(x, s.inverse, kMagic));
 }
+__device__ __forceinline__ void quantize8(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 r = fma2(pair(f, j), both(s.inverse), both(kMagic));
+    q[2 * j] = __float_as_uint(r.x), q[2 * j + 1] = __float_as_uint(r.y);
+  }
+}
 
 // The low bytes of four words.
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -259,10 +292,11 @@ template <typename T>
 __device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
   bool border = false;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = fmaf(f[j], s.inverse, f[j] * s.inverse_rest), m = t + kMagic;
-    q[j] = __float_as_uint(m);
-    if (sizeof(T) == 4) border |= fabsf(t - (m - kMagic)) == 0.5f;
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = pair(f, j), t = fma2(x, both(s.inverse), mul2(x, both(s.inverse_rest)));
+    const float2 r = add2(t, both(kMagic));
+    q[2 * j] = __float_as_uint(r.x), q[2 * j + 1] = __float_as_uint(r.y);
+    if (sizeof(T) == 4) border |= fabsf(t.x - (r.x - kMagic)) == 0.5f || fabsf(t.y - (r.y - kMagic)) == 0.5f;
   }
   if (sizeof(T) == 4 && border)
 #pragma unroll
@@ -293,22 +327,45 @@ struct WarpTeam {
   __device__ __forceinline__ uint32_t max(uint32_t v) { return warp_max(v); }
 };
 
-// One barrier a reduction: the halves of `scratch` [2][32] are used in turn, and a half's readers have passed the
-// next reduction's barrier before it is written again.
+// One barrier a reduction: the halves of `scratch` [2][kMaxWarps] are used in turn, and a half's readers have passed
+// the next reduction's barrier before it is written again.  Up to kFewWarps every thread joins the warps' parts from
+// wide loads, beyond them a warp's lanes by shuffles (layer norm of 2048 x 5120, 10 warps: 13.5 and 14.0 us; norm of
+// 4096 x 8001, 16 warps: 33.9 and 33.3 us).
+constexpr int kMaxWarps = 20, kFewWarps = 12;
+
 struct BlockTeam {
   float* scratch;
   int half = 0;
-  __device__ __forceinline__ float exchange(float v) {
-    const int lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
-    float* s = scratch + half * 32;
+  // Before the kernel's first barrier: the parts of warps that the block does not have are neutral.
+  static __device__ __forceinline__ void clear(float* scratch) {
+    for (int i = threadIdx.x; i < 2 * kMaxWarps; i += blockDim.x) scratch[i] = 0.f;
+  }
+  __device__ __forceinline__ const float* exchange(float v) {
+    float* s = scratch + half * kMaxWarps;
     half ^= 1;
-    if (lane == 0) s[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
     __syncthreads();
+    return s;
+  }
+  __device__ __forceinline__ float lane_part(const float* s) const {
+    const int lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x) >> 5;
     return lane < warps ? s[lane] : 0.f;  // 0: neutral for sums and for maxima of magnitudes
   }
-  __device__ __forceinline__ float sum(float v) { return warp_sum(exchange(warp_sum(v))); }
+  __device__ __forceinline__ float sum(float v) {
+    const float* s = exchange(warp_sum(v));
+    if (blockDim.x > kFewWarps * 32) return warp_sum(lane_part(s));
+    float2 lo = both(0.f), hi = both(0.f);
+#pragma unroll
+    for (int k = 0; k < kFewWarps / 4; ++k) {
+      const float4 p = reinterpret_cast<const float4*>(s)[k];
+      lo = add2(lo, make_float2(p.x, p.y)), hi = add2(hi, make_float2(p.z, p.w));
+    }
+    lo = add2(lo, hi);
+    return lo.x + lo.y;
+  }
   __device__ __forceinline__ uint32_t max(uint32_t v) {
-    return warp_max(__float_as_uint(exchange(__uint_as_float(warp_max(v)))));
+    const float* s = exchange(__uint_as_float(warp_max(v)));
+    return warp_max(__float_as_uint(lane_part(s)));
   }
 };
 
@@ -322,46 +379,45 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
                                           const GranuleMap<EXACT>& m, Team& team) {
   if (a.kind == QCC_NORM_NONE) return;
   if (a.kind == QCC_NORM_LAYER) {
-    float s = 0.f;
+    float2 s = both(0.f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[i][j];
-    const float mean = team.sum(s) * inv_n;
+      for (int j = 0; j < 4; ++j) s = add2(s, pair(v[i], j));
+    const float mean = team.sum(s.x + s.y) * inv_n;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] -= mean;
+      for (int j = 0; j < 4; ++j) set_pair(v[i], j, add2(pair(v[i], j), both(-mean)));
       if (!m.whole(i))
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (EXACT || !m.has(i, j)) v[i][j] = 0.f;
     }
   }
-  float s = 0.f;
+  float2 s = both(0.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += v[i][j] * v[i][j];
-  const float rstd = rsqrtf(team.sum(s) * inv_n + a.eps);
+    for (int j = 0; j < 4; ++j) s = fma2(pair(v[i], j), pair(v[i], j), s);
+  const float rstd = rsqrtf(team.sum(s.x + s.y) * inv_n + a.eps);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float w[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) set_pair(v[i], j, mul2(pair(v[i], j), both(rstd)));
     if (a.weight != nullptr) {
       load_param8<P>(a.weight, a.dtype, m, i, w);
       if (a.weight_offset != 0.f)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] += a.weight_offset;
+        for (int j = 0; j < 4; ++j) set_pair(w, j, add2(pair(w, j), both(a.weight_offset)));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * w[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= rstd;
+      for (int j = 0; j < 4; ++j) set_pair(v[i], j, mul2(pair(v[i], j), pair(w, j)));
     }
     if (a.bias != nullptr) {
       load_param8<P>(a.bias, a.dtype, m, i, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] += w[j];
+      for (int j = 0; j < 4; ++j) set_pair(v[i], j, add2(pair(v[i], j), pair(w, j)));
     }
   }
 }
@@ -390,7 +446,7 @@ __device__ __forceinline__ void apply_gate(float (&v)[VPT][8], const BlockNormAr
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= s;
+      for (int j = 0; j < 4; ++j) set_pair(v[i], j, mul2(pair(v[i], j), both(s)));
     return;
   }
 #pragma unroll
@@ -411,7 +467,8 @@ template <typename R, bool EXACT>
 __device__ __forceinline__ void join8(float (&v)[8], const float (&r)[8], const BlockNormArgs& a, int64_t t,
                                       const GranuleMap<EXACT>& m, int i) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = a.residual_scale * r[j] + a.branch_scale * v[j];
+  for (int j = 0; j < 4; ++j)
+    set_pair(v, j, fma2(both(a.residual_scale), pair(r, j), mul2(both(a.branch_scale), pair(v, j))));
   store_granule(static_cast<R*>(a.res_out) + t * a.ld_res_out, m, i, v);
 }
 
@@ -436,8 +493,7 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
       uint32_t q[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = quantize(v[i][j], s);
+      quantize8(v[i], s, q);
       store_int8x8(row, m, i, q);
     }
   } else if (a.out_dtype == QCC_DTYPE_F32) {
@@ -596,7 +652,9 @@ struct RowNorm {
 // One block a row; outputs are written in the last pass, so they may be the inputs themselves.  Single elements and
 // repeated reads make it slow (join of 4096 x 5120 with a residual off by 6 bytes: 167 us, 32 us on shared granules).
 __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int dtype, int res_dtype) {
-  __shared__ float scratch[64];
+  __shared__ __align__(16) float scratch[2 * kMaxWarps];
+  BlockTeam::clear(scratch);
+  __syncthreads();
   grid_dependency_wait();
   grid_dependency_trigger();
   const int64_t t = blockIdx.x;
@@ -646,10 +704,11 @@ constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
 
 // Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.  Two
 // granules a thread up to 640 threads for norms (8192 x 5120 bf16: 31.8 us, 34.4 us with four; fp32 60.6 and 76.2 us),
-// four from 192 threads on for plain quantisation, whose threads do little else (4096 x 5120: 13.1 us, 17 with two).
+// four from 192 threads on for plain quantisation, whose threads do little else (4096 x 5120: 12.5 us, 17 with two).
 template <Mode MODE, int VPT, bool EXACT>
 struct RingShape {
   static constexpr int kThreads = VPT == 2 ? (MODE == kQuantize ? 192 : 640) : VPT == 4 ? 576 : 512;
+  static_assert(kThreads <= 32 * kMaxWarps);
   static constexpr int kBlocks = EXACT && (VPT == 2 || (VPT == 4 && MODE != kJoin)) ? 2 : 1;
 };
 
@@ -688,20 +747,22 @@ __device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row,
 
 // A block a row at a time, rows gridDim.x apart; thread 0 keeps `depth` rows of bulk copies ahead, so DRAM is busy
 // while the block reduces.  Several small blocks an SM hide each other's reductions.  Measured (bf16): norm of
-// 8192 x 5120 31.8 us (5.3 of 6.45 TB/s), join 62.6 us (5.4 TB/s), int8 rows of 4096 x 17408 37.5 us (5.7 TB/s).
-// The issue slots are 70 to 75 % busy then, about 20 instructions an element of the join: they bound it, not DRAM.
-// Layer norms take a third reduction and odd widths two loads for eight parameters (4096 x 8001: 34.4 us, 8000:
-// 28.0 us).
+// 8192 x 5120 31.6 us (5.3 of 6.45 TB/s), join 61 us (5.5 TB/s), int8 rows of 4096 x 17408 37.8 us (5.7 TB/s).
+// The issue slots are 65 to 69 % busy then, 17 instructions an element of the norm, 33 of the join: they and the
+// reductions' latency bound it, not DRAM.
+// Layer norms take a second reduction (42.8 us) and odd widths two loads for eight parameters (4096 x 8001: 33.3 us,
+// 8000: 28 us).
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)
     ring_kernel(const BlockNormArgs a, int depth) {
   using P = ParamType<T, R, MODE>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMaxDepth];
-  __shared__ float scratch[64];
+  __shared__ __align__(16) float scratch[2 * kMaxWarps];
   constexpr int kResidual = MODE == kJoin ? sizeof(R) : 0;
   const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + slot_bytes(a.hidden, kResidual);
   const uint64_t policy = policy_evict_first();
+  BlockTeam::clear(scratch);
   if (threadIdx.x == 0) {
     for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
