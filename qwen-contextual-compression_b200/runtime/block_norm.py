@@ -115,11 +115,6 @@ class BlockNorm:
         self._params.weight, self._params.bias = self._weight_ptr, self._bias_ptr
         self._params.dtype = code
 
-    def _changed(self, p: torch.Tensor, ptr: int) -> bool:
-        """Whether a parameter's data was replaced (``p.data = ...``, ``module.to(...)``) since _bind."""
-        return (p.data_ptr() != ptr or p.dtype is not self._dtype or p.numel() != self.hidden
-                or p.get_device() != self._index or not p.is_contiguous())
-
     @property
     def kind(self) -> str:
         return next(name for name, code in KINDS.items() if code == self._params.kind)
@@ -134,16 +129,20 @@ class BlockNorm:
 
     def _for(self, hidden: int, index: int):
         """The norm as a C argument for rows of `hidden` values on a device, after its checks against them."""
+        # A module may have replaced its parameters' data (``p.data = ...``, ``module.to(...)``); an address has one
+        # device.
         weight, bias = self.weight, self.bias
         if weight is not None:
             if weight.requires_grad:
                 _lib.refuse_grad("BlockNorm", weight)
-            if self._changed(weight, self._weight_ptr):
+            if (weight.data_ptr() != self._weight_ptr or weight.dtype is not self._dtype
+                    or weight.numel() != self.hidden or not weight.is_contiguous()):
                 self._bind()
         if bias is not None:
             if bias.requires_grad:
                 _lib.refuse_grad("BlockNorm", bias)
-            if self._changed(bias, self._bias_ptr):
+            if (bias.data_ptr() != self._bias_ptr or bias.dtype is not self._dtype
+                    or bias.numel() != self.hidden or not bias.is_contiguous()):
                 self._bind()
         if self.hidden is not None:
             if self.hidden != hidden:
