@@ -538,9 +538,12 @@ QCC_API int qcc_indexed_ffn_prefill(const void* x, int64_t ldx, int n_tokens, in
  * Outputs of type QCC_DTYPE_I8 are int8 rows with one scale each:
  *   row_scale[t] = amax / 127,  q = round_half_even(127 * v / amax),
  * amax the row's largest magnitude; of the exact quotient where rows are taken
- * as they are (no norm), of the fp32 quotient after a norm.  A row with amax < 2^-119 gets scale 0
- * and zeros; a row that holds a NaN or an infinity gets scale NaN and zeros,
- * so that every product with it is NaN.
+ * as they are (no norm), of the quotient rounded to fp32 after a norm.  After an
+ * RMS norm without a bias the factor rsqrt(...) of the row cancels: the quotient
+ * is that of the products v * (weight_offset + weight) in fp32 (exact products
+ * for 16-bit values; with bf16 values, no offset, the exact quotient).  A row
+ * with amax < 2^-119 gets scale 0 and zeros; a row that holds a NaN or an
+ * infinity gets scale NaN and zeros, so that every product with it is NaN.
  * ------------------------------------------------------------------------- */
 #define QCC_NORM_NONE 0
 #define QCC_NORM_RMS 1

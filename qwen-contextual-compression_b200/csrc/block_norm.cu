@@ -230,25 +230,26 @@ __device__ __forceinline__ void store_granule(T* row, const GranuleMap<EXACT>& m
   }
 }
 
-// max(a, |f|), NaN if either is.
-__device__ __forceinline__ float larger(float a, float f) {
+// max(|a|, |f|, |g|), NaN if any is.
+__device__ __forceinline__ float larger(float a, float f, float g) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(f)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(f), "f"(g));
   return r;
 }
 
 // Bits of |f|: ordered like the magnitudes, infinities and then NaNs above all finite values.
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
 
-// What a row's largest magnitude (its bits) makes of its int8 form.
+// What a row's largest magnitude (its bits) makes of its int8 form, for values that `factor` (1 to 2) still has to
+// multiply: a factor of a whole row changes its scale and none of its quotients.
 struct RowScale {
   float amax, scale, inverse, inverse_rest;  // inverse 0: the row is stored as zeros
-  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+  __device__ __forceinline__ explicit RowScale(uint32_t bits, float factor = 1.f) {
     amax = __uint_as_float(bits);
-    const bool finite = bits <= 0x7F7FFFFFu, kept = finite && amax >= kSmallestAmax;
+    const bool finite = bits <= 0x7F7FFFFFu, kept = finite && amax * factor >= kSmallestAmax;
     inverse = kept ? 127.f / amax : 0.f;
     inverse_rest = kept ? fmaf(-inverse, amax, 127.f) / amax : 0.f;
-    scale = kept ? amax / 127.f : finite ? 0.f : NAN;
+    scale = kept ? amax / 127.f * factor : finite ? 0.f : NAN;
   }
 };
 
@@ -265,15 +266,16 @@ __device__ __forceinline__ int settle_border(float x, float amax, int q) {
 
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, held in the low bits
 
-// int8 of computed values (norms), in the low byte: the rounding of x * inverse, within 1.6e-5 of a step of the
-// quotient.
-__device__ __forceinline__ uint32_t quantize(float x, const RowScale& s) {
-  return __float_as_uint(fmaf(x, s.inverse, kMagic));
+// int8 of computed values (norms), in the low bytes: round_half_even of 127 x / amax rounded to fp32.  The reciprocal's
+// remainder brings the quotient within 2^-28 of itself before its rounding (2^-47 where the remainder is a normal
+// number), so a border k + 1/2 comes out as such.
+__device__ __forceinline__ float2 quotient2(float2 x, const RowScale& s) {
+  return fma2(x, both(s.inverse), mul2(x, both(s.inverse_rest)));
 }
 __device__ __forceinline__ void quantize8(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 r = fma2(pair(f, j), both(s.inverse), both(kMagic));
+    const float2 r = add2(quotient2(pair(f, j), s), both(kMagic));
     q[2 * j] = __float_as_uint(r.x), q[2 * j + 1] = __float_as_uint(r.y);
   }
 }
@@ -293,7 +295,7 @@ __device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowSc
   bool border = false;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 x = pair(f, j), t = fma2(x, both(s.inverse), mul2(x, both(s.inverse_rest)));
+    const float2 t = quotient2(pair(f, j), s);
     const float2 r = add2(t, both(kMagic));
     q[2 * j] = __float_as_uint(r.x), q[2 * j + 1] = __float_as_uint(r.y);
     if (sizeof(T) == 4) border |= fabsf(t.x - (r.x - kMagic)) == 0.5f || fabsf(t.y - (r.y - kMagic)) == 0.5f;
@@ -373,11 +375,27 @@ struct BlockTeam {
 // The arithmetic of a row.
 // ---------------------------------------------------------------------------
 
+// The int8 form of an RMS norm without a bias needs the quotients of the products value * weight only: 1 / rms is a
+// factor of the whole row.  Products of two 16-bit values are exact in fp32, and those of half the largest one's
+// magnitude lie on the border 63.5 in earnest (one in 10 000 of 5120 wide bf16 rows), where a rounding by 1 / rms
+// would decide.  So the values are multiplied by a power of two, which rounds nothing, and the rest of 1 / rms, in
+// [1, 2), goes into the row's scale.
+__device__ __forceinline__ bool keeps_ratios(const qcc_norm_params& a) {
+  return a.kind == QCC_NORM_RMS && a.bias == nullptr;
+}
+__device__ __forceinline__ float power_part(float rstd) {
+  return __uint_as_float(__float_as_uint(rstd) & 0x7F800000u);
+}
+__device__ __forceinline__ float factor_part(float rstd) {
+  return __uint_as_float((__float_as_uint(rstd) & 0x007FFFFFu) | 0x3F800000u);
+}
+
 // v <- N(v) over the row's values (entries outside the row are 0 on entry, and stay so where they are summed).
+// Returns 1 / its deviation; with `ratios` only that one's power of two has been applied.
 template <typename P, int VPT, bool EXACT, typename Team>
-__device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_params& a, float inv_n,
-                                          const GranuleMap<EXACT>& m, Team& team) {
-  if (a.kind == QCC_NORM_NONE) return;
+__device__ __forceinline__ float normalise(float (&v)[VPT][8], const qcc_norm_params& a, float inv_n,
+                                           const GranuleMap<EXACT>& m, Team& team, bool ratios = false) {
+  if (a.kind == QCC_NORM_NONE) return 1.f;
   if (a.kind == QCC_NORM_LAYER) {
     float2 s = both(0.f);
 #pragma unroll
@@ -401,11 +419,12 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
 #pragma unroll
     for (int j = 0; j < 4; ++j) s = fma2(pair(v[i], j), pair(v[i], j), s);
   const float rstd = rsqrtf(team.sum(s.x + s.y) * inv_n + a.eps);
+  const float by = ratios ? power_part(rstd) : rstd;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float w[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) set_pair(v[i], j, mul2(pair(v[i], j), both(rstd)));
+    for (int j = 0; j < 4; ++j) set_pair(v[i], j, mul2(pair(v[i], j), both(by)));
     if (a.weight != nullptr) {
       load_param8<P>(a.weight, a.dtype, m, i, w);
       if (a.weight_offset != 0.f)
@@ -420,6 +439,7 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], const qcc_norm_par
       for (int j = 0; j < 4; ++j) set_pair(v[i], j, add2(pair(v[i], j), pair(w, j)));
     }
   }
+  return rstd;
 }
 
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t e) {
@@ -477,14 +497,15 @@ template <typename P, int VPT, bool EXACT, typename Team>
 __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormArgs& a, int64_t t,
                                            const GranuleMap<EXACT>& m, Team& team) {
   if (a.out == nullptr) return;
-  normalise<P>(v, a.next, a.inv_hidden, m, team);
   if (a.out_dtype == QCC_DTYPE_I8) {
+    const bool ratios = keeps_ratios(a.next);
+    const float rstd = normalise<P>(v, a.next, a.inv_hidden, m, team, ratios);
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = larger(amax, v[i][j]);
-    const RowScale s(team.max(__float_as_uint(amax)));
+      for (int j = 0; j < 8; j += 2) amax = larger(amax, v[i][j], v[i][j + 1]);
+    const RowScale s(team.max(__float_as_uint(amax)), ratios ? factor_part(rstd) : 1.f);
     if (m.id == 0) a.row_scale[t] = s.scale;
     int8_t* row = static_cast<int8_t*>(a.out) + t * a.ld_out;
 #pragma unroll
@@ -496,7 +517,10 @@ __device__ __forceinline__ void finish_row(float (&v)[VPT][8], const BlockNormAr
       quantize8(v[i], s, q);
       store_int8x8(row, m, i, q);
     }
-  } else if (a.out_dtype == QCC_DTYPE_F32) {
+    return;
+  }
+  normalise<P>(v, a.next, a.inv_hidden, m, team);
+  if (a.out_dtype == QCC_DTYPE_F32) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) store_granule(static_cast<float*>(a.out) + t * a.ld_out, m, i, v[i]);
   } else {
@@ -623,11 +647,11 @@ __global__ void __launch_bounds__(32 * kWarpRows) warp_kernel(const BlockNormArg
   finish_row<P>(v, a, t, m, team);
 }
 
-// One norm's row statistics and an element's normed value.
+// One norm's row statistics and an element's normed value, without `factor` where the norm's ratios are wanted.
 struct RowNorm {
-  float mean = 0.f, rstd = 1.f;
+  float mean = 0.f, rstd = 1.f, factor = 1.f;
   template <typename F>
-  __device__ __forceinline__ RowNorm(const qcc_norm_params& p, int n, BlockTeam& team, F value) {
+  __device__ __forceinline__ RowNorm(const qcc_norm_params& p, int n, BlockTeam& team, F value, bool ratios = false) {
     if (p.kind == QCC_NORM_NONE) return;
     float s = 0.f;
     if (p.kind == QCC_NORM_LAYER) {
@@ -640,6 +664,7 @@ struct RowNorm {
       s += d * d;
     }
     rstd = 1.f / sqrtf(team.sum(s) / static_cast<float>(n) + p.eps);
+    if (ratios) factor = factor_part(rstd), rstd = power_part(rstd);
   }
   __device__ __forceinline__ float apply(const qcc_norm_params& p, float v, int e) const {
     if (p.kind == QCC_NORM_NONE) return v;
@@ -671,12 +696,14 @@ __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int d
                                (t / a.gate.rows_each) * a.gate.ld + (a.gate.cols == 1 ? 0 : e)), a.gate.act);
     return a.residual_scale * load_any(a.res, res_dtype, t * a.ld_res + e) + a.branch_scale * v;
   };
-  const RowNorm next(a.next, n, team, joined);
+  const bool to_int8 = a.out != nullptr && a.out_dtype == QCC_DTYPE_I8, ratios = to_int8 && keeps_ratios(a.next);
+  const RowNorm next(a.next, n, team, joined, ratios);
+  const bool as_is = a.res == nullptr && a.next.kind == QCC_NORM_NONE;
   RowScale s(0u);
-  if (a.out != nullptr && a.out_dtype == QCC_DTYPE_I8) {
+  if (to_int8) {
     uint32_t amax = 0;
     for (int e = threadIdx.x; e < n; e += blockDim.x) amax = max(amax, magnitude(next.apply(a.next, joined(e), e)));
-    s = RowScale(team.max(amax));
+    s = RowScale(team.max(amax), next.factor);
     if (threadIdx.x == 0) a.row_scale[t] = s.scale;
   }
   for (int e = threadIdx.x; e < n; e += blockDim.x) {
@@ -684,11 +711,11 @@ __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int d
     if (a.res != nullptr) store_as(a.res_out, t * a.ld_res_out + e, res_dtype, r);
     if (a.out == nullptr) continue;
     const float x = next.apply(a.next, r, e);
-    if (a.out_dtype == QCC_DTYPE_I8)
+    if (to_int8)
       static_cast<int8_t*>(a.out)[t * a.ld_out + e] = static_cast<int8_t>(
-          s.inverse == 0.f                                      ? 0
-          : a.res == nullptr && a.next.kind == QCC_NORM_NONE ? settle_border(x, s.amax, __float2int_rn(x * s.inverse))
-                                                             : static_cast<int>(quantize(x, s)));
+          s.inverse == 0.f ? 0
+          : as_is          ? settle_border(x, s.amax, __float2int_rn(x * s.inverse))
+                           : __float2int_rn(quotient2(both(x), s).x));
     else
       store_as(a.out, t * a.ld_out + e, a.out_dtype, x);
   }

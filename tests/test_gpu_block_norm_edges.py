@@ -1,0 +1,96 @@
+"""Block norms, the join and row quantisation where they can go wrong: borders of the int8 form."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import conftest  # noqa: F401
+from qcc_b200.runtime.block_norm import BlockNorm, residual_norm
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def make(shape, dtype, seed, scale=1.0, shift=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=gen) * scale + shift).to(dtype).cuda()
+
+
+def int8_of_products(u):
+    """round_half_even of 127 u / amax in fp32, for fp32 products u.  In float64 127 u is exact, and its quotient's
+    rounding to float64 moves it over no border between two fp32 numbers: a quotient of a 31-bit by a 24-bit number
+    that is no such border is 2^-49 or more of itself away from one."""
+    u = u.double()
+    amax = u.abs().amax(-1, keepdim=True)
+    return torch.round((127 * u / amax).float()).to(torch.int8), amax
+
+
+def rows_with_ties(rows, hidden, dtype, weight_dtype, seed):
+    """Rows and weights whose products reach half of the largest one in many places, by factors of other significands."""
+    x = make((rows, hidden), dtype, seed, 0.3).clamp(-1.5, 1.5)
+    w = make(hidden, weight_dtype, seed + 1, 0.1, 1.0).clamp(0.5, 1.5)
+    big_x = (3.0 + 0.5 * torch.rand(rows, 1, generator=torch.Generator().manual_seed(seed + 2))).to(BF16)
+    big_w = 1.2109375
+    x[:, hidden // 3] = big_x[:, 0].to(dtype).cuda()
+    w[hidden // 3] = big_w
+    ties = torch.arange(0, hidden, 7, device="cuda")
+    ties = ties[ties != hidden // 3]
+    half, same = ties[::2], ties[1::2]
+    x[:, half], w[half] = (big_x / 2).to(dtype).cuda(), big_w       # half the value, the same weight
+    x[:, same], w[same] = (big_x / 4).to(dtype).cuda().neg(), 2 * big_w
+    return x, w
+
+
+# Rows of a warp, of many warps, of the ring (refilled at 2200 x 2056 and 1300 x 4001), and of the kernel of single
+# elements (16-bit rows with weights of the other 16-bit type).
+@pytest.mark.parametrize("rows,hidden", [(3, 40), (5, 517), (9, 1000), (2049, 1536), (6, 5120), (2200, 2056),
+                                         (1300, 4001), (2, 20000)])
+@pytest.mark.parametrize("dtype,weight_dtype", [(BF16, BF16), (BF16, FP32), (FP16, FP16), (FP32, BF16), (FP32, FP32),
+                                                (BF16, FP16), (FP16, BF16)])
+def test_int8_of_an_rms_norm_rounds_the_products_quotient(rows, hidden, dtype, weight_dtype):
+    x, w = rows_with_ties(rows, hidden, dtype, weight_dtype, 3)
+    for offset in (0.0, 1.0):
+        weight = (w.float() - offset).to(weight_dtype)
+        norm = BlockNorm(weight, weight_offset=offset)
+        u = x.float() * (weight.float() + offset)
+        want, amax = int8_of_products(u)
+        q, s = norm(x, quantize=True)
+        assert torch.equal(q, want)
+        # The scale: the mean of squares is within 43 * 2^-24 of exact (its root halves that), and rsqrt, the product,
+        # the quotient and the factor round 6 times.
+        size = (x.double().square().mean(1, keepdim=True) + norm.eps).sqrt()
+        exact = amax / size / 127
+        assert bool(((s.double()[:, None] - exact).abs() <= (22 + 6) * U32 * exact).all())
+        if offset == 0.0 and dtype == weight_dtype:
+            # Behind a join: the sum of branch and residual, rounded to fp32, takes the rows' place.
+            residual = make((rows, hidden), dtype, 9, 0.25)
+            want, _ = int8_of_products((x.float() + residual.float()) * weight.float())
+            r, (q, s) = residual_norm(x, residual, next_norm=norm, quantize=True)
+            assert torch.equal(q, want)
+
+
+def test_int8_of_an_rms_norm_without_a_weight():
+    x = make((7, 3000), BF16, 1)
+    x[:, 5] = 8.0
+    x[:, 9] = -4.0
+    q, s = BlockNorm()(x, quantize=True)
+    want, amax = int8_of_products(x.float())
+    assert torch.equal(q, want) and bool((q[:, 9] == -64).all())
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_int8_of_an_rms_norm_of_tiny_and_huge_rows(eps):
+    """The row factor is a power of two and a rest: rows near fp32's ends keep their ratios and their scales."""
+    base = make((6, 520), FP32, 4)
+    x = base * torch.tensor([2.0 ** -60, 2.0 ** -58, 1.0, 2.0 ** 50, 2.0 ** 58, 0.0], device="cuda")[:, None]
+    w = make(520, FP32, 5, 0.2, 1.0)
+    q, s = BlockNorm(w, eps=eps)(x, quantize=True)
+    want, amax = int8_of_products(x * w)
+    assert torch.equal(q[:5], want[:5])
+    exact = amax / (x.double().square().mean(1, keepdim=True) + eps).sqrt() / 127
+    # Squares that fall below 2^-126 are off by 2^-150 each, 2^-36 of a row's sum of 2^-112 or more.
+    assert bool(((s[:5].double()[:, None] - exact[:5]).abs() <= 28 * U32 * exact[:5]).all())
+    assert bool(s[5].isnan()) if eps == 0.0 else float(s[5]) == 0.0
+    assert bool((q[5] == 0).all())
