@@ -115,6 +115,7 @@ SIGNATURES = {
     "qcc_indexed_ffn_prefill": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_void_p, _c_int64, _c_int,
                                          _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_int64, _c_int,
                                          _c_void_p]),
+    "qcc_set_wait_limit": (_c_int, [ctypes.c_uint64]),
     "qcc_norm_rows": (_c_int, [_c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int64, _c_int,
                                _c_void_p, _c_void_p]),
     "qcc_residual_norm": (_c_int, [_c_void_p, _c_int64, _c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_void_p,

@@ -38,7 +38,7 @@ namespace qcc {
 namespace {
 
 constexpr int kMaxHidden = 32768;
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kDrainNs = 2000000000ull;  // for copies in flight after a wait that ran out
 // A row whose largest magnitude is below this is stored as zeros: its scale
 // (and 127 / amax) would leave the normal fp32 range.
 constexpr float kSmallestAmax = 1.504632769052528e-36f;   // 2^-119
@@ -61,6 +61,7 @@ struct BlockNormArgs {
   int shift0;             // elements of row 0 before its first 16-byte boundary's granule, 0..7
   bool gate_in_granules;  // the gate's rows, in the branch's type, share its granules
   float inv_hidden;       // 1 / hidden
+  uint64_t wait_ns;       // bound of the ring's waits for its copies
 };
 
 // ---------------------------------------------------------------------------
@@ -728,6 +729,9 @@ constexpr int kMaxDepth = 8;
 // Shared memory that a ring kernel's blocks on an SM share: two rows each in kRoom, more rows each only within
 // kDeepRoom (what is left caches the parameters: 208 KB of rings cost the norm of 8192 x 5120 rows 10 %).
 constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
+// Threads of an SM's ring blocks together: more blocks leave each a shallower ring (norm of 8192 x 5120, blocks of 320
+// threads: 30.7 us with four and three rows each, 35.6 with five and two).
+constexpr int kMostThreads = 1344;
 
 // Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.  Two
 // granules a thread up to 640 threads for norms (8192 x 5120 bf16: 31.8 us, 34.4 us with four; fp32 60.6 and 76.2 us),
@@ -772,6 +776,34 @@ __device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row,
   return to_words(e);
 }
 
+template <typename T>
+__host__ __device__ constexpr int code_of() {
+  return std::is_same_v<T, __nv_bfloat16> ? QCC_DTYPE_BF16 : std::is_same_v<T, __half> ? QCC_DTYPE_F16 : QCC_DTYPE_F32;
+}
+
+// The end of a block whose wait for row t (slot s) ran out: its rows from t on become NaN (int8: zeros, and NaN as the
+// scale), and thread 0 sees the copies in flight in, which would land in the shared memory of a later block.  Not
+// inlined: the registers of this path would cost the norms 15 %.
+__device__ __noinline__ void give_up(const BlockNormArgs& a, int res_dtype, uint64_t* full, int depth, int64_t t, int s,
+                                     int phase) {
+  if (threadIdx.x == 0)
+    for (int64_t u = t, k = 0; k < depth && u < a.rows; ++k, u += gridDim.x) {
+      mbar_wait_suspended(&full[s], phase, kDrainNs);
+      if (++s == depth) s = 0, phase ^= 1;
+    }
+  for (; t < a.rows; t += gridDim.x) {
+    for (int e = threadIdx.x; e < a.hidden; e += blockDim.x) {
+      if (a.res_out != nullptr) store_as(a.res_out, t * a.ld_res_out + e, res_dtype, NAN);
+      if (a.out == nullptr) continue;
+      if (a.out_dtype == QCC_DTYPE_I8)
+        static_cast<int8_t*>(a.out)[t * a.ld_out + e] = 0;
+      else
+        store_as(a.out, t * a.ld_out + e, a.out_dtype, NAN);
+    }
+    if (threadIdx.x == 0 && a.out != nullptr && a.out_dtype == QCC_DTYPE_I8) a.row_scale[t] = NAN;
+  }
+}
+
 // A block a row at a time, rows gridDim.x apart; thread 0 keeps `depth` rows of bulk copies ahead, so DRAM is busy
 // while the block reduces.  Several small blocks an SM hide each other's reductions.  Measured (bf16): norm of
 // 8192 x 5120 31.6 us (5.3 of 6.45 TB/s), join 61 us (5.5 TB/s), int8 rows of 4096 x 17408 37.8 us (5.7 TB/s).
@@ -781,17 +813,18 @@ __device__ __forceinline__ Pack8<E> load_slot(const uint8_t* slot, const E* row,
 // 8000: 28 us).
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)
-    ring_kernel(const BlockNormArgs a, int depth) {
+    ring_kernel(const __grid_constant__ BlockNormArgs a, int depth) {
   using P = ParamType<T, R, MODE>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t full[kMaxDepth];
+  __shared__ volatile int missing[2][kMaxDepth];  // by the phase and slot of a row whose copies did not arrive
   __shared__ __align__(16) float scratch[2 * kMaxWarps];
   constexpr int kResidual = MODE == kJoin ? sizeof(R) : 0;
   const int y_bytes = slot_bytes(a.hidden, sizeof(T)), bytes = y_bytes + slot_bytes(a.hidden, kResidual);
   const uint64_t policy = policy_evict_first();
   BlockTeam::clear(scratch);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < depth; ++s) mbar_init(&full[s], 1), missing[0][s] = missing[1][s] = 0;
     fence_barrier_init();
   }
   __syncthreads();
@@ -818,11 +851,10 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     const GranuleMap<EXACT> m = {a.hidden, shift, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
     const RowCopy c(a, t, shift);
     const uint8_t* slot = ring + s * bytes;
-    const bool arrived = mbar_wait_suspended(&full[s], phase, kWaitNs);
+    if (!mbar_wait_suspended(&full[s], phase, a.wait_ns)) missing[phase][s] = 1;
     Pack8<T> words[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) words[i] = load_slot(slot, y + t * a.ldy, c, m, i);
-    if (!arrived) words[0].w[0].x = 0xFFFFFFFFu;  // a NaN in every type: the row becomes NaN by its sums or its scale
     float v[VPT][8];
     if (MODE != kQuantize)
 #pragma unroll
@@ -837,7 +869,13 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
         join8<R>(v[i], r, a, t, m, i);
       }
     }
-    __syncthreads();  // the slot has been read
+    // The slot has been read; by a thread whose wait ran out perhaps too early, and then the block writes NaN over what
+    // it made of the row.  A thread that is a row ahead of this test marks that row's own entry.
+    __syncthreads();
+    if (missing[phase][s] != 0) {
+      give_up(a, code_of<R>(), full, depth, t, s, phase);
+      return;
+    }
     const int64_t ahead = t + static_cast<int64_t>(depth) * gridDim.x;
     if (threadIdx.x == 0 && ahead < a.rows) fetch(ahead, s);
     if (MODE == kQuantize)
@@ -888,7 +926,7 @@ bool launch_ring(const BlockNormArgs& a, int granules, int device, cudaStream_t 
     cudaFuncAttributes attr;
     return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? (attr.numRegs + 7) / 8 * 8 : 128;
   }();
-  const int resident = std::max(1, std::min(65536 / (regs * threads), 2048 / threads));
+  const int resident = std::max(1, std::min(65536 / (regs * threads), kMostThreads / threads));
   const int blocks = std::max(1, std::min(resident, kRoom / (2 * slot)));
   const int64_t grid = std::min<int64_t>(a.rows, static_cast<int64_t>(device_info(device).num_sms) * blocks);
   const int64_t each = (a.rows + grid - 1) / grid;
@@ -921,11 +959,6 @@ bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStrea
   return launch_ring<T, R, MODE, 8, EXACT>(a, granules, device, stream);
 }
 
-template <typename T>
-constexpr int code_of() {
-  return std::is_same_v<T, __nv_bfloat16> ? QCC_DTYPE_BF16 : std::is_same_v<T, __half> ? QCC_DTYPE_F16 : QCC_DTYPE_F32;
-}
-
 template <typename T, typename R, Mode MODE>
 bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStream_t stream) {
   constexpr int es = sizeof(T), rs = sizeof(R);
@@ -936,6 +969,7 @@ bool launch_rows(BlockNormArgs a, int dtype, int res_dtype, int device, cudaStre
     return (p.weight == nullptr && p.bias == nullptr) || known(p.dtype);
   };
   a.inv_hidden = 1.f / static_cast<float>(a.hidden);
+  a.wait_ns = wait_limit_ns();
   a.shift0 = static_cast<int>(reinterpret_cast<uintptr_t>(a.y) / es % 8);
   const bool row_gate = a.gate.values != nullptr && a.gate.cols > 1;
   const bool together =

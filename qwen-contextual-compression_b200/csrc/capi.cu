@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -17,6 +18,7 @@ namespace qcc {
 
 namespace {
 thread_local cudaError_t g_last_error = cudaSuccess;
+std::atomic<uint64_t> g_wait_limit_ns{2000000000ull};
 
 // record n = [gate[n, :Hp] | up[n, :Hp] | down[:Hp, n]], zero padded.
 // Grid-stride over (record, element) pairs: consecutive threads of a warp
@@ -86,6 +88,8 @@ void record_cuda_error(cudaError_t err) {
   if (err != cudaSuccess) g_last_error = err;
 }
 
+uint64_t wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+
 bool cuda_ok(cudaError_t err) {
   if (err == cudaSuccess) return true;
   record_cuda_error(err);
@@ -136,6 +140,11 @@ bool ensure_max_dynamic_smem(const void* kernel, int device) {
 }
 
 }  // namespace qcc
+
+extern "C" int qcc_set_wait_limit(uint64_t limit_ns) {
+  qcc::g_wait_limit_ns.store(limit_ns, std::memory_order_relaxed);
+  return QCC_OK;
+}
 
 extern "C" int qcc_version(void) { return QCC_ABI_VERSION; }
 

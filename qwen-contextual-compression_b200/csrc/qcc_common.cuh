@@ -72,11 +72,25 @@ __device__ __forceinline__ void grid_dependency_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// The same wait for threads that have nothing else to do: each try lets the
+// One look at a barrier's phase, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// The bounded wait for threads that have nothing else to do: each try lets the
 // hardware suspend the thread (for up to 100 us), so that waiting warps leave
-// the issue slots to the working ones.
+// the issue slots to the working ones.  A limit of 0 looks once.
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_test(bar, parity)) return true;
+  if (limit_ns == 0) return false;
   const uint64_t start = global_timer_ns();
   while (true) {
     uint32_t done;

@@ -45,6 +45,9 @@ void record_cuda_error(cudaError_t err);
 void clear_stale_error();
 bool launch_ok();
 
+// Bound of the block norms' waits (qcc_set_wait_limit).
+uint64_t wait_limit_ns();
+
 int decode_max_batch(int hidden, int dtype);
 size_t decode_workspace_bytes(int batch, int hidden, int dtype);
 

@@ -1,11 +1,12 @@
-"""Block norms, the join and row quantisation where they can go wrong: borders of the int8 form."""
+"""Block norms, the join and row quantisation where they can go wrong: borders of the int8 form, waits that run out."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 import conftest  # noqa: F401
-from qcc_b200.runtime.block_norm import BlockNorm, residual_norm
+from qcc_b200 import _lib
+from qcc_b200.runtime.block_norm import BlockNorm, quantize_rows, residual_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,57 @@ def test_int8_of_an_rms_norm_of_tiny_and_huge_rows(eps):
     assert bool(((s[:5].double()[:, None] - exact[:5]).abs() <= 28 * U32 * exact[:5]).all())
     assert bool(s[5].isnan()) if eps == 0.0 else float(s[5]) == 0.0
     assert bool((q[5] == 0).all())
+
+
+@pytest.fixture
+def no_waiting():
+    """Launches made inside give up at once unless their copies are there already."""
+    lib = _lib.library()
+    assert lib.qcc_set_wait_limit(0) == _lib.OK
+    yield
+    lib.qcc_set_wait_limit(2_000_000_000)
+    torch.cuda.synchronize()
+
+
+def given_up_or(got, want):
+    """Every row is the right one or NaN all over; returns how many are NaN."""
+    nan = got.isnan()
+    lost = nan.all(-1)
+    assert torch.equal(nan.any(-1), lost)
+    assert torch.equal(got[~lost], want[~lost])
+    return int(lost.sum())
+
+
+@pytest.mark.parametrize("rows,hidden", [(300, 5120), (2300, 5120), (2300, 4001), (3, 20000), (700, 9000)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_a_wait_that_runs_out_leaves_whole_rows_of_nan(rows, hidden, dtype, request):
+    x, residual = make((rows, hidden), dtype, 1), make((rows, hidden), dtype, 2)
+    norm = BlockNorm(make(hidden, dtype, 3, 0.1, 1.0))
+
+    def calls():
+        alone = residual_norm(x, residual, branch_scale=0.5)  # no reduction between the copies and the sum's store
+        r, y = residual_norm(x, residual, post=norm, next_norm=norm)
+        r8, (q, s) = residual_norm(x, residual, next_norm=norm, quantize=True)
+        return [alone, r, y, r8, norm(x)], [(q, s), norm(x, quantize=True), quantize_rows(x)]
+
+    want = calls()
+    for flat in want[0]:
+        assert not bool(flat.isnan().any())
+    request.getfixturevalue("no_waiting")
+    floats, ints = calls()
+    torch.cuda.synchronize()
+    for got, right in zip(floats, want[0]):
+        assert given_up_or(got, right) > 0
+    for (q, s), (right_q, right_s) in zip(ints, want[1]):
+        lost = s.isnan()
+        assert bool(lost.any()) and bool((q[lost] == 0).all())
+        assert torch.equal(q[~lost], right_q[~lost]) and torch.equal(s[~lost], right_s[~lost])
+    # In place, then with the ordinary bound again: nothing of the launches that gave up arrives later.
+    alone = residual_norm(x, residual.clone(), branch_scale=0.5, residual_out=residual.clone())
+    assert given_up_or(alone, want[0][0]) > 0
+    _lib.library().qcc_set_wait_limit(2_000_000_000)
+    again = calls()
+    for got, right in zip(again[0], want[0]):
+        assert torch.equal(got, right)
+    for (q, s), (right_q, right_s) in zip(again[1], want[1]):
+        assert torch.equal(q, right_q) and torch.equal(s, right_s)
