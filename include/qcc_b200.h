@@ -574,12 +574,13 @@ typedef struct qcc_gate_params {
   int act;
 } qcc_gate_params;
 
-/* Bound, in ns, on each wait of the block norms' later launches for their own
- * copies (2 s until set; 0: a wait looks once and gives up unless the copies
- * are there already).  A launch whose wait ran out leaves the rows that it
- * still had to write as NaN (int8: zeros and a scale of NaN), sees its copies
- * in and ends; there is no status word.  Process-wide; a captured launch keeps
- * the bound that it was captured with. */
+/* Bound, in ns, on each wait of later launches of the block norms and of the
+ * 8-bit integer products for their own copies (2 s until set, 60 s at most; 0:
+ * a wait looks once and gives up unless the copies are there already).  A
+ * block whose wait ran out leaves the rows or the tiles that it still had to
+ * write as NaN (int8: zeros and a scale of NaN), sees its copies in and ends;
+ * there is no status word.  Process-wide; a captured launch keeps the bound
+ * that it was captured with. */
 QCC_API int qcc_set_wait_limit(uint64_t limit_ns);
 
 /* out[t] = N(x[t]) for the rows of x [rows, hidden] (row stride ldx >= hidden,

@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     const GranuleMap<EXACT> m = {a.hidden, shift, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
     const RowCopy c(a, t, shift);
     const uint8_t* slot = ring + s * bytes;
-    if (!mbar_wait_suspended(&full[s], phase, a.wait_ns)) missing[phase][s] = 1;
+    if (!mbar_wait_suspended<true>(&full[s], phase, a.wait_ns)) missing[phase][s] = 1;
     Pack8<T> words[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) words[i] = load_slot(slot, y + t * a.ldy, c, m, i);

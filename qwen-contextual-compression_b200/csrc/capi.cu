@@ -142,6 +142,7 @@ bool ensure_max_dynamic_smem(const void* kernel, int device) {
 }  // namespace qcc
 
 extern "C" int qcc_set_wait_limit(uint64_t limit_ns) {
+  if (limit_ns > 60000000000ull) return QCC_ERR_INVALID_ARGUMENT;
   qcc::g_wait_limit_ns.store(limit_ns, std::memory_order_relaxed);
   return QCC_OK;
 }

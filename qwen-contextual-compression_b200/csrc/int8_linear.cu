@@ -33,6 +33,7 @@ struct Int8Args {
   void* y;
   int64_t ldy;
   int y_dtype;
+  uint64_t wait_ns;  // bound of the waits for copies and for free slots
 };
 
 // silu with the fast exponential and quotient: exp's argument rounds once (an
@@ -56,14 +57,16 @@ __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) 
 // Gated: 32 lanes are 16 gate rows and the up rows of the same 16 channels, so
 // one shuffle brings two tokens' gate and up together and every lane has one
 // output of the two to finish.
-// Waits are bounded; a tile whose wait ran out is written as NaN.
+// Waits are bounded.  A CTA (or pair) whose wait ran out starts nothing more,
+// sees its MMAs and copies in (copies would land in the shared memory of a
+// later block) and writes NaN: the stream kernel its tile, a pair all its tiles.
 // ---------------------------------------------------------------------------
 
 constexpr int kTileRows = 128;  // weight rows of a CTA's tile: TMEM lanes
 constexpr int kTileCols = 128;  // bytes of K per stage (one swizzled row)
 constexpr uint32_t kMaxSplit = 8;  // CTAs of a stream kernel's cluster, at most
 constexpr int kAhead = 6;       // blocks of the weight that a stream kernel's CTA brings to L2 before it waits
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kDrainNs = 2000000000ull;  // for MMAs and copies in flight after a wait that ran out
 
 // What one lane needs to finish its weight row's outputs.
 template <bool GATED, typename O>
@@ -204,12 +207,12 @@ __global__ void __launch_bounds__(128)
   const uint32_t tmem = tmem_slot;
   grid_dependency_trigger();
 
+  int issued = 0;  // thread 0: blocks whose copies it started
   if (threadIdx.x == 0) {
     const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
-    int issued = 0;
     for (; issued < count; ++issued) {
       const int s = issued % STAGES;
-      if (issued >= STAGES && !mbar_wait_suspended(&empty[s], (issued / STAGES - 1) & 1, kWaitNs)) {
+      if (issued >= STAGES && !mbar_wait_suspended(&empty[s], (issued / STAGES - 1) & 1, a.wait_ns)) {
         failed = 1;
         break;
       }
@@ -225,15 +228,11 @@ __global__ void __launch_bounds__(128)
       }
       tma_load_2d_hint(w + S::kWBytes, &tm_x, k, t0, &full[s], keep);
     }
-    // A copy must not land after this CTA has gone: after a wait that ran out, see the issued ones in.
-    if (issued < count)
-      for (int i = max(0, issued - STAGES); i < issued; ++i)
-        mbar_wait_suspended(&full[i % STAGES], (i / STAGES) & 1, kWaitNs);
   } else if (threadIdx.x == 32) {
     constexpr uint32_t idesc = idesc_s8(kTileRows, BN);
     for (int i = 0; i < count; ++i) {
       const int s = i % STAGES;
-      if (!mbar_wait_suspended(&full[s], (i / STAGES) & 1, kWaitNs)) {
+      if (!mbar_wait_suspended(&full[s], (i / STAGES) & 1, a.wait_ns)) {
         failed = 1;
         break;
       }
@@ -248,9 +247,15 @@ __global__ void __launch_bounds__(128)
     tc_commit(&done);
   }
   __syncwarp();
-  if (!mbar_wait_suspended(&done, 0, 4 * kWaitNs)) failed = 1;
+  if (!mbar_wait_suspended(&done, 0, 4 * max(a.wait_ns, kDrainNs))) failed = 1;
   tc_fence_after_sync();
   __syncthreads();
+  if (failed != 0) {
+    if (threadIdx.x == 0)
+      for (int i = max(0, issued - STAGES); i < issued; ++i)
+        mbar_wait_suspended(&full[i % STAGES], (i / STAGES) & 1, kDrainNs);
+    __syncthreads();
+  }
 
   const int tokens = min(BN, a.tokens - t0);
   const uint32_t from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed;
+  __shared__ int failed, issued;  // issued: column blocks whose copies this CTA started
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank;
@@ -397,8 +402,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = tmem_slot;
   grid_dependency_trigger();
 
-  if (threadIdx.x == 0) {
+  // This CTA's copies of column block b of a tile into stage s, counted (with the other CTA's) on the even CTA's barrier.
+  const auto load = [&](int row, int token, int b, int s) {
     const uint64_t keep = policy_evict_last();
+    uint8_t* w = ring + s * kPairStage;
+    const uint32_t bar = cluster_addr(&full[s], 0);
+    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (128 + half_tokens) * kTileCols);
+    const int k = b * kTileCols;
+    if (GATED) {
+      const int n0 = row * kChannels + static_cast<int>(rank) * 64;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        tma_load_3d_pair(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, 0, bar, keep);
+    } else {
+      tma_load_2d_pair(w, &tm_w, k, row * kChannels + static_cast<int>(rank) * 128, bar, keep);
+    }
+    tma_load_2d_pair(w + 128 * kTileCols, &tm_x, k, token * plan.tile_tokens + static_cast<int>(rank) * half_tokens,
+                     bar, keep);
+  };
+
+  if (threadIdx.x == 0) {
     int n = 0;  // stage uses so far
     bool ok = true;
     for (int i = pair; i < tiles && ok; i += pairs) {
@@ -406,40 +429,22 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       pair_tile(plan, i, row, token);
       for (int b = 0; b < blocks; ++b, ++n) {
         const int s = n % kPairStages;
-        if (n >= kPairStages && !mbar_wait_suspended(&empty[s], (n / kPairStages - 1) & 1, kWaitNs)) {
+        if (n >= kPairStages && !mbar_wait_suspended(&empty[s], (n / kPairStages - 1) & 1, a.wait_ns)) {
+          note_failure(&failed, rank);
           ok = false;
           break;
         }
-        uint8_t* w = ring + s * kPairStage;
-        const uint32_t bar = cluster_addr(&full[s], 0);
-        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (128 + half_tokens) * kTileCols);
-        const int k = b * kTileCols;
-        if (GATED) {
-          const int n0 = row * kChannels + static_cast<int>(rank) * 64;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            tma_load_3d_pair(w + q * 32 * kTileCols, &tm_w, k, n0 + q * 16, 0, bar, keep);
-        } else {
-          tma_load_2d_pair(w, &tm_w, k, row * kChannels + static_cast<int>(rank) * 128, bar, keep);
-        }
-        tma_load_2d_pair(w + 128 * kTileCols, &tm_x, k, token * plan.tile_tokens + static_cast<int>(rank) * half_tokens,
-                         bar, keep);
+        load(row, token, b, s);
       }
     }
-    if (!ok) {
-      note_failure(&failed, rank);
-      // Copies in flight land before the cluster's last barrier: the even CTA's barriers count both CTAs' bytes.
-      if (rank == 0)
-        for (int i = max(0, n - kPairStages); i < n; ++i)
-          mbar_wait_suspended(&full[i % kPairStages], (i / kPairStages) & 1, kWaitNs);
-    }
+    issued = n;
   } else if (threadIdx.x == 32 && rank == 0) {
     const uint32_t idesc = idesc_s8(256, plan.tile_tokens);
     int n = 0, done = 0;
     bool ok = true;
     for (int i = pair; i < tiles && ok; i += pairs, ++done) {
       const int acc = done & 1;
-      if (done >= 2 && !mbar_wait_suspended(&acc_empty[acc], (done / 2 - 1) & 1, kWaitNs)) {
+      if (done >= 2 && !mbar_wait_suspended(&acc_empty[acc], (done / 2 - 1) & 1, a.wait_ns)) {
         note_failure(&failed, rank);
         ok = false;
         break;
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tc_fence_after_sync();
       for (int b = 0; b < blocks; ++b, ++n) {
         const int s = n % kPairStages;
-        if (!mbar_wait_suspended(&full[s], (n / kPairStages) & 1, kWaitNs)) {
+        if (!mbar_wait_suspended(&full[s], (n / kPairStages) & 1, a.wait_ns)) {
           note_failure(&failed, rank);
           ok = false;
           break;
@@ -462,13 +467,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       tc_commit_pair(&acc_full[acc]);
     }
+    if (!ok && done > 0) mbar_wait_suspended(&acc_full[(done - 1) & 1], ((done - 1) / 2) & 1, kDrainNs);
   } else if (warp >= 2) {
     const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
     int done = 0;
     bool broken = false;
     for (int i = pair; i < tiles; i += pairs, ++done) {
       const int acc = done & 1;
-      if (!broken && !mbar_wait_suspended(&acc_full[acc], (done / 2) & 1, 4 * kWaitNs)) note_failure(&failed, rank);
+      if (!broken && !mbar_wait_suspended(&acc_full[acc], (done / 2) & 1, 4 * max(a.wait_ns, kDrainNs)))
+        note_failure(&failed, rank);
       broken = *static_cast<volatile int*>(&failed) != 0;  // and all tiles after it: their waits would run out too
       tc_fence_after_sync();
       int row, token;
@@ -500,6 +507,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before_sync();
   cluster_sync();  // no barrier of this CTA is signalled and none of its memory read after this
   tc_fence_after_sync();
+  if (*static_cast<volatile int*>(&failed) != 0) {  // in both CTAs or in neither
+    if (threadIdx.x == 0) {
+      // The even CTA's barriers complete by both CTAs' bytes: the CTA that started fewer blocks starts the others,
+      // whose stages are free (the other CTA found them so), and the even one sees all of them in.
+      const int most = max(issued, cluster_load(smem_addr(&issued), rank ^ 1u));
+      for (int n = issued; n < most; ++n) {
+        int row, token;
+        pair_tile(plan, pair + n / blocks * pairs, row, token);
+        load(row, token, n % blocks, n % kPairStages);
+      }
+      if (rank == 0)
+        for (int i = max(0, most - kPairStages); i < most; ++i)
+          mbar_wait_suspended(&full[i % kPairStages], (i / kPairStages) & 1, kDrainNs);
+    }
+    for (int i = pair; i < tiles; i += pairs) {
+      int row, token;
+      pair_tile(plan, i, row, token);
+      const int n0 = row * kChannels + static_cast<int>(rank) * (kChannels / 2), t0 = token * plan.tile_tokens;
+      const int channels = min(kChannels / 2, a.channels - n0), tokens = min(plan.tile_tokens, a.tokens - t0);
+      for (int e = threadIdx.x; e < channels * tokens; e += kPairThreads)
+        static_cast<O*>(a.y)[(t0 + e / channels) * a.ldy + n0 + e % channels] = static_cast<O>(NAN);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
@@ -654,6 +686,7 @@ int run_int8_linear(Int8Args a, bool gated, cudaStream_t stream) {
   int device = 0;
   if (!cuda_ok(cudaGetDevice(&device))) return QCC_ERR_CUDA;
   clear_stale_error();
+  a.wait_ns = wait_limit_ns();
   return gated ? launch<true>(a, device, stream) : launch<false>(a, device, stream);
 }
 
@@ -664,12 +697,12 @@ extern "C" int qcc_int8_linear(const int8_t* x, int64_t ldx, const float* x_scal
                                const float* w_scale, const void* bias, int bias_dtype, int tokens, int channels,
                                int cols, void* y, int64_t ldy, int y_dtype, cudaStream_t stream) {
   return qcc::run_int8_linear({x, ldx, x_scale, w, ldw, w_scale, bias, bias_dtype, tokens, channels, cols, y, ldy,
-                               y_dtype}, false, stream);
+                               y_dtype, 0}, false, stream);
 }
 
 extern "C" int qcc_int8_gated_linear(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
                                      const float* w_scale, int tokens, int channels, int cols, void* y, int64_t ldy,
                                      int y_dtype, cudaStream_t stream) {
   return qcc::run_int8_linear({x, ldx, x_scale, w, ldw, w_scale, nullptr, QCC_DTYPE_F32, tokens, channels, cols, y,
-                               ldy, y_dtype}, true, stream);
+                               ldy, y_dtype, 0}, true, stream);
 }

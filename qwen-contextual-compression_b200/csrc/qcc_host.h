@@ -45,7 +45,7 @@ void record_cuda_error(cudaError_t err);
 void clear_stale_error();
 bool launch_ok();
 
-// Bound of the block norms' waits (qcc_set_wait_limit).
+// Bound of the block norms' and the int8 products' waits (qcc_set_wait_limit).
 uint64_t wait_limit_ns();
 
 int decode_max_batch(int hidden, int dtype);

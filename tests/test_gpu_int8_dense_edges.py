@@ -1,0 +1,48 @@
+"""The 8-bit integer products where they can go wrong: waits that run out, and every kernel over several tiles."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import conftest  # noqa: F401
+from qcc_b200 import _lib
+from qcc_b200.runtime.int8_dense import int8_gated_linear, int8_linear
+from test_gpu_int8_dense import check_gated, check_linear, operands, product64
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture
+def no_waiting():
+    """Launches made inside give up at once unless their copies are there already."""
+    lib = _lib.library()
+    assert lib.qcc_set_wait_limit(0) == _lib.OK
+    yield
+    lib.qcc_set_wait_limit(2_000_000_000)
+    torch.cuda.synchronize()
+
+
+# The stream kernel alone, with its columns split over a cluster, with 32, 64 and 128 tokens a tile; and CTA pairs with
+# one and with several tiles (more than 74), short and long columns.
+@pytest.mark.parametrize("tokens,rows,cols", [(1, 40000, 700), (3, 256, 9000), (30, 1000, 4000), (60, 500, 100),
+                                              (100, 5120, 17408), (600, 4000, 2000), (1100, 6000, 1500),
+                                              (1100, 6000, 300)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_a_wait_that_runs_out_leaves_nan(tokens, rows, cols, gated, request):
+    call = int8_gated_linear if gated else int8_linear
+    xq, xs, wq, ws = operands(tokens, rows, cols)
+    channels = rows // 2 if gated else rows
+    want = call(xq, xs, wq, ws, out_dtype=FP32)
+    request.getfixturevalue("no_waiting")
+    flat = torch.full((tokens * channels + 64,), 7.0, device="cuda")
+    got = call(xq, xs, wq, ws, out=flat[:tokens * channels].view(tokens, channels))
+    torch.cuda.synchronize()
+    assert bool((flat[tokens * channels:] == 7).all())
+    lost = got.isnan()
+    assert bool(lost.any()) and torch.equal(got[~lost], want[~lost])
+    # With the ordinary bound again nothing of the launch that gave up arrives later.
+    _lib.library().qcc_set_wait_limit(2_000_000_000)
+    for _ in range(3):
+        assert torch.equal(call(xq, xs, wq, ws, out_dtype=FP32), want)
