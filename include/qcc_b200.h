@@ -587,7 +587,7 @@ QCC_API int qcc_set_wait_limit(uint64_t limit_ns);
  * elements) in dtype; out in out_dtype (bf16, fp16, fp32, or QCC_DTYPE_I8 with
  * row_scale [rows]).  norm (host memory) NULL is the identity: with
  * QCC_DTYPE_I8 it quantises rows as they are.  out may be x itself (same type
- * and stride).  hidden <= 32768.  Rows whose addresses are all multiples of 16
+ * and stride).  hidden <= 32768 (131071 for rows quantised as they are).  Rows whose addresses are all multiples of 16
  * bytes take wide loads. */
 QCC_API int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, int hidden, const qcc_norm_params* norm,
                           void* out, int64_t ld_out, int out_dtype, float* row_scale, cudaStream_t stream);

@@ -25,7 +25,8 @@
 //                 copies that runs ahead of the arithmetic;
 //   plain_kernel  single elements, read again in each pass: rows of tensors
 //                 that do not share their granules (mixed alignments), mixes of
-//                 three element types, and rows beyond the ring's.
+//                 three element types, and rows beyond the ring's (up to
+//                 131071 values for rows that are quantised as they are).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -38,6 +39,7 @@ namespace qcc {
 namespace {
 
 constexpr int kMaxHidden = 32768;
+constexpr int kMaxQuantized = 131071;  // rows as they are to int8: the widest that the int8 products take
 constexpr uint64_t kDrainNs = 2000000000ull;  // for copies in flight after a wait that ran out
 // A row whose largest magnitude is below this is stored as zeros: its scale
 // (and 127 / amax) would leave the normal fp32 range.
@@ -1050,7 +1052,8 @@ extern "C" int qcc_norm_rows(const void* x, int64_t ldx, int dtype, int rows, in
   if (!qcc::valid_dtype(dtype) || !(qcc::valid_dtype(out_dtype) || out_dtype == QCC_DTYPE_I8)) return QCC_ERR_DTYPE;
   if (!qcc::valid_norm(norm)) return QCC_ERR_INVALID_ARGUMENT;
   if (rows < 0 || hidden < 1 || ldx < hidden || ld_out < hidden) return QCC_ERR_SHAPE;
-  if (hidden > qcc::kMaxHidden) return QCC_ERR_UNSUPPORTED;
+  const bool as_is = out_dtype == QCC_DTYPE_I8 && (norm == nullptr || norm->kind == QCC_NORM_NONE);
+  if (hidden > (as_is ? qcc::kMaxQuantized : qcc::kMaxHidden)) return QCC_ERR_UNSUPPORTED;
   if (rows == 0) return QCC_OK;
   if (x == nullptr || out == nullptr || (out_dtype == QCC_DTYPE_I8 && row_scale == nullptr))
     return QCC_ERR_INVALID_ARGUMENT;

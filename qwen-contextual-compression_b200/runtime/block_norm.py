@@ -24,14 +24,15 @@ _raw_stream, _current_device = _lib.raw_stream, _lib.current_device
 KINDS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 GATES = {None: _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
 MAX_HIDDEN = 32768
+MAX_QUANTIZED = 131071  # columns of rows that are quantised as they are: as many as the int8 products take
 MAX_ROWS = 2 ** 31 - 1
 
 
-def _check_hidden(x: torch.Tensor, what: str) -> None:
+def _check_hidden(x: torch.Tensor, what: str, most: int = MAX_HIDDEN) -> None:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} must be [..., hidden] with hidden >= 1, got {tuple(x.shape)}")
-    if x.shape[-1] > MAX_HIDDEN:
-        raise ValueError(f"{what} has {x.shape[-1]} values a row: at most {MAX_HIDDEN}")
+    if x.shape[-1] > most:
+        raise ValueError(f"{what} has {x.shape[-1]} values a row: at most {most}")
 
 
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -166,7 +167,7 @@ def _run_norm(x, norm, out, out_dtype, quantize):
     shape = x.shape
     hidden = shape[-1] if shape else 0
     if not 0 < hidden <= MAX_HIDDEN:
-        _check_hidden(x, "x")
+        _check_hidden(x, "x", MAX_HIDDEN if norm is not None else MAX_QUANTIZED)
     code = _lib.dtype_code(x.dtype)
     if x.requires_grad:
         _lib.refuse_grad("BlockNorm", x)
@@ -211,7 +212,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     amax < 2^-119 gets scale 0 and zeros; one that holds a NaN or an infinity
     gets scale NaN and zeros, so every product with it is NaN.  The int8 rows
     start on multiples of 16 bytes, as ``runtime.int8_dense`` wants them.  At
-    most 32768 columns.
+    most 131071 columns (rows beyond 32768 read their values twice).
     """
     return _run_norm(x, None, None, None, True)
 

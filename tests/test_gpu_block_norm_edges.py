@@ -97,6 +97,21 @@ def test_int8_of_an_rms_norm_of_tiny_and_huge_rows(eps):
     assert bool((q[5] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows,cols", [(3, 32769), (5, 36864), (2, 53248), (1, 131071)])
+def test_quantize_rows_as_wide_as_the_products(rows, cols, dtype):
+    x = make((rows, cols), dtype, 4, 3.0)
+    q, s = quantize_rows(x)
+    amax = x.double().abs().amax(1, keepdim=True)
+    want = torch.round(127 * x.double() / amax)  # exact but for borders, which are borders in float64 as well
+    assert q.stride(0) % 16 == 0 and torch.equal(q.double(), want)
+    assert torch.equal(s.cpu(), (amax[:, 0].cpu() / 127).float())
+    with pytest.raises(ValueError, match="131071"):
+        quantize_rows(torch.zeros((1, 131072), dtype=dtype, device="cuda"))
+    with pytest.raises(ValueError, match="32768"):
+        BlockNorm()(x, quantize=True)
+
+
 @pytest.fixture
 def no_waiting():
     """Launches made inside give up at once unless their copies are there already."""

@@ -6,7 +6,7 @@ import torch
 
 import conftest  # noqa: F401
 from qcc_b200 import _lib
-from qcc_b200.runtime.int8_dense import int8_gated_linear, int8_linear
+from qcc_b200.runtime.int8_dense import Int8GatedFFN, int8_gated_linear, int8_linear, quantize_rows
 from test_gpu_int8_dense import check_gated, check_linear, operands, product64
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +46,23 @@ def test_a_wait_that_runs_out_leaves_nan(tokens, rows, cols, gated, request):
     _lib.library().qcc_set_wait_limit(2_000_000_000)
     for _ in range(3):
         assert torch.equal(call(xq, xs, wq, ws, out_dtype=FP32), want)
+
+
+def test_layer_of_more_than_32768_neurons():
+    hidden, inner, tokens = 64, 36864, 5
+    gen = torch.Generator().manual_seed(0)
+
+    def make(*shape, scale):
+        return (torch.randn(shape, generator=gen) * scale).to(BF16).cuda()
+
+    gate, up, down = make(inner, hidden, scale=0.1), make(inner, hidden, scale=0.1), make(hidden, inner, scale=0.01)
+    x = make(tokens, hidden, scale=1.0)
+    for ffn in (Int8GatedFFN.from_weights(gate, up, down),
+                Int8GatedFFN.from_weights(gate, up, down.t().contiguous(), transposed_down=True)):
+        stored = ffn.gate_up(x, out_dtype=BF16)
+        hq, hs = quantize_rows(stored)
+        check_linear(ffn(x), product64(hq, hs, ffn.down.weight, ffn.down.scale))
+        dense = (torch.nn.functional.silu(x.double() @ gate.double().t()) * (x.double() @ up.double().t())) \
+            @ down.double().t()
+        # Each of the four roundings to int8 is half a step, 1/254 of a row's largest value, at most.
+        assert float((ffn(x).double() - dense).norm() / dense.norm()) < 0.05
