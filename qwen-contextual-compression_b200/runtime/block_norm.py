@@ -80,7 +80,7 @@ class BlockNorm:
     for models that store the weight's difference from one.
     """
 
-    __slots__ = ("weight", "bias", "hidden", "_index", "_dtype", "_params", "_ref", "_weight_ptr",
+    __slots__ = ("weight", "bias", "_hidden", "_index", "_dtype", "_params", "_ref", "_weight_ptr",
                  "_bias_ptr")
 
     def __init__(self, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, kind: str = "rms",
@@ -89,8 +89,6 @@ class BlockNorm:
             raise ValueError(f"kind must be one of {tuple(KINDS)}")
         if not 0 <= eps < float("inf"):
             raise ValueError("eps must be finite and not negative")
-        if weight is None and weight_offset != 0.0:
-            raise ValueError("weight_offset needs a weight")
         self.weight, self.bias = weight, bias
         self._params = _lib.NormParams(None, None, _lib.DTYPE_F32, KINDS[kind], weight_offset, eps)
         self._ref = ctypes.byref(self._params)
@@ -98,6 +96,8 @@ class BlockNorm:
 
     def _bind(self) -> None:
         """Checks weight and bias as they are now and writes them into the C argument."""
+        if self.weight is None and self._params.weight_offset != 0.0:
+            raise ValueError("weight_offset needs a weight")
         hidden, index, dtype, code = None, None, None, _lib.DTYPE_F32
         for p in (self.weight, self.bias):
             if p is None:
@@ -111,10 +111,15 @@ class BlockNorm:
             if index not in (None, p.get_device()):
                 raise RuntimeError("all tensors must share a device")
             hidden, index, dtype, code = p.shape[0], p.get_device(), p.dtype, _lib.dtype_code(p.dtype)
-        self.hidden, self._index, self._dtype = hidden, index, dtype
+        self._hidden, self._index, self._dtype = hidden, index, dtype
         self._weight_ptr, self._bias_ptr = _lib.ptr(self.weight), _lib.ptr(self.bias)
         self._params.weight, self._params.bias = self._weight_ptr, self._bias_ptr
         self._params.dtype = code
+
+    @property
+    def hidden(self) -> int | None:
+        """The length of the weight and the bias; None without either."""
+        return next((p.shape[0] for p in (self.weight, self.bias) if p is not None), None)
 
     @property
     def kind(self) -> str:
@@ -130,24 +135,30 @@ class BlockNorm:
 
     def _for(self, hidden: int, index: int):
         """The norm as a C argument for rows of `hidden` values on a device, after its checks against them."""
-        # A module may have replaced its parameters' data (``p.data = ...``, ``module.to(...)``); an address has one
-        # device.
+        # A module may have replaced its parameters' data (``p.data = ...``, ``module.to(...)``), a user the parameters
+        # themselves; an address has one device.
         weight, bias = self.weight, self.bias
-        if weight is not None:
+        if weight is None:
+            if self._weight_ptr is not None:
+                self._bind()
+        else:
             if weight.requires_grad:
                 _lib.refuse_grad("BlockNorm", weight)
             if (weight.data_ptr() != self._weight_ptr or weight.dtype is not self._dtype
-                    or weight.numel() != self.hidden or not weight.is_contiguous()):
+                    or weight.numel() != self._hidden or not weight.is_contiguous()):
                 self._bind()
-        if bias is not None:
+        if bias is None:
+            if self._bias_ptr is not None:
+                self._bind()
+        else:
             if bias.requires_grad:
                 _lib.refuse_grad("BlockNorm", bias)
             if (bias.data_ptr() != self._bias_ptr or bias.dtype is not self._dtype
-                    or bias.numel() != self.hidden or not bias.is_contiguous()):
+                    or bias.numel() != self._hidden or not bias.is_contiguous()):
                 self._bind()
-        if self.hidden is not None:
-            if self.hidden != hidden:
-                raise ValueError(f"the norm has {self.hidden} weights, its input {hidden} values a row")
+        if self._hidden is not None:
+            if self._hidden != hidden:
+                raise ValueError(f"the norm has {self._hidden} weights, its input {hidden} values a row")
             if self._index != index:
                 raise RuntimeError("all tensors must share a device")
         return self._ref

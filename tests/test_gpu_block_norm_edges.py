@@ -112,6 +112,25 @@ def test_quantize_rows_as_wide_as_the_products(rows, cols, dtype):
         BlockNorm()(x, quantize=True)
 
 
+def test_parameters_taken_away():
+    """A norm whose weight or bias becomes None no longer reads the tensor that it had."""
+    x = make((5, 512), FP32, 1)
+    weight, bias = make(512, FP32, 2), make(512, FP32, 3)
+    norm = BlockNorm(weight, bias, kind="layer")
+    norm(x)
+    norm.weight = None
+    assert torch.equal(norm(x), BlockNorm(None, bias, kind="layer")(x))
+    norm.bias = None
+    assert norm.hidden is None and torch.equal(norm(x), BlockNorm(kind="layer")(x))
+    assert torch.equal(norm(x[:, :100]), BlockNorm(kind="layer")(x[:, :100]))
+    norm.weight, norm.bias = weight, bias
+    assert norm.hidden == 512 and torch.equal(norm(x), BlockNorm(weight, bias, kind="layer")(x))
+    shifted = BlockNorm(weight, weight_offset=1.0)
+    shifted.weight = None
+    with pytest.raises(ValueError, match="weight_offset"):
+        shifted(x)
+
+
 @pytest.fixture
 def no_waiting():
     """Launches made inside give up at once unless their copies are there already."""
