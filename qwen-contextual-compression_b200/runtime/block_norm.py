@@ -80,8 +80,7 @@ class BlockNorm:
     for models that store the weight's difference from one.
     """
 
-    __slots__ = ("weight", "bias", "_hidden", "_index", "_dtype", "_params", "_ref", "_weight_ptr",
-                 "_bias_ptr")
+    __slots__ = ("weight", "bias", "_constants", "_bound")
 
     def __init__(self, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, kind: str = "rms",
                  eps: float = 1e-6, weight_offset: float = 0.0):
@@ -90,16 +89,17 @@ class BlockNorm:
         if not 0 <= eps < float("inf"):
             raise ValueError("eps must be finite and not negative")
         self.weight, self.bias = weight, bias
-        self._params = _lib.NormParams(None, None, _lib.DTYPE_F32, KINDS[kind], weight_offset, eps)
-        self._ref = ctypes.byref(self._params)
+        self._constants = KINDS[kind], weight_offset, eps
         self._bind()
 
-    def _bind(self) -> None:
-        """Checks weight and bias as they are now and writes them into the C argument."""
-        if self.weight is None and self._params.weight_offset != 0.0:
+    def _bind(self) -> tuple:
+        """Checks weight and bias as they are now and makes the C argument of them.  It is replaced, never rewritten:
+        another thread may be launching with the one before."""
+        weight, bias = self.weight, self.bias
+        if weight is None and self._constants[1] != 0.0:
             raise ValueError("weight_offset needs a weight")
         hidden, index, dtype, code = None, None, None, _lib.DTYPE_F32
-        for p in (self.weight, self.bias):
+        for p in (weight, bias):
             if p is None:
                 continue
             if p.get_device() < 0:
@@ -111,10 +111,10 @@ class BlockNorm:
             if index not in (None, p.get_device()):
                 raise RuntimeError("all tensors must share a device")
             hidden, index, dtype, code = p.shape[0], p.get_device(), p.dtype, _lib.dtype_code(p.dtype)
-        self._hidden, self._index, self._dtype = hidden, index, dtype
-        self._weight_ptr, self._bias_ptr = _lib.ptr(self.weight), _lib.ptr(self.bias)
-        self._params.weight, self._params.bias = self._weight_ptr, self._bias_ptr
-        self._params.dtype = code
+        weight_ptr, bias_ptr = _lib.ptr(weight), _lib.ptr(bias)
+        params = _lib.NormParams(weight_ptr, bias_ptr, code, *self._constants)
+        self._bound = bound = weight_ptr, bias_ptr, dtype, hidden, index, ctypes.byref(params)
+        return bound
 
     @property
     def hidden(self) -> int | None:
@@ -123,45 +123,44 @@ class BlockNorm:
 
     @property
     def kind(self) -> str:
-        return next(name for name, code in KINDS.items() if code == self._params.kind)
+        return next(name for name, code in KINDS.items() if code == self._constants[0])
 
     @property
     def eps(self) -> float:
-        return self._params.eps
+        return self._bound[5]._obj.eps
 
     @property
     def weight_offset(self) -> float:
-        return self._params.weight_offset
+        return self._bound[5]._obj.weight_offset
 
     def _for(self, hidden: int, index: int):
         """The norm as a C argument for rows of `hidden` values on a device, after its checks against them."""
         # A module may have replaced its parameters' data (``p.data = ...``, ``module.to(...)``), a user the parameters
         # themselves; an address has one device.
+        weight_ptr, bias_ptr, dtype, length, device, ref = self._bound
         weight, bias = self.weight, self.bias
         if weight is None:
-            if self._weight_ptr is not None:
-                self._bind()
+            same = weight_ptr is None
         else:
             if weight.requires_grad:
                 _lib.refuse_grad("BlockNorm", weight)
-            if (weight.data_ptr() != self._weight_ptr or weight.dtype is not self._dtype
-                    or weight.numel() != self._hidden or not weight.is_contiguous()):
-                self._bind()
+            same = (weight.data_ptr() == weight_ptr and weight.dtype is dtype and weight.numel() == length
+                    and weight.is_contiguous())
         if bias is None:
-            if self._bias_ptr is not None:
-                self._bind()
+            same = same and bias_ptr is None
         else:
             if bias.requires_grad:
                 _lib.refuse_grad("BlockNorm", bias)
-            if (bias.data_ptr() != self._bias_ptr or bias.dtype is not self._dtype
-                    or bias.numel() != self._hidden or not bias.is_contiguous()):
-                self._bind()
-        if self._hidden is not None:
-            if self._hidden != hidden:
-                raise ValueError(f"the norm has {self._hidden} weights, its input {hidden} values a row")
-            if self._index != index:
+            same = (same and bias.data_ptr() == bias_ptr and bias.dtype is dtype and bias.numel() == length
+                    and bias.is_contiguous())
+        if not same:
+            _, _, _, length, device, ref = self._bind()
+        if length is not None:
+            if length != hidden:
+                raise ValueError(f"the norm has {length} weights, its input {hidden} values a row")
+            if device != index:
                 raise RuntimeError("all tensors must share a device")
-        return self._ref
+        return ref
 
     def __call__(self, x: torch.Tensor, *, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
                  quantize: bool = False):

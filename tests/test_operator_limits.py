@@ -3,8 +3,11 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 import conftest  # noqa: F401
 from qcc_b200 import _lib
+from qcc_b200.runtime.block_norm import BlockNorm
 
 
 def test_wait_limit_is_a_minute_at_most():
@@ -28,3 +31,37 @@ def test_widest_rows():
         assert call(32769, identity, _lib.DTYPE_BF16) == _lib.ERR_UNSUPPORTED
     assert call(32768, rms, _lib.DTYPE_I8) == _lib.OK
     assert call(32769, rms, _lib.DTYPE_I8) == _lib.ERR_UNSUPPORTED
+
+
+class Parameter:
+    """What BlockNorm asks of a CUDA tensor."""
+    requires_grad, dtype = False, torch.float32
+
+    def __init__(self, address, length):
+        self.address, self.shape = address, (length,)
+
+    def get_device(self):
+        return 0
+
+    def dim(self):
+        return 1
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return self.address
+
+    def numel(self):
+        return self.shape[0]
+
+
+def test_a_norm_that_is_launching_keeps_its_argument():
+    """Two threads share a norm: the one that finds its weight replaced leaves the other's C argument as it was."""
+    norm = BlockNorm(Parameter(256, 64), eps=1e-5, kind="rms", weight_offset=1.0)
+    launching = norm._for(64, 0)
+    norm.weight = Parameter(512, 32)
+    replaced = norm._for(32, 0)
+    assert launching._obj.weight == 256 and replaced._obj.weight == 512
+    assert norm._for(32, 0) is replaced
+    assert abs(norm.eps - 1e-5) < 1e-12 and norm.weight_offset == 1.0 and norm.kind == "rms" and norm.hidden == 32
