@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _PACKAGE_DIR = Path(__file__).resolve().parent
 _LIBRARY_PATH = _PACKAGE_DIR / "libqcc_b200.so"
@@ -188,10 +189,15 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
-    """Raise where autograd would expect a gradient: these entry points have no backward."""
+    """Raise where autograd would expect a gradient or a tangent: these entry points have no derivatives.  Callers ask
+    for this check where a tensor has ``requires_grad`` or a level of forward-mode differentiation is open."""
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} has no backward: call it under torch.no_grad() or detach its inputs")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: unpack its dual inputs")
 
 
 try:  # the raw queries avoid building a torch.cuda.Stream and the lazy-initialisation check per call

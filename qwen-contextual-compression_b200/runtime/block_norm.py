@@ -20,7 +20,7 @@ import torch
 
 from .. import _lib
 
-_raw_stream, _current_device = _lib.raw_stream, _lib.current_device
+_raw_stream, _current_device, _forward_ad = _lib.raw_stream, _lib.current_device, _lib.forward_ad
 KINDS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 GATES = {None: _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
 MAX_HIDDEN = 32768
@@ -142,14 +142,14 @@ class BlockNorm:
         if weight is None:
             same = weight_ptr is None
         else:
-            if weight.requires_grad:
+            if weight.requires_grad or _forward_ad._current_level >= 0:
                 _lib.refuse_grad("BlockNorm", weight)
             same = (weight.data_ptr() == weight_ptr and weight.dtype is dtype and weight.numel() == length
                     and weight.is_contiguous())
         if bias is None:
             same = same and bias_ptr is None
         else:
-            if bias.requires_grad:
+            if bias.requires_grad or _forward_ad._current_level >= 0:
                 _lib.refuse_grad("BlockNorm", bias)
             same = (same and bias.data_ptr() == bias_ptr and bias.dtype is dtype and bias.numel() == length
                     and bias.is_contiguous())
@@ -179,8 +179,8 @@ def _run_norm(x, norm, out, out_dtype, quantize):
     if not 0 < hidden <= MAX_HIDDEN:
         _check_hidden(x, "x", MAX_HIDDEN if norm is not None else MAX_QUANTIZED)
     code = _lib.dtype_code(x.dtype)
-    if x.requires_grad:
-        _lib.refuse_grad("BlockNorm", x)
+    if x.requires_grad or _forward_ad._current_level >= 0:
+        _lib.refuse_grad("quantize_rows" if norm is None else "BlockNorm", x)
     norm_ref = None if norm is None else norm._for(hidden, index)
     rows, ld = _rows(x)
     t = x.numel() // hidden
@@ -285,7 +285,8 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
         raise ValueError(f"gate_activation must be one of {tuple(GATES)}")
     if next_norm is None and (quantize or out is not None or out_dtype is not None):
         raise ValueError("quantize, out and out_dtype need a next_norm")
-    if branch.requires_grad or residual.requires_grad or (gate is not None and gate.requires_grad):
+    if (branch.requires_grad or residual.requires_grad or (gate is not None and gate.requires_grad)
+            or _forward_ad._current_level >= 0):
         _lib.refuse_grad("residual_norm", branch, residual, gate)
     post_ref = None if post is None else post._for(hidden, index)
     next_ref = None if next_norm is None else next_norm._for(hidden, index)

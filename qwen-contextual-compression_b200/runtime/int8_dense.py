@@ -23,7 +23,7 @@ from .. import _lib
 from .block_norm import int8_rows, quantize_rows
 from .packing import PackedFFNWeights, validate_weight_shapes
 
-_raw_stream, _current_device = _lib.raw_stream, _lib.current_device
+_raw_stream, _current_device, _forward_ad = _lib.raw_stream, _lib.current_device, _lib.forward_ad
 MAX_COLS = 131071       # |q| <= 128: the int32 sums cannot overflow
 MAX_TOKENS = 1 << 20
 MAX_CHANNELS = 1 << 19
@@ -65,7 +65,8 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
         raise ValueError("w must have rows and columns")
     if cols > MAX_COLS or tokens > MAX_TOKENS or channels > MAX_CHANNELS:
         raise ValueError(f"at most {MAX_TOKENS} tokens, {MAX_CHANNELS} channels and {MAX_COLS} columns")
-    if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
+    if (x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad)
+            or _forward_ad._current_level >= 0):
         _lib.refuse_grad("the int8 product", x_scale, w_scale, bias)
     if out is None:
         if out_dtype is None:

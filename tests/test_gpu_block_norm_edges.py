@@ -3,10 +3,12 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import conftest  # noqa: F401
 from qcc_b200 import _lib
 from qcc_b200.runtime.block_norm import BlockNorm, quantize_rows, residual_norm
+from qcc_b200.runtime.int8_dense import int8_gated_linear, int8_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -129,6 +131,35 @@ def test_parameters_taken_away():
     shifted.weight = None
     with pytest.raises(ValueError, match="weight_offset"):
         shifted(x)
+
+
+def test_tangents_are_refused():
+    """A dual tensor's tangent would be dropped: the call is refused, and calls without one inside the level are not."""
+    x, weight, gate = make((4, 64), FP32, 1), make(64, FP32, 2), make((4, 1), FP32, 3)
+    norm = BlockNorm(weight)
+    wq, ws = quantize_rows(make((8, 64), FP32, 4))
+    xq, xs = quantize_rows(x)
+    bias = make(8, FP32, 5)
+    want = norm(x)
+    with forward_ad.dual_level():
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, weight, gate, xs, ws, bias)]
+        dual_x, dual_weight, dual_gate, dual_xs, dual_ws, dual_bias = dual
+        for call in (lambda: norm(dual_x), lambda: norm(dual_x, quantize=True), lambda: quantize_rows(dual_x),
+                     lambda: BlockNorm(dual_weight)(x), lambda: BlockNorm(weight, dual_weight)(x),
+                     lambda: residual_norm(dual_x, x), lambda: residual_norm(x, dual_x),
+                     lambda: residual_norm(x, x, gate=dual_gate), lambda: residual_norm(x, x, post=BlockNorm(dual_weight)),
+                     lambda: int8_linear(xq, dual_xs, wq, ws), lambda: int8_linear(xq, xs, wq, dual_ws),
+                     lambda: int8_linear(xq, xs, wq, ws, bias=dual_bias),
+                     lambda: int8_gated_linear(xq, dual_xs, wq, ws)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(norm(x), want)
+        assert torch.equal(norm(forward_ad.unpack_dual(dual_x).primal), want)
+    grad = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="quantize_rows has no backward"):
+        quantize_rows(grad)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(norm, (x,), (x,))
 
 
 @pytest.fixture
