@@ -23,7 +23,8 @@ class FFNBlock:
 
     ffn: a callable y = ffn(x, *args, **kwargs) -- ``IndexedSparseFFN`` (args:
     the selected ids), ``BlockSparsePrefill`` (the tiles' blocks),
-    ``Int8GatedFFN`` (none), ...  An ``Int8GatedFFN`` gets pre's int8 rows.
+    ``Int8GatedFFN`` (none), ...  An ``Int8GatedFFN`` gets pre's int8 rows.  Of
+    a tuple (``OracleModeFFN``: y and its ids) the first item is y.
     dtype: the type of x (and of y) when it is not the residual's, e.g. bf16
     records under an fp32 residual.  ``quantize_next``: next_norm(r) as int8
     rows, for a next block that takes them.
@@ -51,6 +52,8 @@ class FFNBlock:
         if int8:
             kwargs.setdefault("out_dtype", dtype)
         y = self.ffn(x, *args, **kwargs)
+        if isinstance(y, tuple):
+            y = y[0]
         return residual_norm(y, residual, post=self.post, gate=gate, gate_activation=self.gate_activation,
                              residual_scale=self.residual_scale, branch_scale=self.branch_scale,
                              next_norm=self.next_norm, quantize=self.quantize_next)
