@@ -15,7 +15,15 @@ from __future__ import annotations
 import torch
 
 from .block_norm import BlockNorm, residual_norm
+from .engine import IndexedSparseFFN
+from .ffn import TorchDynamicSparseFFN
 from .int8_dense import Int8GatedFFN
+from .oracle_mode import OracleModeFFN
+from .prefill import BlockSparsePrefill
+from .sharded import ShardedIndexedFFN
+
+# FFNs that take rows [T, hidden] only; other callables get x with the residual's leading axes.
+_OF_ROWS = IndexedSparseFFN, TorchDynamicSparseFFN, OracleModeFFN, BlockSparsePrefill, ShardedIndexedFFN
 
 
 class FFNBlock:
@@ -40,10 +48,11 @@ class FFNBlock:
         self.residual_scale, self.branch_scale, self.dtype = float(residual_scale), float(branch_scale), dtype
 
     def __call__(self, residual: torch.Tensor, *args, x=None, gate: torch.Tensor | None = None, **kwargs):
-        """r, or (r, next input) with a next_norm, for residual [T, hidden].
+        """r, or (r, next input) with a next_norm, for residual [..., hidden] (int8 next inputs are rows [T, hidden]).
 
         x: pre(residual) when the previous block made it (its next_norm's
-        output; int8 rows for an ``Int8GatedFFN``); args and kwargs go to ffn.
+        output; int8 rows for an ``Int8GatedFFN``); args and kwargs go to ffn,
+        whose tokens are the residual's rows in order.
         """
         dtype = self.dtype or residual.dtype
         int8 = isinstance(self.ffn, Int8GatedFFN)
@@ -51,9 +60,13 @@ class FFNBlock:
             x = self.pre(residual, quantize=True) if int8 else self.pre(residual, out_dtype=dtype)
         if int8:
             kwargs.setdefault("out_dtype", dtype)
+        elif isinstance(self.ffn, _OF_ROWS) and x.dim() != 2:
+            x = x.reshape(-1, x.shape[-1])
         y = self.ffn(x, *args, **kwargs)
         if isinstance(y, tuple):
             y = y[0]
+        if int8 or isinstance(self.ffn, _OF_ROWS):
+            y = y.reshape(residual.shape)
         return residual_norm(y, residual, post=self.post, gate=gate, gate_activation=self.gate_activation,
                              residual_scale=self.residual_scale, branch_scale=self.branch_scale,
                              next_norm=self.next_norm, quantize=self.quantize_next)
