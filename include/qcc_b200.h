@@ -619,8 +619,9 @@ QCC_API int qcc_residual_norm(const void* branch, int64_t ld_branch, int dtype, 
  * float type (runtime/ffn.py:11-17).
  * ------------------------------------------------------------------------- */
 
-/* y[t, n] = (sum_k x[t, k] w[n, k]) * (x_scale[t] * w_scale[n]) + bias[n];
- * bias (NULL: none) is [channels] in bias_dtype; w has `channels` rows. */
+/* y[t, n] = (sum_k x[t, k] w[n, k]) * (x_scale[t] * w_scale[n]) + bias[n],
+ * also where the scales' product alone would leave fp32's normal range; bias
+ * (NULL: none) is [channels] in bias_dtype; w has `channels` rows. */
 QCC_API int qcc_int8_linear(const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw,
                             const float* w_scale, const void* bias, int bias_dtype, int tokens, int channels,
                             int cols, void* y, int64_t ldy, int y_dtype, cudaStream_t stream);

@@ -1,7 +1,7 @@
 // Products of 8-bit integer matrices with a scale per token and per channel.
 //
 //   acc[t, n] = sum_k xq[t, k] * wq[n, k]                 (int32, exact)
-//   y[t, n]   = fp32(acc) * (xs[t] * ws[n]) + bias[n]     rounded once
+//   y[t, n]   = fp32(acc) * (xs[t] * ws[n]) + bias[n]     rounded once (scales at the ends of fp32: see scaled())
 // and, for the gated form (wq holds the gate rows 0..N-1, then the up rows),
 //   y[t, n]   = silu(g) * u  with g, u the two products of channel n.
 #include <cuda.h>
@@ -41,6 +41,22 @@ struct Int8Args {
 // Below g = -87.3 the quotient, under 2^-119, becomes 0.
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
+// Scales whose product is a normal number whatever the other one is: fp32(sum) * (xs * ws) then rounds three times.
+__device__ __forceinline__ bool ordinary_scale(float s) {
+  return s == 0.f || (fabsf(s) >= 0x1p-62f && fabsf(s) <= 0x1p62f);
+}
+
+// sum * xs * ws for other scales, whose product can leave the normal range though the result does not: it would lose
+// places or become 0 (rows of values near 2^-119), or infinity, and NaN for a sum of 0.  The smaller scale first then:
+// it shrinks the sum, or xs * ws and with it the result are beyond the range anyway.
+__device__ __forceinline__ float scaled(int sum, float xs, float ws) {
+  const float v = static_cast<float>(sum);
+  const float product = xs * ws;
+  if (fabsf(product) >= 0x1p-126f && fabsf(product) <= 0x1.fffffep127f) return v * product;
+  const bool x_first = fabsf(xs) < fabsf(ws);
+  return v * (x_first ? xs : ws) * (x_first ? ws : xs);
+}
+
 __device__ __forceinline__ float bias_value(const void* bias, int dtype, int n) {
   if (bias == nullptr) return 0.f;
   if (dtype == QCC_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[n]);
@@ -75,6 +91,7 @@ struct RowOutput {
   int64_t ldy;
   float ws, ws_up, bias;
   bool in;  // the channel exists
+  bool ordinary;  // its scales are ordinary ones
 
   // row0: the first weight row (gated: channel) of the 32-lane group.  A tile whose wait ran out is `broken`: its
   // scales become NaN, and so do its outputs.
@@ -86,11 +103,35 @@ struct RowOutput {
     ws = broken ? NAN : in ? a.ws[n] : 0.f;
     ws_up = GATED && in ? a.ws[a.channels + n] : 0.f;
     bias = !GATED && in ? bias_value(a.bias, a.bias_dtype, n) : 0.f;
+    ordinary = ordinary_scale(ws) && ordinary_scale(ws_up);
+  }
+
+  // The same as finish for scales that are not ordinary, in few instructions rather than in short time.
+  template <int J>
+  __device__ __forceinline__ void finish_extreme(const int (&acc)[J], int c, int tokens, float xs, int lane) const {
+#pragma unroll 1
+    for (int k = 0; k < J && c + k < tokens; ++k) {
+      int sum = 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) sum = j == k ? acc[j] : sum;
+      const float scale = __shfl_sync(0xffffffffu, xs, k);
+      O* to = y + static_cast<int64_t>(c + k) * ldy;
+      if (GATED) {  // lanes 0-15 hold the gate's sums, lanes 16-31 the up rows'
+        const int up = __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (lane < 16 && in) *to = static_cast<O>(silu(scaled(sum, scale, ws)) * scaled(up, scale, ws_up));
+      } else if (in) {
+        *to = static_cast<O>(scaled(sum, scale, ws) + bias);
+      }
+    }
   }
 
   // Finishes tokens c .. c + J - 1 (those below `tokens`) from their sums; lane j holds token c + j's scale.
   template <int J>
   __device__ __forceinline__ void finish(const int (&acc)[J], int c, int tokens, float xs, int lane) const {
+    if (!__all_sync(0xffffffffu, ordinary && ordinary_scale(xs))) {
+      finish_extreme(acc, c, tokens, xs, lane);
+      return;
+    }
     O* to = y + static_cast<int64_t>(c) * ldy;
     if (GATED) {
       // Lanes 0-15 finish the even tokens, lanes 16-31 the odd ones.
@@ -250,12 +291,6 @@ __global__ void __launch_bounds__(128)
   if (!mbar_wait_suspended(&done, 0, 4 * max(a.wait_ns, kDrainNs))) failed = 1;
   tc_fence_after_sync();
   __syncthreads();
-  if (failed != 0) {
-    if (threadIdx.x == 0)
-      for (int i = max(0, issued - STAGES); i < issued; ++i)
-        mbar_wait_suspended(&full[i % STAGES], (i / STAGES) & 1, kDrainNs);
-    __syncthreads();
-  }
 
   const int tokens = min(BN, a.tokens - t0);
   const uint32_t from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
@@ -271,7 +306,7 @@ __global__ void __launch_bounds__(128)
     tc_fence_before_sync();
     __syncthreads();
   } else {
-    // The ring is free (every MMA has completed).
+    // The ring is free: every MMA has completed (where a wait ran out copies may still land in it, and all is NaN).
     int* partial = reinterpret_cast<int*>(ring);
 #pragma unroll 1
     for (int c = 0; c < tokens; c += 16) {
@@ -312,6 +347,9 @@ __global__ void __launch_bounds__(128)
     __syncwarp();
     cluster_sync();  // the other CTAs have read this one's sums
   }
+  if (failed != 0 && threadIdx.x == 0)
+    for (int i = max(0, issued - STAGES); i < issued; ++i)
+      mbar_wait_suspended(&full[i % STAGES], (i / STAGES) & 1, kDrainNs);
   if (warp == 1) tmem_dealloc(tmem, S::kTmemCols);
 }
 

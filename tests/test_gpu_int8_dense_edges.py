@@ -66,3 +66,36 @@ def test_layer_of_more_than_32768_neurons():
             @ down.double().t()
         # Each of the four roundings to int8 is half a step, 1/254 of a row's largest value, at most.
         assert float((ffn(x).double() - dense).norm() / dense.norm()) < 0.05
+
+
+@pytest.mark.parametrize("tokens,cols", [(3, 40), (40, 1500), (130, 200)])
+def test_scales_at_the_ends_of_fp32(tokens, cols):
+    """The product of the scales leaves the normal range, the result does not."""
+    rows = 96
+    xq, _, wq, _ = operands(tokens, rows, cols)
+    xq[0, 0], wq[0] = 0, 0  # sums of 0 under scales whose product is infinite
+    exponents = torch.tensor([-126.0, -120.0, -100.0, -75.0, -40.0, 0.0, 40.0, 70.0, 100.0], device="cuda")
+    xs = 1.3 * 2.0 ** exponents[torch.arange(tokens, device="cuda") % 9]
+    ws = 1.7 * 2.0 ** exponents[(torch.arange(rows, device="cuda") * 5 + 2) % 9]
+    xs[1] = 0.0
+    sums = (xq.double() @ wq.double().t())
+    want = sums * xs.double()[:, None] * ws.double()
+    y = int8_linear(xq, xs, wq, ws, out_dtype=FP32)
+    largest, least = torch.finfo(FP32).max, 2.0 ** -126
+    over = want.abs() > largest
+    assert bool((y[over].double() == torch.sign(want[over]) * float("inf")).all())
+    # Three roundings (the sum's, and one a scale), and half a step of the smallest numbers.
+    bound = 3 * 2.0 ** -24 * want.abs() * (1 + 2.0 ** -20) + 2.0 ** -149
+    assert bool(((y.double() - want).abs() <= bound)[~over].all())
+    assert bool((y[:, 0] == 0).all()) and bool((y[1] == 0).all())
+    assert int(((want.abs() >= least) & (xs.double()[:, None] * ws.double() < least)).sum()) > 0
+    # Gate and up rows alike: the gate ordinary, the up rows at the ends.
+    gate_ws = torch.full((rows // 2,), 2.0 ** -14, device="cuda")
+    ws2 = torch.cat([gate_ws, ws[rows // 2:]])
+    xs2 = torch.where(exponents[torch.arange(tokens, device="cuda") % 9] <= -100.0, xs, torch.ones_like(xs))
+    both = sums * xs2.double()[:, None] * ws2.double()
+    g, u = both[:, :rows // 2], both[:, rows // 2:]
+    h = int8_gated_linear(xq, xs2, wq, ws2, out_dtype=FP32)
+    fits = (g * torch.sigmoid(g) * u).abs() <= largest
+    fits &= u.abs() <= largest
+    check_gated(h[fits], g[fits], u[fits])
