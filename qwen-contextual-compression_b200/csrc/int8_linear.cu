@@ -36,10 +36,13 @@ struct Int8Args {
   uint64_t wait_ns;  // bound of the waits for copies and for free slots
 };
 
-// silu with the fast exponential and quotient: exp's argument rounds once (an
-// error of |g| roundings in exp), exp and the quotient are off by 2 ulp each.
-// Below g = -87.3 the quotient, under 2^-119, becomes 0.
-__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+// silu with the fast exponential and quotient, from exp(-|g|), at most 1: exp's argument rounds once (an error of |g|
+// roundings in exp), exp and the quotient are off by 2 ulp each, and the divisor is between 1 and 2 (beyond 2^126, as
+// 1 + exp(-g) is below g = -87.3, the fast quotient is 0).
+__device__ __forceinline__ float silu(float g) {
+  const float e = __expf(-fabsf(g));
+  return __fdividef(g < 0.f ? g * e : g, 1.f + e);
+}
 
 // Scales whose product is a normal number whatever the other one is: fp32(sum) * (xs * ws) then rounds three times.
 __device__ __forceinline__ bool ordinary_scale(float s) {

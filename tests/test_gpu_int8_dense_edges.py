@@ -99,3 +99,24 @@ def test_scales_at_the_ends_of_fp32(tokens, cols):
     fits = (g * torch.sigmoid(g) * u).abs() <= largest
     fits &= u.abs() <= largest
     check_gated(h[fits], g[fits], u[fits])
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_silu_far_below_zero(tokens):
+    """silu keeps its value down to fp32's smallest numbers, and large up projections show it."""
+    channels = 9000  # of pair tiles at 300 tokens
+    xq = torch.zeros((tokens, 16), dtype=torch.int8, device="cuda")
+    xq[:, 0], xq[:, 1] = -127, 127
+    wq = torch.zeros((2 * channels, 16), dtype=torch.int8, device="cuda")
+    wq[:channels, 0], wq[channels:, 1] = 127, 127
+    depth = torch.linspace(70.0, 101.0, channels, device="cuda")
+    ws = torch.cat([depth / 127 ** 2, torch.full((channels,), 1e30 / 127 ** 2, device="cuda")])
+    xs = torch.ones(tokens, device="cuda")
+    both = product64(xq, xs, wq, ws)
+    g, u = both[:, :channels], both[:, channels:]
+    h = int8_gated_linear(xq, xs, wq, ws, out_dtype=FP32)
+    want = g * torch.sigmoid(g) * u
+    # As in the products' tests, with exp's smallest numbers off by 2^-149 at most instead of an error of 2^-119 |u|.
+    bound = want.abs() * (2.0 ** -24 + (16 + 4 * g.abs()) * 2.0 ** -24 * 1.01) + 2.0 ** -148 * g.abs() * u.abs()
+    assert bool(((h.double() - want).abs() <= bound).all())
+    assert bool((h != 0).all())
