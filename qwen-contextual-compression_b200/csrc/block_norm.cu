@@ -452,8 +452,12 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t e) {
 }
 
 __device__ __forceinline__ float gate_value(float g, int act) {
-  // The fast exponential and quotient are off by |g| + 8 roundings at most, and exact at the ends (0 and 1).
-  if (act == QCC_GATE_SIGMOID) return __fdividef(1.f, 1.f + __expf(-g));
+  // The fast exponential and quotient are off by |g| + 8 roundings at most, and exact at the ends (0 and 1).  From
+  // exp(-|g|): beyond 2^126, as 1 + exp(-g) is below g = -87.3, the fast quotient is 0.
+  if (act == QCC_GATE_SIGMOID) {
+    const float e = __expf(-fabsf(g));
+    return __fdividef(g < 0.f ? e : 1.f, 1.f + e);
+  }
   if (act == QCC_GATE_TANH) return tanhf(g);
   return g;
 }

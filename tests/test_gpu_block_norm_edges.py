@@ -162,6 +162,23 @@ def test_tangents_are_refused():
         torch.func.jvp(norm, (x,), (x,))
 
 
+@pytest.mark.parametrize("shape", [(64, 1), (64, 40), (64, 1029)])
+def test_sigmoid_gate_far_from_zero(shape):
+    """The sigmoid keeps its value down to fp32's smallest numbers, and large branches show it."""
+    rows, cols = shape
+    values = torch.cat([torch.linspace(-101.0, -80.0, 48), torch.tensor([-1e4, -float("inf"), float("inf"), 1e4, 0.0]),
+                        torch.linspace(80.0, 101.0, 11)]).cuda()
+    gate = values[:, None].expand(rows, cols).contiguous()
+    hidden = max(cols, 40)
+    branch = torch.full((rows, hidden), 1e30, device="cuda")
+    r = residual_norm(branch, torch.zeros_like(branch), gate=gate, gate_activation="sigmoid")
+    want = torch.sigmoid(gate.double()) * branch.double()
+    # |g| + 8 roundings of the gate and one of the product; exp's smallest numbers are off by 2^-149 at most.
+    bound = want * (values.double().abs().clamp(max=128.0)[:, None] + 10) * U32 + 2.0 ** -149 * branch.double()
+    assert bool(((r.double() - want).abs() <= bound).all())
+    assert bool((r[48] == 0).all()) and bool((r[49] == 0).all()) and bool((r[50] == branch[50]).all())
+
+
 @pytest.fixture
 def no_waiting():
     """Launches made inside give up at once unless their copies are there already."""
