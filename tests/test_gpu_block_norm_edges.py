@@ -9,6 +9,7 @@ import conftest  # noqa: F401
 from qcc_b200 import _lib
 from qcc_b200.runtime.block_norm import BlockNorm, quantize_rows, residual_norm
 from qcc_b200.runtime.int8_dense import int8_gated_linear, int8_linear
+from test_gpu_block_norm import assert_rows_close, norm64
 
 pytestmark = pytest.mark.gpu
 
@@ -177,6 +178,90 @@ def test_sigmoid_gate_far_from_zero(shape):
     bound = want * (values.double().abs().clamp(max=128.0)[:, None] + 10) * U32 + 2.0 ** -149 * branch.double()
     assert bool(((r.double() - want).abs() <= bound).all())
     assert bool((r[48] == 0).all()) and bool((r[49] == 0).all()) and bool((r[50] == branch[50]).all())
+
+
+def close_int8(q, s, want, bound):
+    """int8 rows of computed values: within half a step, and what the fp32 values are off (in their row's amax)."""
+    amax = want.abs().amax(-1, keepdim=True)
+    return bool(((q.double() * s.double()[:, None] - want).abs() <= 0.5 * amax / 127 + bound * U32 * amax).all())
+
+
+# More rows a block than its ring holds, twice over: at 5120 values (16 bits) 592 to 1184 blocks of two or three rows.
+@pytest.mark.parametrize("rows,hidden,dtype", [(6000, 5120, BF16), (6001, 4001, FP16), (4000, 5120, FP32),
+                                               (3001, 2051, FP32), (2000, 12288, BF16), (1500, 20000, BF16)])
+def test_rings_that_come_round(rows, hidden, dtype):
+    x, residual = make((rows, hidden), dtype, 1, 2.0, 0.5), make((rows, hidden), dtype, 2)
+    rms = BlockNorm(make(hidden, dtype, 3, 0.2, 1.0))
+    layer = BlockNorm(make(hidden, dtype, 3, 0.2, 1.0), make(hidden, dtype, 4, 0.2), kind="layer")
+    for norm in (rms, layer):
+        want = norm64(x.double(), norm)
+        extra = None if norm.bias is None else norm.bias.expand(rows, hidden)
+        assert_rows_close(norm(x), want, extra)
+        assert close_int8(*norm(x, quantize=True), want, 520 + 127 * 4)
+    q, s = quantize_rows(x)
+    amax = x.double().abs().amax(1, keepdim=True)
+    assert torch.equal(q.double(), torch.round(127 * x.double() / amax))
+    assert torch.equal(s, (amax[:, 0] / 127).float())
+    b = norm64(x.double(), layer)
+    want = residual.double() + 0.5 * b
+    scale = torch.maximum(b.abs(), residual.double().abs())
+    want_x = norm64(want, rms)
+    # Into tensors of their own, then in place over the branch and the residual: the copies that run ahead read the
+    # ends of rows that other blocks write at the same time.
+    r, y = residual_norm(x, residual, post=layer, branch_scale=0.5, next_norm=rms)
+    assert_rows_close(r, want, scale)
+    assert_rows_close(y, want_x, 4 * want_x.abs() + 4)
+    r8, (q, s) = residual_norm(x, residual, post=layer, branch_scale=0.5, next_norm=rms, quantize=True)
+    assert torch.equal(r8, r) and close_int8(q, s, want_x, 1024 + 127 * 4)
+    over_r, over_y = residual_norm(x, residual, post=layer, branch_scale=0.5, next_norm=rms, residual_out=residual,
+                                   out=x)
+    assert over_r is residual and over_y is x
+    assert torch.equal(over_r, r) and torch.equal(over_y, y)
+    again = rms(x)
+    assert torch.equal(rms(x, out=x), again)
+
+
+@pytest.mark.parametrize("rows,hidden", [(700, 2049), (1, 5120), (900, 5120), (7, 1111), (3, 100)])
+@pytest.mark.parametrize("offset,pad", [(3, 5), (0, 3), (1, 0), (0, 0), (8, 8)])
+def test_join_in_place_over_views(rows, hidden, offset, pad):
+    """The join over its own branch and residual, as views into wider buffers: both outputs, and nothing around them."""
+    size = offset + rows * (hidden + pad) + 16
+    buffers = [make((size,), BF16, 20 + i) for i in range(2)]
+    branch, residual = (b.as_strided((rows, hidden), (hidden + pad, 1), offset) for b in buffers)
+    norm = BlockNorm(make(hidden, BF16, 3, 0.2, 1.0), make(hidden, BF16, 4, 0.2), kind="layer")
+    gate = make((rows, hidden), BF16, 5)
+    b = norm64(branch.double(), norm) * gate.double()
+    want = residual.double() + b
+    scale = torch.maximum(b.abs(), residual.double().abs())
+    want_x = norm64(want, norm)
+    kept = [buffer.clone() for buffer in buffers]
+    r, x = residual_norm(branch, residual, post=norm, gate=gate, next_norm=norm, residual_out=residual, out=branch)
+    assert r is residual and x is branch
+    assert_rows_close(r, want, scale)
+    assert_rows_close(x, want_x, 4 * want_x.abs() + norm.bias.double().abs() + 4)
+    for now, before in zip(buffers, kept):
+        now.as_strided((rows, hidden), (hidden + pad, 1), offset).zero_()
+        before.as_strided((rows, hidden), (hidden + pad, 1), offset).zero_()
+        assert torch.equal(now, before)
+
+
+@pytest.mark.parametrize("low", [BF16, FP16])
+@pytest.mark.parametrize("rows,hidden", [(3, 64), (5, 1111), (40, 5120), (2, 20000), (1, 32768)])
+def test_join_of_mixed_types(rows, hidden, low):
+    """An fp32 branch with parameters, gate and output of 16 bits, and a 16-bit branch with those of the other type."""
+    other = FP16 if low is BF16 else BF16
+    for dtype, kind in ((FP32, low), (low, other)):
+        branch, residual = make((rows, hidden), dtype, 1), make((rows, hidden), FP32, 2, 3.0)
+        post = BlockNorm(make(hidden, kind, 3, 0.2, 1.0))
+        following = BlockNorm(make(hidden, kind, 4, 0.2, 1.0), make(hidden, kind, 5, 0.2), kind="layer")
+        gate = make((rows, hidden), kind, 6)
+        r, x = residual_norm(branch, residual, post=post, gate=gate, next_norm=following, out_dtype=kind)
+        b = norm64(branch.double(), post) * gate.double()
+        want = residual.double() + b
+        assert r.dtype == FP32 and x.dtype == kind
+        assert_rows_close(r, want, 3 * torch.maximum(b.abs(), residual.double().abs()))
+        want_x = norm64(want, following)
+        assert_rows_close(x, want_x, 4 * want_x.abs() + following.bias.double().abs() + 4)
 
 
 @pytest.fixture

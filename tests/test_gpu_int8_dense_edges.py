@@ -120,3 +120,43 @@ def test_silu_far_below_zero(tokens):
     bound = want.abs() * (2.0 ** -24 + (16 + 4 * g.abs()) * 2.0 ** -24 * 1.01) + 2.0 ** -148 * g.abs() * u.abs()
     assert bool(((h.double() - want).abs() <= bound).all())
     assert bool((h != 0).all())
+
+
+# By the kernels' rules on 148 SMs: CTA pairs with one tile and with several (more than 74, so that both accumulators,
+# the stages across tiles and groups of eight token tiles come round), with tiles of few tokens at the end (1800: eight
+# of 225) and fewer column blocks than stages; and the stream kernel with tiles of 128 tokens, one and two of them.
+LINEAR = [(300, 5000, 700), (1111, 5000, 900), (2600, 2100, 300), (1800, 2600, 200), (4096, 1300, 130),
+          (65, 5120, 17408), (128, 5120, 17408), (250, 5120, 17408)]
+GATED = [(300, 2500, 700), (1111, 2500, 900), (2600, 1100, 300), (1800, 1300, 200), (4096, 700, 130),
+         (65, 5200, 5120), (128, 5200, 5120)]
+
+
+@pytest.mark.parametrize("tokens,rows,cols", LINEAR)
+def test_linear_over_several_tiles(tokens, rows, cols):
+    xq, xs, wq, ws = operands(tokens, rows, cols)
+    want = product64(xq, xs, wq, ws)
+    bias = torch.randn(rows, generator=torch.Generator().manual_seed(3)).cuda()
+    for dtype in (BF16, FP16, FP32):
+        flat = torch.full((tokens * rows + 64,), 7.0, dtype=dtype, device="cuda")
+        y = int8_linear(xq, xs, wq, ws, bias=bias, out=flat[:tokens * rows].view(tokens, rows))
+        check_linear(y, want, bias)
+        assert bool((flat[tokens * rows:] == 7).all())
+        assert torch.equal(int8_linear(xq, xs, wq, ws, bias=bias, out_dtype=dtype), y)
+    # A token's result does not depend on the batch or the kernel that it comes in.
+    for t in (1, 40, 65):
+        part = int8_linear(xq[-t:], xs[-t:], wq, ws, bias=bias, out_dtype=FP32)
+        assert torch.equal(part, y[-t:])
+
+
+@pytest.mark.parametrize("tokens,rows,cols", GATED)
+def test_gated_over_several_tiles(tokens, rows, cols):
+    xq, xs, wq, ws = operands(tokens, 2 * rows, cols)
+    both = product64(xq, xs, wq, ws)
+    for dtype in (BF16, FP16, FP32):
+        flat = torch.full((tokens * rows + 64,), 7.0, dtype=dtype, device="cuda")
+        h = int8_gated_linear(xq, xs, wq, ws, out=flat[:tokens * rows].view(tokens, rows))
+        check_gated(h, both[:, :rows], both[:, rows:])
+        assert bool((flat[tokens * rows:] == 7).all())
+        assert torch.equal(int8_gated_linear(xq, xs, wq, ws, out_dtype=dtype), h)
+    for t in (1, 40, 65):
+        assert torch.equal(int8_gated_linear(xq[-t:], xs[-t:], wq, ws, out_dtype=FP32), h[-t:])
