@@ -62,6 +62,34 @@ def _out_rows(out: torch.Tensor, shape: torch.Size, rows: int, dtype: torch.dtyp
     return max(view.stride(0), hidden)
 
 
+def _overlap(a: tuple, b: tuple) -> bool:
+    """Whether rows given as (address, bytes between rows, bytes of a row, rows) share memory.  Rows of two different
+    strides, neither of them dense, may be interleaved in any way: taken as apart."""
+    (pa, sa, na, ta), (pb, sb, nb, tb) = a, b
+    if not (ta and tb) or pb >= pa + (ta - 1) * sa + na or pa >= pb + (tb - 1) * sb + nb:
+        return False
+    if sa == sb and ta > 1 and tb > 1:
+        apart = (pb - pa) % sa  # views side by side in wider rows
+        return apart < na or apart + nb > sa
+    for (p, s, n, t), (q, r, m, u) in ((a, b), (b, a)):
+        if t == 1 or s == n:  # dense: the first of the other's rows that ends behind its start
+            i = max(0, (p - q - m) // r + 1) if u > 1 else 0
+            return i < u and q + i * r < p + (t - 1) * s + n
+    return False
+
+
+def _extent(x: torch.Tensor, ld: int, cols: int, rows: int) -> tuple:
+    size = x.element_size()
+    return x.data_ptr(), (ld if rows > 1 else cols) * size, cols * size, rows
+
+
+def _check_overlap(out: tuple, name: str, inputs: tuple) -> None:
+    """An output may be an input itself (its rows and type), or apart from it."""
+    for what, rows in inputs:
+        if rows is not None and out != rows and _overlap(out, rows):
+            raise ValueError(f"{name} overlaps {what} without being it")
+
+
 def int8_rows(rows: int, cols: int, device: torch.device) -> torch.Tensor:
     """Uninitialised int8 [rows, cols] whose rows start on multiples of 16 bytes."""
     pad = -cols % 16
@@ -205,6 +233,7 @@ def _run_norm(x, norm, out, out_dtype, quantize):
         out_dtype = out_dtype or out.dtype
         out_code = _lib.dtype_code(out_dtype)
         ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
+        _check_overlap(_extent(out, ld_out, hidden, t), "out", (("x", _extent(rows, ld, hidden, t)),))
     lib = _lib.library()
     args = (rows.data_ptr(), ld, code, t, hidden, norm_ref, out.data_ptr(), ld_out, out_code,
             None if scale is None else scale.data_ptr())
@@ -266,8 +295,9 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
     leading axes match branch's, with trailing ones of them allowed to be 1 or
     missing altogether ([hidden], [T, 1], [T, hidden], [B, 1, hidden], ...).
     Returns r without a ``next_norm``, else (r, x), or (r, (int8, scales)) with
-    ``quantize=True``.  ``residual_out`` may be residual (in place) and ``out``
-    branch; other overlaps of inputs and outputs are not supported.
+    ``quantize=True``.  An output may be branch or residual itself
+    (``residual_out=residual, out=branch`` run in place); other overlaps are
+    refused.
     """
     index = branch.get_device()
     if index < 0 or residual.get_device() != index or (gate is not None and gate.get_device() != index):
@@ -296,11 +326,13 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
     t = branch.numel() // hidden
     if t > MAX_ROWS:
         raise ValueError(f"branch has {t} rows: at most {MAX_ROWS}")
+    given = out is not None
     if residual_out is None:
         residual_out = torch.empty_like(residual) if res_rows is residual else residual.new_empty(shape)
         ld_res_out = hidden
     else:
         ld_res_out = _out_rows(residual_out, shape, t, residual.dtype, index, "residual_out")
+        given = True
     scale_ptr, out_ptr, ld_out, out_code = None, None, hidden, code
     if next_norm is not None:
         if quantize:
@@ -321,6 +353,20 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
             out_code = _lib.dtype_code(out_dtype)
             ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
         out_ptr = out.data_ptr()
+    if given:
+        inputs = (("branch", _extent(rows, ld, hidden, t)), ("residual", _extent(res_rows, ld_res, hidden, t)))
+        r_extent = _extent(residual_out, ld_res_out, hidden, t)
+        x_extent = None if out is None else _extent(out, ld_out, hidden, t)
+        _check_overlap(r_extent, "residual_out", inputs)
+        if x_extent is not None:
+            _check_overlap(x_extent, "out", inputs)
+            if _overlap(x_extent, r_extent):
+                raise ValueError("out overlaps residual_out")
+        if gate is not None:
+            g_extent = _extent(gate_rows, max(gate_rows.stride(0), 1), gate_rows.shape[1], gate_rows.shape[0])
+            for name, extent in (("residual_out", r_extent), ("out", x_extent)):
+                if extent is not None and _overlap(extent, g_extent):
+                    raise ValueError(f"{name} overlaps the gate")
     lib = _lib.library()
     args = (rows.data_ptr(), ld, code, res_rows.data_ptr(), ld_res, res_code, t, hidden, post_ref, gate_ref,
             residual_scale, branch_scale, residual_out.data_ptr(), ld_res_out, next_ref, out_ptr, ld_out, out_code,

@@ -264,6 +264,41 @@ def test_join_of_mixed_types(rows, hidden, low):
         assert_rows_close(x, want_x, 4 * want_x.abs() + following.bias.double().abs() + 4)
 
 
+@pytest.mark.parametrize("hidden", [64, 1111, 5120])
+def test_overlaps_are_refused_unless_an_output_is_an_input(hidden):
+    rows = 40
+    norm = BlockNorm(make(hidden, BF16, 3, 0.2, 1.0))
+    flat = make((rows * 2 * hidden + hidden,), BF16, 1)
+    x = flat[:rows * hidden].view(rows, hidden)
+    behind = flat[hidden:hidden + rows * hidden].view(rows, hidden)  # x, a row later
+    residual = make((rows, hidden), BF16, 2)
+    other = torch.empty_like(x)
+    # Views side by side in wider rows are apart.
+    wide = make((rows, 2 * hidden), BF16, 4)
+    left, right = wide[:, :hidden], wide[:, hidden:]
+    want = norm(left)
+    norm(left, out=right)
+    assert torch.equal(right, want)
+    r, y = residual_norm(left, residual, next_norm=norm, residual_out=right, out=left)
+    assert r is right and y is left
+    # An output in an input's place, whichever it is.
+    want = residual_norm(x, residual, next_norm=norm)
+    for r_out, x_out in ((1, 0), (0, 1), (None, 1), (0, None), (1, None), (None, 0)):
+        pair = [x.clone(), residual.clone()]
+        got = residual_norm(*pair, next_norm=norm, residual_out=None if r_out is None else pair[r_out],
+                            out=None if x_out is None else pair[x_out])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for call in (lambda: norm(x, out=behind), lambda: norm(behind, out=x), lambda: norm(wide[:, 1:hidden + 1], out=left),
+                 lambda: residual_norm(x, residual, residual_out=behind),
+                 lambda: residual_norm(residual, x, next_norm=norm, out=behind),
+                 lambda: residual_norm(x, residual, next_norm=norm, residual_out=other, out=other),
+                 lambda: residual_norm(x, residual, next_norm=norm, residual_out=x, out=x),
+                 lambda: residual_norm(x, residual, gate=other, residual_out=other),
+                 lambda: residual_norm(x, residual, gate=other[1], next_norm=norm, out=other)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+
+
 @pytest.fixture
 def no_waiting():
     """Launches made inside give up at once unless their copies are there already."""

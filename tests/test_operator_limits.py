@@ -2,12 +2,13 @@
 from __future__ import annotations
 
 import ctypes
+import random
 
 import torch
 
 import conftest  # noqa: F401
 from qcc_b200 import _lib
-from qcc_b200.runtime.block_norm import BlockNorm
+from qcc_b200.runtime.block_norm import BlockNorm, _overlap
 
 
 def test_wait_limit_is_a_minute_at_most():
@@ -65,3 +66,28 @@ def test_a_norm_that_is_launching_keeps_its_argument():
     assert launching._obj.weight == 256 and replaced._obj.weight == 512
     assert norm._for(32, 0) is replaced
     assert abs(norm.eps - 1e-5) < 1e-12 and norm.weight_offset == 1.0 and norm.kind == "rms" and norm.hidden == 32
+
+
+def test_overlap_of_rows():
+    """Against the bytes themselves; rows that are certain to overlap are found, rows that are apart never refused."""
+    rng = random.Random(0)
+    certain = 0
+    for _ in range(4000):
+        extents = []
+        for _ in range(2):
+            size, rows = rng.randint(1, 6), rng.randint(0, 4)
+            extents.append((rng.randint(0, 40), size + rng.choice([0, 0, 1, 3, 7]), size, rows))
+        if rng.random() < 0.5:  # views of one wider tensor
+            extents[1] = (extents[1][0], extents[0][1], min(extents[1][2], extents[0][1]), extents[0][3])
+        a, b = extents
+        used = [{p + i * s + k for i in range(t) for k in range(n)} for p, s, n, t in extents]
+        shared = bool(used[0] & used[1])
+        found = _overlap(a, b)
+        assert found == _overlap(b, a)
+        dense = any(t <= 1 or s == n for _, s, n, t in extents)
+        if a[1] == b[1] or dense:
+            assert found == shared, (a, b)
+            certain += shared
+        else:
+            assert not found or shared
+    assert certain > 300
