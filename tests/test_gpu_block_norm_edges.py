@@ -299,6 +299,25 @@ def test_overlaps_are_refused_unless_an_output_is_an_input(hidden):
             call()
 
 
+def test_rows_beyond_2_to_the_31_elements():
+    """Offsets of the last rows pass 32 bits: they come out as they do alone."""
+    rows, hidden = 430_000, 5120
+    x = torch.empty((rows, hidden), dtype=BF16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))
+    norm = BlockNorm(make(hidden, BF16, 3, 0.2, 1.0))
+    last = slice(rows - 70, rows)
+    part = x[last].clone()
+    assert torch.equal(norm(x)[last], norm(part))
+    q, s = norm(x, quantize=True)
+    want = norm(part, quantize=True)
+    assert torch.equal(q[last], want[0]) and torch.equal(s[last], want[1])
+    q, s = quantize_rows(x)
+    want = quantize_rows(part)
+    assert torch.equal(q[last], want[0]) and torch.equal(s[last], want[1])
+    r, y = residual_norm(x, x, post=norm, next_norm=norm, residual_out=x)
+    want = residual_norm(part, part, post=norm, next_norm=norm)
+    assert r is x and torch.equal(r[last], want[0]) and torch.equal(y[last], want[1])
+
+
 @pytest.fixture
 def no_waiting():
     """Launches made inside give up at once unless their copies are there already."""

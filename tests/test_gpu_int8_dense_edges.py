@@ -160,3 +160,21 @@ def test_gated_over_several_tiles(tokens, rows, cols):
         assert torch.equal(int8_gated_linear(xq, xs, wq, ws, out_dtype=dtype), h)
     for t in (1, 40, 65):
         assert torch.equal(int8_gated_linear(xq[-t:], xs[-t:], wq, ws, out_dtype=FP32), h[-t:])
+
+
+def test_outputs_beyond_2_to_the_31_elements():
+    """The most tokens that are taken, with outputs whose offsets pass 32 bits."""
+    tokens, rows, cols = 1 << 20, 2100, 20
+    xq, xs, wq, ws = operands(70, rows, cols)
+    xq = torch.cat([xq.new_zeros((tokens - 70, 32)), torch.nn.functional.pad(xq, (0, 12))])[:, :cols]
+    xs = torch.cat([torch.ones(tokens - 70, device="cuda"), xs])
+    y = int8_linear(xq, xs, wq, ws)
+    check_linear(y[-70:], product64(xq[-70:], xs[-70:], wq, ws))
+    assert not bool(y[:-70].any())
+    with pytest.raises(ValueError, match="tokens"):
+        int8_linear(torch.zeros((tokens + 1, 16), dtype=torch.int8, device="cuda"), torch.zeros(tokens + 1, device="cuda"),
+                    wq[:, :16], ws)
+    del y
+    both = product64(xq[-70:], xs[-70:], wq, ws)
+    h = int8_gated_linear(xq, xs, wq, ws)
+    check_gated(h[-70:], both[:, :rows // 2], both[:, rows // 2:])
