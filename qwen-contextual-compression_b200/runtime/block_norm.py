@@ -48,6 +48,8 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 def _out_rows(out: torch.Tensor, shape: torch.Size, rows: int, dtype: torch.dtype, index: int, what: str) -> int:
     """Checks a caller's output tensor; returns the stride of its rows."""
+    if out.requires_grad:
+        _lib.refuse_grad(f"writing {what}", out)
     if out.shape != shape or out.dtype != dtype or out.get_device() != index:
         raise ValueError(f"{what} must be {tuple(shape)} in {dtype} on the inputs' device")
     hidden = shape[-1]

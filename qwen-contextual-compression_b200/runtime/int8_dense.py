@@ -76,6 +76,8 @@ def _products(xq, x_scale, wq, w_scale, bias, out, out_dtype, gated):
         ldy = channels
     else:
         y_code = _lib.dtype_code(out.dtype)
+        if out.requires_grad:
+            _lib.refuse_grad("writing out", out)
         if (out.shape != (tokens, channels) or (out_dtype or out.dtype) != out.dtype
                 or (out.stride(1) != 1 and channels != 1) or (tokens > 1 and out.stride(0) < channels)):
             raise ValueError("out must be a row-contiguous [tokens, channels] tensor of out_dtype")

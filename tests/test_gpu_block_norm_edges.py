@@ -299,6 +299,22 @@ def test_overlaps_are_refused_unless_an_output_is_an_input(hidden):
             call()
 
 
+def test_outputs_that_require_a_gradient_are_refused():
+    """Autograd would not see the write into a leaf (or into a tensor that a backward pass has kept)."""
+    x, norm = make((4, 64), FP32, 1), BlockNorm()
+    leaf = torch.zeros_like(x).requires_grad_()
+    xq, xs = quantize_rows(x)
+    square = torch.zeros((4, 4), device="cuda", requires_grad=True)
+    for call in (lambda: norm(x, out=leaf), lambda: residual_norm(x, x, residual_out=leaf),
+                 lambda: residual_norm(x, x, next_norm=norm, out=leaf), lambda: int8_linear(xq, xs, xq, xs, out=square),
+                 lambda: int8_gated_linear(xq, xs, xq, xs, out=square[:, :2])):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(leaf.detach(), norm(x)) or torch.equal(leaf.detach(), norm(2 * x))
+
+
 def test_rows_beyond_2_to_the_31_elements():
     """Offsets of the last rows pass 32 bits: they come out as they do alone."""
     rows, hidden = 430_000, 5120
