@@ -68,7 +68,7 @@ def _overlap(a: tuple, b: tuple) -> bool:
     """Whether rows given as (address, bytes between rows, bytes of a row, rows) share memory.  Rows of two different
     strides, neither of them dense, may be interleaved in any way: taken as apart."""
     (pa, sa, na, ta), (pb, sb, nb, tb) = a, b
-    if not (ta and tb) or pb >= pa + (ta - 1) * sa + na or pa >= pb + (tb - 1) * sb + nb:
+    if pb >= pa + (ta - 1) * sa + na or pa >= pb + (tb - 1) * sb + nb or not (ta and tb):
         return False
     if sa == sb and ta > 1 and tb > 1:
         apart = (pb - pa) % sa  # views side by side in wider rows
@@ -81,7 +81,7 @@ def _overlap(a: tuple, b: tuple) -> bool:
 
 
 def _extent(x: torch.Tensor, ld: int, cols: int, rows: int) -> tuple:
-    size = x.element_size()
+    size = x.itemsize
     return x.data_ptr(), (ld if rows > 1 else cols) * size, cols * size, rows
 
 
@@ -356,14 +356,16 @@ def residual_norm(branch: torch.Tensor, residual: torch.Tensor, *, post: BlockNo
             ld_out = _out_rows(out, shape, t, out_dtype, index, "out")
         out_ptr = out.data_ptr()
     if given:
-        inputs = (("branch", _extent(rows, ld, hidden, t)), ("residual", _extent(res_rows, ld_res, hidden, t)))
-        r_extent = _extent(residual_out, ld_res_out, hidden, t)
-        x_extent = None if out is None else _extent(out, ld_out, hidden, t)
-        _check_overlap(r_extent, "residual_out", inputs)
-        if x_extent is not None:
-            _check_overlap(x_extent, "out", inputs)
-            if _overlap(x_extent, r_extent):
-                raise ValueError("out overlaps residual_out")
+        branch_extent, res_extent = _extent(rows, ld, hidden, t), _extent(res_rows, ld_res, hidden, t)
+        r_extent = res_extent if residual_out is res_rows else _extent(residual_out, ld_res_out, hidden, t)
+        x_extent = branch_extent if out is rows else None if out is None else _extent(out, ld_out, hidden, t)
+        if x_extent is not None and _overlap(x_extent, r_extent):
+            raise ValueError("out overlaps residual_out")
+        if r_extent is not res_extent or x_extent is not branch_extent:  # else that was the one test that is left
+            inputs = ("branch", branch_extent), ("residual", res_extent)
+            _check_overlap(r_extent, "residual_out", inputs)
+            if x_extent is not None:
+                _check_overlap(x_extent, "out", inputs)
         if gate is not None:
             g_extent = _extent(gate_rows, max(gate_rows.stride(0), 1), gate_rows.shape[1], gate_rows.shape[0])
             for name, extent in (("residual_out", r_extent), ("out", x_extent)):
