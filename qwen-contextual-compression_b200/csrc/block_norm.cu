@@ -788,10 +788,9 @@ __host__ __device__ constexpr int code_of() {
 }
 
 // The end of a block whose wait for row t (slot s) ran out: its rows from t on become NaN (int8: zeros, and NaN as the
-// scale), and thread 0 sees the copies in flight in, which would land in the shared memory of a later block.  Not
-// inlined: the registers of this path would cost the norms 15 %.
-__device__ __noinline__ void give_up(const BlockNormArgs& a, int res_dtype, uint64_t* full, int depth, int64_t t, int s,
-                                     int phase) {
+// scale), and thread 0 sees the copies in flight in, which would land in the shared memory of a later block.
+__device__ __forceinline__ void give_up(const BlockNormArgs& a, int res_dtype, uint64_t* full, int depth, int64_t t,
+                                        int s, int phase) {
   if (threadIdx.x == 0)
     for (int64_t u = t, k = 0; k < depth && u < a.rows; ++k, u += gridDim.x) {
       mbar_wait_suspended(&full[s], phase, kDrainNs);
@@ -808,6 +807,11 @@ __device__ __noinline__ void give_up(const BlockNormArgs& a, int res_dtype, uint
     }
     if (threadIdx.x == 0 && a.out != nullptr && a.out_dtype == QCC_DTYPE_I8) a.row_scale[t] = NAN;
   }
+}
+
+__device__ __noinline__ void give_up_call(const BlockNormArgs& a, int res_dtype, uint64_t* full, int depth, int64_t t,
+                                          int s, int phase) {
+  give_up(a, res_dtype, full, depth, t, s, phase);
 }
 
 // A block a row at a time, rows gridDim.x apart; thread 0 keeps `depth` rows of bulk copies ahead, so DRAM is busy
@@ -852,6 +856,12 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     }
   BlockTeam team = {scratch};
   int s = 0, phase = 0;
+  // Where the way out of a wait that ran out stands decides the loop's registers: behind the loop for norms of two whole
+  // granules a thread (4096 x 8000 27.8 us, 34.8 with a call from inside), a call for the others (norm of 4096 x 8001
+  // 34.0 and 48.4 us; join of 4096 x 12288 73.4 and 85.7, rows to int8 of 4096 x 17408 34.9 and 36.0).  Inline inside
+  // the loop it costs the norms 15 %.
+  constexpr bool kGiveUpLast = EXACT && VPT == 2 && MODE == kNorm;
+  int64_t lost = a.rows;
   for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
     const int shift = EXACT ? 0 : row_shift(a, t);
     const GranuleMap<EXACT> m = {a.hidden, shift, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
@@ -879,7 +889,11 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     // it made of the row.  A thread that is a row ahead of this test marks that row's own entry.
     __syncthreads();
     if (missing[phase][s] != 0) {
-      give_up(a, code_of<R>(), full, depth, t, s, phase);
+      if (kGiveUpLast) {
+        lost = t;
+        break;
+      }
+      give_up_call(a, code_of<R>(), full, depth, t, s, phase);
       return;
     }
     const int64_t ahead = t + static_cast<int64_t>(depth) * gridDim.x;
@@ -890,6 +904,7 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
       finish_row<P>(v, a, t, m, team);
     if (++s == depth) s = 0, phase ^= 1;
   }
+  if (kGiveUpLast && lost < a.rows) give_up(a, code_of<R>(), full, depth, lost, s, phase);
 }
 
 // ---------------------------------------------------------------------------
