@@ -576,7 +576,7 @@ typedef struct qcc_gate_params {
 
 /* Bound, in ns, on each wait of later launches of the block norms and of the
  * 8-bit integer products for their own copies (2 s until set, 60 s at most; 0:
- * a wait looks once and gives up unless the copies are there already).  A
+ * a wait gives up unless the copies are there already).  A
  * block whose wait ran out leaves the rows or the tiles that it still had to
  * write as NaN (int8: zeros and a scale of NaN), sees its copies in and ends;
  * there is no status word.  Process-wide; a captured launch keeps the bound

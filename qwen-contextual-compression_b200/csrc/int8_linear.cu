@@ -96,18 +96,20 @@ struct RowOutput {
   bool in;  // the channel exists
   bool ordinary;  // its scales are ordinary ones
 
-  // row0: the first weight row (gated: channel) of the 32-lane group.  A tile whose wait ran out is `broken`: its
-  // scales become NaN, and so do its outputs.
-  __device__ __forceinline__ RowOutput(const Int8Args& a, int row0, int t0, int lane, bool broken) {
+  // row0: the first weight row (gated: channel) of the 32-lane group.
+  __device__ __forceinline__ RowOutput(const Int8Args& a, int row0, int t0, int lane) {
     const int n = row0 + (GATED ? lane & 15 : lane);
     in = n < a.channels;
     ldy = a.ldy;
     y = static_cast<O*>(a.y) + static_cast<int64_t>(t0) * a.ldy + n;
-    ws = broken ? NAN : in ? a.ws[n] : 0.f;
+    ws = in ? a.ws[n] : 0.f;
     ws_up = GATED && in ? a.ws[a.channels + n] : 0.f;
     bias = !GATED && in ? bias_value(a.bias, a.bias_dtype, n) : 0.f;
     ordinary = ordinary_scale(ws) && ordinary_scale(ws_up);
   }
+
+  // For a tile whose wait ran out: its scales become NaN, and so do its outputs.
+  __device__ __forceinline__ void break_off() { ws = NAN, ordinary = false; }
 
   // The same as finish for scales that are not ordinary, in few instructions rather than in short time.
   template <int J>
@@ -251,6 +253,13 @@ __global__ void __launch_bounds__(128)
   const uint32_t tmem = tmem_slot;
   grid_dependency_trigger();
 
+  // What the outputs need besides the sums arrives while those are made.
+  const int tokens = min(BN, a.tokens - t0);
+  RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane);
+  const auto token_scale = [&](int c) { return c + lane < tokens ? a.xs[t0 + c + lane] : 0.f; };
+  constexpr int kRun = 4;  // of a split: tokens a warp sums at a time; the cluster's CTAs take runs in turn
+  float xs = token_scale(splits == 1 ? 0 : static_cast<int>(rank) * kRun);
+
   int issued = 0;  // thread 0: blocks whose copies it started
   if (threadIdx.x == 0) {
     const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
@@ -295,16 +304,16 @@ __global__ void __launch_bounds__(128)
   tc_fence_after_sync();
   __syncthreads();
 
-  const int tokens = min(BN, a.tokens - t0);
   const uint32_t from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
   if (splits == 1) {
-    const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, failed != 0);
+    if (failed != 0) out.break_off();
 #pragma unroll 1
     for (int c = 0; c < tokens; c += 16) {
-      const float xs = c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
+      const float xs_next = token_scale(c + 16);
       int acc[16];
       tmem_load16(from + c, acc);
       out.finish(acc, c, tokens, xs, lane);
+      xs = xs_next;
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -327,10 +336,9 @@ __global__ void __launch_bounds__(128)
     int flags[kMaxSplit];
 #pragma unroll
     for (uint32_t r = 0; r < kMaxSplit; ++r) flags[r] = r < splits ? cluster_load(smem_addr(&failed), r) : 0;
-    int any = 0;
-    constexpr int kRun = 4;  // tokens a warp sums at a time; the cluster's CTAs take runs in turn
-    for (int c = static_cast<int>(rank) * kRun; c < tokens; c += static_cast<int>(splits) * kRun) {
-      const float xs = lane < kRun && c + lane < tokens ? a.xs[t0 + c + lane] : 0.f;
+    const int step = static_cast<int>(splits) * kRun;
+    for (int c = static_cast<int>(rank) * kRun; c < tokens; c += step) {
+      const float xs_next = token_scale(c + step);
       int part[kMaxSplit][kRun];
 #pragma unroll
       for (uint32_t r = 0; r < kMaxSplit; ++r)
@@ -340,12 +348,12 @@ __global__ void __launch_bounds__(128)
       int acc[kRun] = {};
 #pragma unroll
       for (uint32_t r = 0; r < kMaxSplit; ++r) {
-        any |= flags[r];
+        if (flags[r] != 0) out.break_off();
 #pragma unroll
         for (int j = 0; j < kRun; ++j) acc[j] += part[r][j];
       }
-      const RowOutput<GATED, O> out(a, n0 + warp * (GATED ? 16 : 32), t0, lane, any != 0);
       out.finish(acc, c, tokens, xs, lane);
+      xs = xs_next;
     }
     __syncwarp();
     cluster_sync();  // the other CTAs have read this one's sums
@@ -522,9 +530,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int row, token;
       pair_tile(plan, i, row, token);
       const int t0 = token * plan.tile_tokens, tokens = min(plan.tile_tokens, a.tokens - t0);
-      const RowOutput<GATED, O> out(
-          a, row * kChannels + static_cast<int>(rank) * (kChannels / 2) + quarter * (GATED ? 16 : 32), t0, lane,
-          broken);
+      RowOutput<GATED, O> out(
+          a, row * kChannels + static_cast<int>(rank) * (kChannels / 2) + quarter * (GATED ? 16 : 32), t0, lane);
+      if (broken) out.break_off();
       const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
       int c = (warp - 2) / 4 * 32;
       for (; c < tokens; c += 64) {

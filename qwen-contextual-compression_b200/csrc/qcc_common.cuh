@@ -86,32 +86,36 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 }
 
 // The bounded wait for threads that have nothing else to do: each try lets the
-// hardware suspend the thread (for up to 100 us), so that waiting warps leave
-// the issue slots to the working ones.  The clock is read after the first look
-// (LOOK_FIRST, fewer registers: for barriers that are mostly complete) or after
-// a first try (for barriers that are mostly not: the clock's read costs the
-// int8 products 3 to 9 %).  A limit of 0 looks once.
+// hardware suspend the thread (for up to 100 us, and not beyond the limit), so
+// that waiting warps leave the issue slots to the working ones.  LOOK_FIRST,
+// for barriers that are mostly complete, begins with a look that never
+// suspends, after which a limit of 0 gives up (fewer registers); otherwise the
+// clock is read after a first try (its read before one costs the int8 products
+// 3 to 9 %, and a branch on the limit 1 %).
 template <bool LOOK_FIRST = false>
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  if (LOOK_FIRST) {
-    if (mbar_test(bar, parity)) return true;
-    if (limit_ns == 0) return false;
-  } else {
-    if (limit_ns == 0) return mbar_test(bar, parity);
-    if (mbar_try_wait(bar, parity)) return true;
-  }
-  const uint64_t start = global_timer_ns();
-  while (true) {
+  const uint32_t hint = LOOK_FIRST || limit_ns > 100000u ? 100000u : static_cast<uint32_t>(limit_ns);
+  const auto attempt = [&] {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(100000u)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(hint)
         : "memory");
-    if (done != 0) return true;
-    if (global_timer_ns() - start > limit_ns) return false;
+    return done != 0;
+  };
+  if (LOOK_FIRST) {
+    if (mbar_test(bar, parity)) return true;
+    if (limit_ns == 0) return false;
+  } else if (attempt()) {
+    return true;
+  }
+  const uint64_t start = global_timer_ns();
+  while (true) {
+    if (attempt()) return true;
+    if (global_timer_ns() - start >= limit_ns) return false;
   }
 }
 
