@@ -270,8 +270,8 @@ __device__ __forceinline__ int settle_border(float x, float amax, int q) {
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers, held in the low bits
 
 // int8 of computed values (norms), in the low bytes: round_half_even of 127 x / amax rounded to fp32.  The reciprocal's
-// remainder brings the quotient within 2^-28 of itself before its rounding (2^-47 where the remainder is a normal
-// number), so a border k + 1/2 comes out as such.
+// remainder brings the quotient within 2^-47 of itself before its rounding, or 2^-28 where the remainder is no longer a
+// normal number (amax above 2^109 or so), so a border k + 1/2 comes out as such.
 __device__ __forceinline__ float2 quotient2(float2 x, const RowScale& s) {
   return fma2(x, both(s.inverse), mul2(x, both(s.inverse_rest)));
 }
@@ -288,11 +288,12 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// int8 of rows as they are: round_half_even(127 x / amax), of the exact quotient, for |x| <= amax.  The quotient with
-// the reciprocal's remainder is within 2^-47 of itself before its one rounding to fp32, so a border k + 1/2 comes out
-// as such.  Values of 16-bit types lie on borders in earnest (small whole numbers times powers of two), and no other
-// quotient of theirs rounds to one: with 11-bit significands those in [2^k, 2^(k+1)) are 2^(k-20) or more away from a
-// border, and fp32 is off by 2^(k-24) there.  fp32 values that round to a border need the exact remainder.
+// int8 of rows as they are: round_half_even(127 x / amax), of the exact quotient, for |x| <= amax.  Before its one
+// rounding to fp32 the quotient is within 2^-28 of itself (see quotient2), less than half a last place, so a border
+// k + 1/2 comes out as such, and what does not come out as one lies on its own side of it.  Values of 16-bit types lie
+// on borders in earnest (small whole numbers times powers of two), and no other quotient of theirs rounds to one: with
+// 11-bit significands those in [2^k, 2^(k+1)) are 2^(k-20) or more away from a border, and fp32 and the quotient before
+// it are off by 2^(k-23) together there.  fp32 values that round to a border need the exact remainder.
 template <typename T>
 __device__ __forceinline__ void quantize8_exact(const float (&f)[8], const RowScale& s, uint32_t (&q)[8]) {
   bool border = false;
@@ -682,7 +683,8 @@ struct RowNorm {
 };
 
 // One block a row; outputs are written in the last pass, so they may be the inputs themselves.  Single elements and
-// repeated reads make it slow (join of 4096 x 5120 with a residual off by 6 bytes: 167 us, 32 us on shared granules).
+// repeated reads make it slow (join of 4096 x 5120 with a residual off by 6 bytes: 167 us, 32 us on shared granules;
+// of fp32 rows with bf16 weights and output 191 us; rows to int8 of 4096 x 36864 543 us, 70 us of bytes).
 __global__ void __launch_bounds__(512) plain_kernel(const BlockNormArgs a, int dtype, int res_dtype) {
   __shared__ __align__(16) float scratch[2 * kMaxWarps];
   BlockTeam::clear(scratch);
@@ -739,7 +741,8 @@ constexpr int kRoom = 208 << 10, kDeepRoom = 128 << 10;
 // threads: 30.7 us with four and three rows each, 35.6 with five and two).
 constexpr int kMostThreads = 1344;
 
-// Threads of a ring block, at most; and blocks of that size an SM that its registers allow without spills.  Two
+// Threads of a ring block, at most; and blocks of that size an SM that its registers allow with no more than 8 bytes of
+// spills.  Two
 // granules a thread up to 640 threads for norms (8192 x 5120 bf16: 31.8 us, 34.4 us with four; fp32 60.6 and 76.2 us),
 // four from 192 threads on for plain quantisation, whose threads do little else (4096 x 5120: 12.5 us, 17 with two).
 template <Mode MODE, int VPT, bool EXACT>
@@ -816,11 +819,11 @@ __device__ __noinline__ void give_up_call(const BlockNormArgs& a, int res_dtype,
 
 // A block a row at a time, rows gridDim.x apart; thread 0 keeps `depth` rows of bulk copies ahead, so DRAM is busy
 // while the block reduces.  Several small blocks an SM hide each other's reductions.  Measured (bf16): norm of
-// 8192 x 5120 31.6 us (5.3 of 6.45 TB/s), join 61 us (5.5 TB/s), int8 rows of 4096 x 17408 37.8 us (5.7 TB/s).
+// 8192 x 5120 31.0 us (5.4 of 6.45 TB/s), join 59.8 us (5.6 TB/s), int8 rows of 4096 x 17408 34.9 us (6.1 TB/s).
 // The issue slots are 65 to 69 % busy then, 17 instructions an element of the norm, 33 of the join: they and the
 // reductions' latency bound it, not DRAM.
-// Layer norms take a second reduction (42.8 us) and odd widths two loads for eight parameters (4096 x 8001: 33.3 us,
-// 8000: 28 us).
+// Layer norms take a second reduction (43.4 us), norms to int8 another and three more instructions a value (42.6 us),
+// odd widths two loads for eight parameters (4096 x 8001: 34.0 us, 8000: 27.8 us) and a store a value to int8 (74 us).
 template <typename T, typename R, Mode MODE, int VPT, bool EXACT>
 __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingShape<MODE, VPT, EXACT>::kBlocks)
     ring_kernel(const __grid_constant__ BlockNormArgs a, int depth) {
@@ -856,10 +859,10 @@ __global__ void __launch_bounds__(RingShape<MODE, VPT, EXACT>::kThreads, RingSha
     }
   BlockTeam team = {scratch};
   int s = 0, phase = 0;
-  // Where the way out of a wait that ran out stands decides the loop's registers: behind the loop for norms of two whole
-  // granules a thread (4096 x 8000 27.8 us, 34.8 with a call from inside), a call for the others (norm of 4096 x 8001
-  // 34.0 and 48.4 us; join of 4096 x 12288 73.4 and 85.7, rows to int8 of 4096 x 17408 34.9 and 36.0).  Inline inside
-  // the loop it costs the norms 15 %.
+  // Where the way out of a wait that ran out stands decides the loop's registers: behind the loop for norms of two
+  // whole granules a thread (4096 x 8000 27.8 us, 34.8 with a call from inside), a call for the others (norm of 4096 x
+  // 8001 34.0 and 48.4 us; join of 4096 x 12288 73.4 and 85.7, rows to int8 of 4096 x 17408 34.9 and 36.0).  Inline
+  // inside the loop it costs the norms 15 %.
   constexpr bool kGiveUpLast = EXACT && VPT == 2 && MODE == kNorm;
   int64_t lost = a.rows;
   for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
@@ -966,7 +969,9 @@ bool launch_granules(const BlockNormArgs& a, int granules, int device, cudaStrea
   if constexpr (EXACT) {
     // Many rows: a warp takes up to 192 granules, or 256 when it only quantises (8192 rows of 1536 bf16: norm 11.5 us
     // against the ring's 14.8, int8 7.3 against 10.8; 2048: int8 9.3 against 11.9, but norm 15.7 against 15.4).  Few
-    // rows: a block's more threads have less latency (500 layer norms of 1536: 3.8 us and 3.3 us).
+    // rows: a block's more threads have less latency (500 layer norms of 1536: 3.8 us and 3.3 us).  Around kManyRows, a
+    // warp and the ring: 2048 rows of 1536 norm 4.1 and 3.7 us, join 6.1 and 6.9, int8 2.4 and 3.8; 4096 rows 5.1 and
+    // 6.0, 10.7 and 12.2, 3.7 and 5.6; 1024 rows 3.6 and 2.9, 4.8 and 5.1, 1.9 and 2.9.
     if (a.rows >= kManyRows && granules <= 192)
       return launch_early(warp_kernel<T, R, MODE, 6, EXACT>, grid, 32 * kWarpRows, 0, stream, a);
     if constexpr (MODE == kQuantize)

@@ -171,9 +171,10 @@ struct RowOutput {
 // its own shared memory, and the cluster adds them over distributed shared
 // memory -- integer sums, so the split changes no bit of the result, and there
 // is no workspace that two calls could share.
-// Measured: gate|up 34816 x 5120, 1 token 28.9 us (6.2 of 6.45 TB/s), 64 tokens
-// 33.3 us; down 5120 x 17408, 1 token 16.8 us (5.3 TB/s: filling the rings and
-// joining the cluster take 3 us), 128 tokens 23.9 us.
+// Measured: gate|up 34816 x 5120, 1 token 28.3 us (6.3 of 6.45 TB/s), 64 tokens
+// 29.5 us, 128 tokens 33.6; down 5120 x 17408, 1 token 16.8 us (5.3 TB/s:
+// filling the rings and joining the cluster take 3 us), 128 tokens 22.5 us, 256
+// 33.2 (twice its floor: 128 x 128 tiles load 3.7 times the operands from L2).
 // ---------------------------------------------------------------------------
 
 template <int BN, int STAGES>
@@ -372,10 +373,11 @@ __global__ void __launch_bounds__(128)
 // columns) let a tile's epilogue run beside the next tile's MMAs.  A pair reads
 // each operand byte of its tile once (128 rows of each per CTA), half of what
 // two single CTAs would.
-// Measured at 4096 tokens: gate|up 34816 x 5120 529 to 570 us (2.8 to 2.6
-// POP/s), down 5120 x 17408 274 to 290 us (320 tiles are 4.3 rounds of 74
-// pairs).  A long run sits at the card's 1000 W with the SMs near 1.5 GHz, as
-// cuBLAS's bf16 product does (1.4 PFLOP/s sustained): power bounds it.
+// Measured at 4096 tokens: gate|up 34816 x 5120 454 us (3.2 POP/s), down 5120 x
+// 17408 230 us (3.2 POP/s; 320 tiles are 4.3 rounds of 74 pairs).  In runs of
+// seconds, with the launches before them, 561 and 309 us: the card sits at its
+// 1000 W then, as in cuBLAS's bf16 product (1.4 PFLOP/s sustained): power
+// bounds it.
 // ---------------------------------------------------------------------------
 
 constexpr int kPairStages = 6;
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = tmem_slot;
   grid_dependency_trigger();
 
-  // This CTA's copies of column block b of a tile into stage s, counted (with the other CTA's) on the even CTA's barrier.
+  // This CTA's copies of column block b of a tile into stage s, counted with the other CTA's on the even one's barrier.
   const auto load = [&](int row, int token, int b, int s) {
     const uint64_t keep = policy_evict_last();
     uint8_t* w = ring + s * kPairStage;
@@ -673,7 +675,7 @@ int launch_pair(const Int8Args& a, int device, cudaStream_t stream) {
   PairPlan plan;
   plan.row_tiles = (a.channels + channels - 1) / channels;
   // As few token tiles as fit, of equal width: a tile's time hardly falls with its width (4096 tokens of the 34816 x
-  // 5120 gated product: 702 us at 256 wide, 889 at 192, 1240 at 128), its weight rows' loads stay.
+  // 5120 gated product: 458 us at 256 wide, 559 at 192, 741 at 128), its weight rows' loads stay.
   plan.token_tiles = (a.tokens + kPairTokens - 1) / kPairTokens;
   plan.tile_tokens = ((a.tokens + plan.token_tiles - 1) / plan.token_tiles + 31) / 32 * 32;
   plan.group = kPairGroup;
@@ -701,13 +703,16 @@ int launch(const Int8Args& a, int device, cudaStream_t stream) {
   if (a.tokens <= 32) return launch_stream<GATED, O, 32, 4>(a, device, stream);
   if (a.tokens <= 64) return launch_stream<GATED, O, 64, 4>(a, device, stream);
   // Pairs where their tiles fill at least half of the SMs (512 tokens, 17408 columns to 5120 channels, 40 tiles: pairs
-  // 55 us, stream 60 us; 256 tokens, 20 tiles: 58 and 33 us).
+  // 48 us, stream 60 us; 256 tokens, 20 tiles: 46 and 33 us; 256 tokens of 4000 x 4000, 16 tiles: 17.3 and 13.4).  Not
+  // right everywhere: 256 tokens of 6000 x 6000, 24 tiles, 25.4 and 33.8.
   const int channels = GATED ? 128 : 256;
   const int64_t pair_tiles = static_cast<int64_t>((a.channels + channels - 1) / channels) *
                              ((a.tokens + kPairTokens - 1) / kPairTokens);
   if (a.tokens > 128 && 4 * pair_tiles >= device_info(device).num_sms) return launch_pair<GATED, O>(a, device, stream);
-  // Narrow token tiles make more CTAs, wide ones load the weight less often (200 tokens of a 4000 x 4000 weight, 98 MB
-  // of loads at 64: 13.2 us, at 128 15.1 us; 256 tokens of 17408 columns to 5120 channels, 522 MB: 52 and 33 us).
+  // Narrow token tiles make more CTAs, wide ones load the weight less often (200 tokens of a 4000 x 4000 weight, 101 MB
+  // of loads at 64: 13.4 us, at 128 17.8 us; 256 tokens of 9000 columns to 2560 channels, 140 MB: 24.1 and 20.4; of
+  // 17408 to 5120, 535 MB: 43.5 and 33.5).  The number of CTAs counts as well: 100 tokens of 6000 x 6000, 109 MB, 22.1
+  // and 18.2.
   if (stream_loads(a, GATED, 64) <= (128 << 20)) return launch_stream<GATED, O, 64, 4>(a, device, stream);
   return launch_stream<GATED, O, 128, 3>(a, device, stream);
 }

@@ -32,7 +32,7 @@ def int8_of_products(u):
 
 
 def rows_with_ties(rows, hidden, dtype, weight_dtype, seed):
-    """Rows and weights whose products reach half of the largest one in many places, by factors of other significands."""
+    """Rows and weights whose products are half of the largest one in many places, by factors of other significands."""
     x = make((rows, hidden), dtype, seed, 0.3).clamp(-1.5, 1.5)
     w = make(hidden, weight_dtype, seed + 1, 0.1, 1.0).clamp(0.5, 1.5)
     big_x = (3.0 + 0.5 * torch.rand(rows, 1, generator=torch.Generator().manual_seed(seed + 2))).to(BF16)
@@ -148,7 +148,8 @@ def test_tangents_are_refused():
         for call in (lambda: norm(dual_x), lambda: norm(dual_x, quantize=True), lambda: quantize_rows(dual_x),
                      lambda: BlockNorm(dual_weight)(x), lambda: BlockNorm(weight, dual_weight)(x),
                      lambda: residual_norm(dual_x, x), lambda: residual_norm(x, dual_x),
-                     lambda: residual_norm(x, x, gate=dual_gate), lambda: residual_norm(x, x, post=BlockNorm(dual_weight)),
+                     lambda: residual_norm(x, x, gate=dual_gate),
+                     lambda: residual_norm(x, x, post=BlockNorm(dual_weight)),
                      lambda: int8_linear(xq, dual_xs, wq, ws), lambda: int8_linear(xq, xs, wq, dual_ws),
                      lambda: int8_linear(xq, xs, wq, ws, bias=dual_bias),
                      lambda: int8_gated_linear(xq, dual_xs, wq, ws)):
@@ -288,7 +289,8 @@ def test_overlaps_are_refused_unless_an_output_is_an_input(hidden):
         got = residual_norm(*pair, next_norm=norm, residual_out=None if r_out is None else pair[r_out],
                             out=None if x_out is None else pair[x_out])
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
-    for call in (lambda: norm(x, out=behind), lambda: norm(behind, out=x), lambda: norm(wide[:, 1:hidden + 1], out=left),
+    for call in (lambda: norm(x, out=behind), lambda: norm(behind, out=x),
+                 lambda: norm(wide[:, 1:hidden + 1], out=left),
                  lambda: residual_norm(x, residual, residual_out=behind),
                  lambda: residual_norm(residual, x, next_norm=norm, out=behind),
                  lambda: residual_norm(x, residual, next_norm=norm, residual_out=other, out=other),

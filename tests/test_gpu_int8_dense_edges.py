@@ -172,8 +172,8 @@ def test_outputs_beyond_2_to_the_31_elements():
     check_linear(y[-70:], product64(xq[-70:], xs[-70:], wq, ws))
     assert not bool(y[:-70].any())
     with pytest.raises(ValueError, match="tokens"):
-        int8_linear(torch.zeros((tokens + 1, 16), dtype=torch.int8, device="cuda"), torch.zeros(tokens + 1, device="cuda"),
-                    wq[:, :16], ws)
+        int8_linear(torch.zeros((tokens + 1, 16), dtype=torch.int8, device="cuda"),
+                    torch.zeros(tokens + 1, device="cuda"), wq[:, :16], ws)
     del y
     both = product64(xq[-70:], xs[-70:], wq, ws)
     h = int8_gated_linear(xq, xs, wq, ws)
