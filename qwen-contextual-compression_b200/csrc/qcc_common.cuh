@@ -87,11 +87,11 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 
 // The bounded wait for threads that have nothing else to do: each try lets the
 // hardware suspend the thread (for up to 100 us, and not beyond the limit), so
-// that waiting warps leave the issue slots to the working ones.  LOOK_FIRST,
-// for barriers that are mostly complete, begins with a look that never
-// suspends, after which a limit of 0 gives up (fewer registers); otherwise the
-// clock is read after a first try (its read before one costs the int8 products
-// 3 to 9 %, and a branch on the limit 1 %).
+// that waiting warps leave the issue slots to the working ones.  The clock is
+// read after a first try (its read before one costs the int8 products 3 to
+// 9 %).  LOOK_FIRST, for barriers that are mostly complete, begins with a look
+// that never suspends, after which a limit of 0 gives up; a branch on the limit
+// costs the products 1 %.
 template <bool LOOK_FIRST = false>
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   const uint32_t hint = LOOK_FIRST || limit_ns > 100000u ? 100000u : static_cast<uint32_t>(limit_ns);
@@ -109,9 +109,8 @@ __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t pari
   if (LOOK_FIRST) {
     if (mbar_test(bar, parity)) return true;
     if (limit_ns == 0) return false;
-  } else if (attempt()) {
-    return true;
   }
+  if (attempt()) return true;
   const uint64_t start = global_timer_ns();
   while (true) {
     if (attempt()) return true;

@@ -1,11 +1,14 @@
 """The 8-bit integer products where they can go wrong: waits that run out, and every kernel over several tiles."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
 import conftest  # noqa: F401
 from qcc_b200 import _lib
+from qcc_b200.runtime.block_norm import BlockNorm, residual_norm
 from qcc_b200.runtime.int8_dense import Int8GatedFFN, int8_gated_linear, int8_linear, quantize_rows
 from test_gpu_int8_dense import check_gated, check_linear, operands, product64
 
@@ -178,3 +181,49 @@ def test_outputs_beyond_2_to_the_31_elements():
     both = product64(xq[-70:], xs[-70:], wq, ws)
     h = int8_gated_linear(xq, xs, wq, ws)
     check_gated(h[-70:], both[:, :rows // 2], both[:, rows // 2:])
+
+
+def test_threads_share_norms_and_layers():
+    """Two threads on streams of their own call the same norm and the same layer at once, eagerly and replaying graphs."""
+    hidden, inner = 512, 1200
+    gen = torch.Generator().manual_seed(0)
+
+    def make(*shape, scale=1.0):
+        return (torch.randn(shape, generator=gen) * scale).to(BF16).cuda()
+
+    norm = BlockNorm(1 + make(hidden, scale=0.1))
+    ffn = Int8GatedFFN.from_weights(make(inner, hidden, scale=0.06), make(inner, hidden, scale=0.06),
+                                    make(hidden, inner, scale=0.04))
+    inputs = [make(t, hidden) for t in (3, 700)]
+
+    def step(x):
+        return residual_norm(ffn(norm(x, quantize=True), out_dtype=BF16), x, next_norm=norm)
+
+    want = [step(x) for x in inputs]
+    graphs, captured = [], []
+    for x in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.append(step(x))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for k in range(30):
+                r, x = step(inputs[i])
+                graphs[i].replay()
+                stream.synchronize()
+                for got in ((r, x), captured[i]):
+                    if not (torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1])):
+                        wrong.append((i, k))
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
