@@ -184,7 +184,7 @@ def test_outputs_beyond_2_to_the_31_elements():
 
 
 def test_threads_share_norms_and_layers():
-    """Two threads on streams of their own call the same norm and the same layer at once, eagerly and replaying graphs."""
+    """Two threads on streams of their own call one norm and one layer at the same time, eagerly and replaying graphs."""
     hidden, inner = 512, 1200
     gen = torch.Generator().manual_seed(0)
 
