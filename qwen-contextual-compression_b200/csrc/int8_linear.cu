@@ -375,9 +375,9 @@ __global__ void __launch_bounds__(128)
 // two single CTAs would.
 // Measured at 4096 tokens: gate|up 34816 x 5120 454 us (3.2 POP/s), down 5120 x
 // 17408 230 us (3.2 POP/s; 320 tiles are 4.3 rounds of 74 pairs).  In runs of
-// seconds, with the launches before them, 561 and 309 us: the card sits at its
-// 1000 W then, as in cuBLAS's bf16 product (1.4 PFLOP/s sustained): power
-// bounds it.
+// seconds, with the launches before them, 561 to 593 and 309 to 329 us: the
+// card sits at its 1000 W then, as in cuBLAS's bf16 product (1.4 PFLOP/s
+// sustained): power bounds it.
 // ---------------------------------------------------------------------------
 
 constexpr int kPairStages = 6;
